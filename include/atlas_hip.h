@@ -852,6 +852,66 @@ int atlas_eval_reduction_verify(const atlas_fr_t *points, const atlas_fr_t *clai
 int atlas_verify_graph(atlas_graph_t g, const atlas_hyperkzg_vk_t *vk, const int32_t *const *inputs, size_t n_inputs, const int32_t *output,
                        size_t output_len, const uint8_t *proof, size_t proof_len, atlas_transcript_t *final_transcript);
 
+/* ---- quantised attention for generation: the answer of a model before it is proved ------------------------------------------------
+ * The attention of a model graph — Einsum (mbk,nbk->bmn), Mul by a constant, Iff with the causal mask, SoftmaxLastAxis, Einsum
+ * (bmk,kbn->mbn), all at scale 2^14 — as one operator, without the graph's [heads, seq, seq] tensors, over packed prompts and token by
+ * token over a paged cache of keys and values.  Integers throughout, so that a row comes out bit for bit as the traced graph (the one
+ * atlas_prove_graph proves) has it, in whatever pieces the keys are visited:
+ *     s = clamp((sum_d q k) >> 14);  s = clamp((s score_mul) >> 14);  z = min(max_j s - s, 2^18 - 1);
+ *     e = (HI[z >> 9] LO[z & 511]) >> 14;  w = 2^28 / sum_j e;  p = (e w) >> 14;  out = clamp((sum_j p v) >> 14)
+ * with the digit tables of SoftmaxLastAxis (atlas-onnx-tracer/src/ops/softmax.rs:74-269), floor shifts and clamps to 32 bits
+ * (ops/einsum.rs:34-213).  Masked keys carry no weight (a graph whose mask fill lies 2^18 or more below every row's maximum); a row that
+ * sees no key is 0.  Any int32 value is computed exactly (sums wrap modulo 2^64, as the graph's do); operands below 2^19 in magnitude take the fast path.
+ *
+ * These entry points enqueue and return: no allocation, no wait, no state between calls, so they can be captured into HIP graphs.  `stream` is the
+ * caller's hipStream_t; NULL = the library stream, ATLAS_STREAM_DEFAULT = HIP's default stream.  Lengths, tables and slots are read on the
+ * device when the launches run.  All pointers are device memory of the calling thread's device (atlas_init / atlas_init_thread).  A workspace
+ * (16-byte aligned) belongs to one call in flight: two streams, or two captured graphs that may run at once, need one each. */
+#define ATLAS_STREAM_DEFAULT ((void *)1)
+typedef struct {
+    size_t n_heads, n_kv_heads;   /* head h reads the keys and values of head h / (n_heads / n_kv_heads); at most 1024 heads */
+    size_t head_dim;              /* 1 .. 256 */
+    int32_t score_mul;            /* the Mul node's constant at scale 2^14, 1 .. 2^14 (2^14: no scaling; 2^14 / sqrt(head_dim) rounded: the usual) */
+    int32_t causal;               /* 1: a token sees the keys up to its own; 0: all keys of its sequence */
+} atlas_attn_shape_t;
+/* int32 rows [token][head][head_dim]: element (t, h, i) at d[t * token_stride + h * head_stride + i] (slices of a fused projection fit) */
+typedef struct { int32_t *d; size_t token_stride, head_stride; } atlas_attn_rows_t;
+/* a paged cache of one layer: k and v [n_blocks][n_kv_heads][block_size][head_dim], int32 (bits = 32) or int16 (bits = 16);
+ * block_size a power of two, at most 4096 */
+typedef struct { void *d_k, *d_v; size_t n_blocks, block_size; int32_t bits; } atlas_kv_cache_t;
+
+/* Attention over packed prompts: sequence i is the rows [cu_seqlens[i], cu_seqlens[i + 1]) of q, k, v and out (n_seqs + 1 ascending offsets from 0, at most
+ * n_tokens).  Rows from cu_seqlens[n_seqs] on are neither read nor written.  out may not overlap q, k or v. */
+size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t *shape, size_t n_seqs, size_t n_tokens);
+int atlas_attn_prompt(const atlas_attn_shape_t *shape, const atlas_attn_rows_t *q, const atlas_attn_rows_t *k, const atlas_attn_rows_t *v,
+                      const int32_t *d_cu_seqlens, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t *out, void *d_workspace, size_t workspace_bytes,
+                      void *stream);
+/* Attention of new tokens over a paged cache that already holds their keys and values (atlas_kv_write): sequence i has the rows
+ * [cu_new[i], cu_new[i + 1]) of q and out (one row: a decoding step; none: a request that pauses), they are the last of its kv_lens[i] keys; key j
+ * lies in block block_table[i * table_stride + j / block_size] at j % block_size.  max_blocks columns of the table are looked at: keys beyond
+ * max_blocks * block_size do not exist, nor do those of a block outside [0, n_blocks). */
+size_t atlas_attn_cached_workspace(const atlas_attn_shape_t *shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t *cache, size_t max_blocks);
+int atlas_attn_cached(const atlas_attn_shape_t *shape, const atlas_attn_rows_t *q, const int32_t *d_cu_new, const int32_t *d_kv_lens, size_t n_seqs, size_t n_tokens,
+                      const atlas_kv_cache_t *cache, const int32_t *d_block_table, size_t max_blocks, size_t table_stride, const atlas_attn_rows_t *out,
+                      void *d_workspace, size_t workspace_bytes, void *stream);
+/* Keys and values of n_tokens rows into the slots of a cache (slot = block * block_size + place in the block; a negative slot: the row is skipped).  Slots are
+ * distinct: rows that share one leave a mixture.  *d_status (optional, the caller clears it) gets ATLAS_KV_NARROW when a value did not fit a
+ * 16-bit cache (its nearest 16-bit value is stored: what follows is not the graph's answer) and ATLAS_KV_BAD_SLOT for a slot behind the cache (skipped). */
+enum { ATLAS_KV_NARROW = 1, ATLAS_KV_BAD_SLOT = 2 };
+int atlas_kv_write(const atlas_attn_shape_t *shape, const atlas_attn_rows_t *k, const atlas_attn_rows_t *v, const int64_t *d_slots, size_t n_tokens,
+                   const atlas_kv_cache_t *cache, uint32_t *d_status, void *stream);
+/* The paging of one step, from request lengths alone: request i has cached_lens[i] tokens in the cache and brings new_lens[i] (-1: it has ended).  free_blocks is a
+ * stack of n_free[0] block ids (room for n_blocks).  First the blocks of ended requests go onto the stack (by request, then by position), then each
+ * request takes the blocks it lacks off its top into block_table[i * table_stride + ..] (table rows of ended requests are left as they are).  Written:
+ * n_free_out (may be n_free), cu_new (n_seqs + 1) and kv_lens for atlas_attn_cached, slots (for atlas_kv_write) and positions (optional) of the new
+ * tokens, in the order of requests; from cu_new[n_seqs] up to max_tokens slots are -1 and positions 0.  *d_status is 0, or the reason why the step does
+ * not fit: then nothing is taken or given back, n_free_out is n_free, cu_new is 0 throughout, kv_lens has the cached lengths and all slots are -1. */
+enum { ATLAS_KV_NO_BLOCKS = 1, ATLAS_KV_NO_COLUMNS = 2, ATLAS_KV_NO_TOKENS = 4, ATLAS_KV_BAD_LENGTH = 8 };
+size_t atlas_kv_plan_workspace(size_t n_seqs, size_t max_tokens);
+int atlas_kv_plan(size_t block_size, size_t n_blocks, const int32_t *d_cached_lens, const int32_t *d_new_lens, size_t n_seqs, int32_t *d_block_table, size_t max_blocks,
+                  size_t table_stride, int32_t *d_free_blocks, const int32_t *d_n_free, int32_t *d_n_free_out, int32_t *d_cu_new, int32_t *d_kv_lens, int64_t *d_slots,
+                  int32_t *d_positions, size_t max_tokens, uint32_t *d_status, void *d_workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,84 @@
+// Quantised attention for generation (include/atlas_hip.h: atlas_attn_*, atlas_kv_write): the attention of a model graph in the graph executor's integers, over packed
+// prompts and over a paged cache.  Mathematics at the kernels (attention_kernels.hip.h).
+#include "runtime.hpp"
+
+#include "attention_kernels.hip.h"
+#include "attention_launch.hpp"
+
+namespace {
+
+using namespace atlas_attn;
+
+Rows rows_of(const atlas_attn_rows_t* r) { return Rows{r->d, (int64_t)r->token_stride, (int64_t)r->head_stride}; }
+Args args_of(const atlas_attn_shape_t* s, const atlas_attn_rows_t* q, const int32_t* cu, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t* out) {
+    Args A{};
+    A.q = rows_of(q); A.out = rows_of(out);
+    A.cu = cu; A.n_seqs = (uint32_t)n_seqs; A.n_tokens = (uint32_t)n_tokens;
+    A.H = (uint32_t)s->n_heads; A.KV = (uint32_t)s->n_kv_heads; A.G = A.H / A.KV; A.d = (uint32_t)s->head_dim;
+    A.mul = s->score_mul; A.causal = s->causal;
+    return A;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens) {
+    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens)) return 0;
+    return 16;
+}
+
+int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
+                      const int32_t* d_cu_seqlens, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t* out, void* d_workspace, size_t workspace_bytes,
+                      void* stream) {
+    const char* why = bad_shape(shape);
+    if (!why) why = bad_sizes(n_seqs, n_tokens);
+    if (!why) why = bad_rows(q, n_tokens, shape->n_heads, shape->head_dim);
+    if (!why) why = bad_rows(k, n_tokens, shape->n_kv_heads, shape->head_dim);
+    if (!why) why = bad_rows(v, n_tokens, shape->n_kv_heads, shape->head_dim);
+    if (!why) why = bad_rows(out, n_tokens, shape->n_heads, shape->head_dim);
+    if (!why) why = bad_out(out, n_tokens, shape->n_heads, shape->head_dim);
+    if (!why && !d_cu_seqlens) why = "attn_prompt: cu_seqlens is null";
+    if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_attn_prompt_workspace(shape, n_seqs, n_tokens))) why = "attn_prompt: workspace is null, unaligned or too small";
+    if (why) return fail(ATLAS_EINVAL, why);
+    if (!n_seqs || !n_tokens) return ATLAS_OK;
+    Launch L;
+    if (int rc = L.begin(stream)) return rc;
+    if (int rc = L.on_device({q->d, k->d, v->d, d_cu_seqlens, out->d, d_workspace})) return rc;
+    Args A = args_of(shape, q, d_cu_seqlens, n_seqs, n_tokens, out);
+    A.k = rows_of(k); A.v = rows_of(v);
+    atlas_attn::k_attn_exact<int32_t><<<dim3((unsigned)n_tokens, A.H), 256, 0, L.stream>>>(A);
+    return L.end();
+}
+
+size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
+    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
+    return 16;
+}
+
+int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const int32_t* d_cu_new, const int32_t* d_kv_lens, size_t n_seqs, size_t n_tokens,
+                      const atlas_kv_cache_t* cache, const int32_t* d_block_table, size_t max_blocks, size_t table_stride, const atlas_attn_rows_t* out,
+                      void* d_workspace, size_t workspace_bytes, void* stream) {
+    const char* why = bad_shape(shape);
+    if (!why) why = bad_sizes(n_seqs, n_tokens);
+    if (!why) why = bad_rows(q, n_tokens, shape->n_heads, shape->head_dim);
+    if (!why) why = bad_rows(out, n_tokens, shape->n_heads, shape->head_dim);
+    if (!why) why = bad_out(out, n_tokens, shape->n_heads, shape->head_dim);
+    if (!why) why = bad_cache(cache);
+    if (!why && (!d_cu_new || !d_kv_lens || !d_block_table)) why = "attn_cached: cu_new, kv_lens or block_table is null";
+    if (!why && (max_blocks > 0x7fffffff / cache->block_size || table_stride < max_blocks || table_stride > 0x7fffffff)) why = "attn_cached: table_stride must be at least max_blocks, the keys of a row below 2^31";
+    if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_attn_cached_workspace(shape, n_seqs, n_tokens, cache, max_blocks))) why = "attn_cached: workspace is null, unaligned or too small";
+    if (why) return fail(ATLAS_EINVAL, why);
+    if (!n_seqs || !n_tokens) return ATLAS_OK;
+    Launch L;
+    if (int rc = L.begin(stream)) return rc;
+    if (int rc = L.on_device({q->d, d_cu_new, d_kv_lens, cache->d_k, cache->d_v, d_block_table, out->d, d_workspace})) return rc;
+    Args A = args_of(shape, q, d_cu_new, n_seqs, n_tokens, out);
+    A.ck = cache->d_k; A.cv = cache->d_v; A.lens = d_kv_lens; A.table = d_block_table; A.table_stride = (int64_t)table_stride;
+    A.n_blocks = (uint32_t)cache->n_blocks; A.log_block = log2_of(cache->block_size); A.max_keys = (uint32_t)(max_blocks * cache->block_size);
+    if (cache->bits == 16) atlas_attn::k_attn_exact<int16_t><<<dim3((unsigned)n_tokens, A.H), 256, 0, L.stream>>>(A);
+    else atlas_attn::k_attn_exact<int32_t><<<dim3((unsigned)n_tokens, A.H), 256, 0, L.stream>>>(A);
+    return L.end();
+}
+
+}  // extern "C"

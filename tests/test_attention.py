@@ -1,0 +1,180 @@
+"""CPU: the exp tables compiled into the attention kernels are the graph executor's, and every refusal of the attention and paging entry points answers on
+the host before anything touches a device."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_exp_tables_are_the_graph_executors(tmp_path):
+    from _attention_ref import exp_tables
+    src = tmp_path / "t.cpp"
+    src.write_text('#include "%s/jolt-atlas_amd/csrc/exp_table.hpp"\n#include <cstdio>\nint main() { constexpr auto t = atlas::make_exp_table();\n'
+                   'for (int v : t.hi) printf("%%d\\n", v);\nfor (int v : t.lo) printf("%%d\\n", v);\n}' % ROOT)
+    subprocess.check_call(["g++", "-std=c++17", str(src), "-o", str(tmp_path / "t")])
+    got = np.array([int(x) for x in subprocess.check_output([str(tmp_path / "t")], text=True).split()])
+    hi, lo = exp_tables()
+    assert np.array_equal(got[:512], hi) and np.array_equal(got[512:], lo)
+
+
+def test_the_reference_is_the_graph_operators():
+    """tests/_attention_ref.py against the oracle executor's operator chain: Einsum, Mul, Iff, SoftmaxLastAxis, Einsum"""
+    from _attention_ref import prompt
+    from oracle import graph as OG
+    nodes, q, k, v = chain(4, 16, 8, 3, 2896)
+    out, _ = OG.execute(nodes, [q, k, v])
+    got = prompt(q.reshape(16, 4, 8), k.reshape(16, 4, 8), v.reshape(16, 4, 8), [16], 2896)
+    assert np.array_equal(out[nodes[-1]["idx"]].reshape(16, 4, 8), got)
+
+
+def chain(heads, seq, hd, seed, score_mul, sigma=1.0):
+    """the attention of a model graph, its mask filled far below every score"""
+    rng = np.random.default_rng(seed)
+    q, k, v = (np.clip(np.round(rng.normal(0, sigma * (1 << 14), seq * heads * hd)), -(1 << 18), (1 << 18) - 1).astype(np.int32) for _ in range(3))
+    full = lambda x: np.full(heads * seq * seq, x, dtype=np.int32)  # noqa: E731
+    mask = np.broadcast_to(np.tril(np.ones((seq, seq), np.int32)), (heads, seq, seq)).reshape(-1)
+    dims = [heads, seq, seq]
+    nodes = [{"op": "Input", "inputs": [], "dims": [seq, heads, hd]}] * 3 + [
+        {"op": "Einsum", "inputs": [0, 1], "dims": dims, "layout": "mbk,nbk->bmn", "scale": 14, "shape": [heads, seq, hd, seq]},
+        {"op": "Constant", "inputs": [], "dims": dims, "data": full(score_mul)},
+        {"op": "Mul", "inputs": [3, 4], "dims": dims, "scale": 14},
+        {"op": "Constant", "inputs": [], "dims": dims, "data": mask},
+        {"op": "Constant", "inputs": [], "dims": dims, "data": full(-(1 << 27))},
+        {"op": "Iff", "inputs": [6, 5, 7], "dims": dims},
+        {"op": "SoftmaxLastAxis", "inputs": [8], "dims": dims, "scale": 14},
+        {"op": "Einsum", "inputs": [9, 2], "dims": [seq, heads, hd], "layout": "bmk,kbn->mbn", "scale": 14, "shape": [heads, seq, seq, hd]}]
+    return [dict(nd, idx=i) for i, nd in enumerate(nodes)], q, k, v
+
+
+class Fake:
+    """a tensor's shape with an address that nothing may look at"""
+
+    def __init__(self, shape, dtype="int32", strides=None, ptr=1 << 40):
+        self.shape, self.dtype, self.ptr = tuple(shape), np.dtype(dtype), ptr
+        self.itemsize = self.dtype.itemsize
+        self._s = tuple(strides) if strides else tuple(int(np.prod(shape[i + 1:])) for i in range(len(shape)))
+
+    def data_ptr(self):
+        return self.ptr
+
+    def stride(self):
+        return self._s
+
+
+def _prompt(**kw):
+    import jolt_atlas_amd.attention as T
+    a = dict(heads=4, kv=2, dim=8, mul=1 << 14, q=Fake((5, 4, 8)), k=Fake((5, 2, 8)), v=Fake((5, 2, 8)), cu=Fake((3,)), out=Fake((5, 4, 8)), ws=Fake((1 << 22,), "uint8"))
+    a.update(kw)
+    at = T.Attention(a["heads"], a["kv"], a["dim"], a["mul"])
+    at.prompt(a["q"], a["k"], a["v"], a["cu"], a["out"], a["ws"])
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(heads=4, kv=3, k=Fake((5, 3, 8)), v=Fake((5, 3, 8))), "must divide"),
+    (dict(heads=0, q=Fake((5, 0, 8)), out=Fake((5, 0, 8))), "must divide"),
+    (dict(dim=257, q=Fake((5, 4, 257)), k=Fake((5, 2, 257)), v=Fake((5, 2, 257)), out=Fake((5, 4, 257))), "head_dim"),
+    (dict(mul=0), "score_mul"), (dict(mul=(1 << 14) + 1), "score_mul"), (dict(mul=-5), "score_mul"),
+    (dict(q=Fake((5, 4, 8), strides=(32, 4, 1))), "strides"),
+    (dict(out=Fake((5, 4, 8), strides=(8, 8, 1))), "overlap"),
+    (dict(out=Fake((5, 4, 8), strides=(0, 8, 1))), "strides"),
+    (dict(q=Fake((5, 4, 8), ptr=(1 << 40) + 2)), "aligned"),
+    (dict(ws=Fake((8,), "uint8")), "workspace"),
+    (dict(ws=Fake((1 << 22,), "uint8", ptr=(1 << 40) + 8)), "workspace"),
+    (dict(cu=Fake((3,), ptr=0)), "cu_seqlens"),
+    (dict(v=Fake((5, 2, 8), ptr=0)), "null"),
+])
+def test_prompt_refusals(kw, why):
+    import jolt_atlas_amd as A
+    with pytest.raises(A.AtlasError, match=why):
+        _prompt(**kw)
+
+
+@pytest.mark.parametrize("kw", [dict(q=Fake((5, 4, 8), "int64")), dict(k=Fake((4, 2, 8))), dict(out=Fake((6, 4, 8))), dict(cu=Fake((0,))), dict(cu=Fake((3,), strides=(2,))),
+                                dict(q=Fake((5, 4, 8), strides=(64, 16, 2))), dict(v=Fake((5, 8)))])
+def test_prompt_refusals_of_the_wrapper(kw):
+    with pytest.raises(ValueError):
+        _prompt(**kw)
+
+
+def _cached(**kw):
+    import jolt_atlas_amd.attention as T
+    a = dict(q=Fake((3, 4, 8)), cu=Fake((3,)), lens=Fake((2,)), ck=Fake((7, 2, 16, 8)), cv=Fake((7, 2, 16, 8)), table=Fake((2, 5)), out=Fake((3, 4, 8)), ws=Fake((1 << 22,), "uint8"))
+    a.update(kw)
+    T.Attention(4, 2, 8).cached(a["q"], a["cu"], a["lens"], T.KVCache(a["ck"], a["cv"]), a["table"], a["out"], a["ws"])
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(ck=Fake((7, 2, 24, 8)), cv=Fake((7, 2, 24, 8))), "block_size"),
+    (dict(ck=Fake((7, 2, 8192, 8)), cv=Fake((7, 2, 8192, 8))), "block_size"),
+    (dict(ck=Fake((0, 2, 16, 8)), cv=Fake((0, 2, 16, 8))), "n_blocks"),
+    (dict(ck=Fake((7, 2, 16, 8), ptr=(1 << 40) + 2)), "alignment"),
+    (dict(cv=Fake((7, 2, 16, 8), ptr=0)), "null"),
+    (dict(lens=Fake((2,), ptr=0)), "null"),
+    (dict(table=Fake((2, 1 << 28))), "table_stride"),
+    (dict(ws=Fake((8,), "uint8")), "workspace"),
+])
+def test_cached_refusals(kw, why):
+    import jolt_atlas_amd as A
+    with pytest.raises(A.AtlasError, match=why):
+        _cached(**kw)
+
+
+@pytest.mark.parametrize("kw", [dict(ck=Fake((7, 2, 16, 8), "int16")), dict(ck=Fake((7, 2, 16, 8), "int64"), cv=Fake((7, 2, 16, 8), "int64")), dict(ck=Fake((7, 3, 16, 8)), cv=Fake((7, 3, 16, 8))),
+                                dict(table=Fake((1, 5))), dict(lens=Fake((1,))), dict(ck=Fake((7, 2, 16, 8), strides=(256, 8, 16, 1)))])
+def test_cached_refusals_of_the_wrapper(kw):
+    with pytest.raises(ValueError):
+        _cached(**kw)
+
+
+def _plan(block=16, n_blocks=9, **kw):
+    import jolt_atlas_amd.attention as T
+    a = dict(have=Fake((2,)), new=Fake((2,)), table=Fake((2, 5)), free=Fake((9,)), n_free=Fake((1,)), n_out=Fake((1,)), cu=Fake((3,)), lens=Fake((2,), ptr=1 << 41), slots=Fake((6,), "int64"),
+             pos=Fake((6,)), status=Fake((1,)), ws=Fake((1 << 12,), "uint8"))
+    a.update(kw)
+    T.Pager(block, n_blocks).plan(a["have"], a["new"], a["table"], a["free"], a["n_free"], a["n_out"], a["cu"], a["lens"], a["slots"], a["pos"], a["status"], a["ws"])
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(block=12), "block_size"), (dict(block=0), "block_size"), (dict(n_blocks=0), "n_blocks"), (dict(lens=Fake((2,))), "may not be"), (dict(ws=Fake((16,), "uint8")), "workspace"),
+    (dict(status=Fake((1,), ptr=0)), "null"), (dict(slots=Fake((6,), "int64", ptr=(1 << 40) + 4)), "aligned"), (dict(have=Fake((2,), ptr=0)), "null"),
+])
+def test_plan_refusals(kw, why):
+    import jolt_atlas_amd as A
+    with pytest.raises(A.AtlasError, match=why):
+        _plan(**kw)
+
+
+@pytest.mark.parametrize("kw", [dict(free=Fake((8,))), dict(table=Fake((1, 5))), dict(cu=Fake((2,))), dict(pos=Fake((5,))), dict(slots=Fake((6,))), dict(new=Fake((2,), "int64"))])
+def test_plan_refusals_of_the_wrapper(kw):
+    with pytest.raises(ValueError):
+        _plan(**kw)
+
+
+def test_write_refusals():
+    import jolt_atlas_amd as A
+    import jolt_atlas_amd.attention as T
+    cache = T.KVCache(Fake((7, 2, 16, 8)), Fake((7, 2, 16, 8)))
+    with pytest.raises(A.AtlasError, match="slots"):
+        cache.write(Fake((5, 2, 8)), Fake((5, 2, 8)), Fake((5,), "int64", ptr=0))
+    with pytest.raises(A.AtlasError, match="strides"):
+        cache.write(Fake((5, 2, 8)), Fake((5, 2, 8), strides=(16, 4, 1)), Fake((5,), "int64"))
+    for k, v, s in ((Fake((5, 2, 8)), Fake((4, 2, 8)), Fake((5,), "int64")), (Fake((5, 2, 8)), Fake((5, 2, 8)), Fake((4,), "int64")), (Fake((5, 2, 8)), Fake((5, 2, 8)), Fake((5,)))):
+        with pytest.raises(ValueError):
+            cache.write(k, v, s)
+
+
+def test_workspace_sizes():
+    import jolt_atlas_amd as A
+    import jolt_atlas_amd.attention as T
+    at = T.Attention(4, 2, 8)
+    cache = T.KVCache(Fake((7, 2, 16, 8)), Fake((7, 2, 16, 8)))
+    assert at.prompt_workspace_bytes(3, 100) > 0 and at.cached_workspace_bytes(3, 3, cache, 5) > 0
+    for bad in (lambda: at.prompt_workspace_bytes(1 << 25, 4), lambda: at.prompt_workspace_bytes(1, (1 << 30) + 1), lambda: T.Attention(4, 3, 8).prompt_workspace_bytes(1, 1),
+                lambda: at.cached_workspace_bytes(1, 1, cache, 1 << 28), lambda: T.Pager(16, 9).workspace_bytes(1 << 25, 4)):
+        with pytest.raises(A.AtlasError):
+            bad()
+    assert A.lib.atlas_attn_prompt_workspace(C.POINTER(T._Shape)(), 1, 1) == 0

@@ -1,0 +1,603 @@
+"""GPU: the quantised attention over packed prompts and over a paged cache, the cache write and the paging plan against their definitions in 64-bit integers.
+Everything is integers: results are equal, or wrong."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from _attention_ref import ONE, attend, plan, prompt
+from _dev import Dev, hip, ok, workspace
+
+pytestmark = pytest.mark.gpu
+MARK = 123456789
+
+
+def values(rng, shape, sigma=1.0):
+    """activations at scale 2^14, one channel in eight four times as large"""
+    x = rng.normal(0, sigma, shape)
+    x[..., ::8] *= 4
+    return np.clip(np.round(x * ONE), -(1 << 18), (1 << 18) - 1).astype(np.int32)
+
+
+def any_int32(rng, shape):
+    x = rng.integers(-(1 << 31), 1 << 31, size=shape, dtype=np.int64)
+    return np.where(rng.random(shape) < 0.1, rng.choice([-(1 << 31), (1 << 31) - 1, 0, -1, 1 << 23, -(1 << 23)], size=shape), x).astype(np.int32)
+
+
+def run_prompt(A, q, k, v, lens, mul=ONE, causal=True, rows=None, views=None):
+    """rows: the rows of the arrays (more than the sequences use); views: strided device views of q, k, v"""
+    import jolt_atlas_amd.attention as T
+    n, H, d = q.shape
+    at = T.Attention(H, k.shape[1], d, mul, causal)
+    cu = Dev(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+    out = Dev(np.full((n, H, d), MARK, np.int32))
+    ws = workspace(at.prompt_workspace_bytes(len(lens), n))
+    dq, dk, dv = views or (Dev(q), Dev(k), Dev(v))
+    assert at.prompt(dq, dk, dv, cu, out, ws) is out
+    return out.numpy()
+
+
+SHAPES = [(1, 1, 1), (4, 4, 4), (4, 4, 16), (4, 2, 20), (6, 2, 32), (5, 5, 33), (16, 16, 64), (8, 2, 64), (3, 1, 80), (8, 1, 96), (12, 4, 128), (7, 7, 100), (2, 1, 192), (3, 3, 256), (5, 1, 255)]
+
+
+@pytest.mark.parametrize("H,KV,d", SHAPES)
+def test_prompt(atlas, H, KV, d):
+    rng = np.random.default_rng(H * 1000 + d)
+    lens = [37, 0, 1, 64, 130, 5, 0, 33, 32, 31, 0]
+    n = sum(lens)
+    q, k, v = values(rng, (n, H, d)), values(rng, (n, KV, d)), values(rng, (n, KV, d))
+    mul = int(round(ONE / np.sqrt(d)))
+    got = run_prompt(atlas, q, k, v, lens, mul)
+    assert np.array_equal(got, prompt(q, k, v, lens, mul))
+
+
+@pytest.mark.parametrize("H,KV,d,n", [(2, 1, 64, 700), (2, 2, 128, 513), (1, 1, 16, 1025), (4, 1, 80, 300), (1, 1, 256, 290)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("mul", [ONE, 1448, 1])
+def test_prompt_longer(atlas, H, KV, d, n, causal, mul):
+    rng = np.random.default_rng(n)
+    lens = [n, 77]
+    N = sum(lens)
+    q, k, v = values(rng, (N, H, d), 0.4 if mul == ONE else 1.0), values(rng, (N, KV, d)), values(rng, (N, KV, d))
+    assert np.array_equal(run_prompt(atlas, q, k, v, lens, mul, causal), prompt(q, k, v, lens, mul, causal))
+
+
+@pytest.mark.parametrize("lens", [[1], [0], [0, 0, 0], [1, 1, 1, 1], [2, 3], [63], [64], [65], [127, 1], [128], [129], [1] * 300, [0] * 70 + [3] + [0] * 70])
+def test_prompt_lengths(atlas, lens):
+    rng = np.random.default_rng(len(lens))
+    n = sum(lens) + 3                       # rows behind the last sequence: neither read nor written
+    q, k, v = values(rng, (n, 4, 16)), values(rng, (n, 2, 16)), values(rng, (n, 2, 16))
+    got = run_prompt(atlas, q, k, v, lens, 4096)
+    assert np.array_equal(got[:n - 3], prompt(q[:n - 3], k[:n - 3], v[:n - 3], lens, 4096))
+    assert (got[n - 3:] == MARK).all()
+
+
+def test_prompt_without_rows_or_sequences(atlas):
+    import jolt_atlas_amd.attention as T
+    at = T.Attention(2, 1, 8)
+    e = lambda h: Dev(np.zeros((0, h, 8), np.int32))  # noqa: E731
+    at.prompt(e(2), e(1), e(1), Dev(np.zeros(4, np.int32)), e(2), workspace(at.prompt_workspace_bytes(3, 0)))
+    x = np.full((5, 2, 8), MARK, np.int32)
+    out = Dev(x)
+    at.prompt(Dev(x), Dev(x[:, :1]), Dev(x[:, :1]), Dev(np.zeros(1, np.int32)), out, workspace(at.prompt_workspace_bytes(0, 5)))
+    assert (out.numpy() == MARK).all()
+
+
+@pytest.mark.parametrize("H,KV,d,n", [(2, 1, 16, 70), (2, 2, 64, 40), (1, 1, 128, 130), (3, 1, 37, 33)])
+@pytest.mark.parametrize("kind", ["any", "edge", "wide_q", "wide_k", "wide_v", "large"])
+def test_prompt_of_any_int32(atlas, H, KV, d, n, kind):
+    """operands beyond what three signed bytes hold, sums that wrap, scores that clamp"""
+    rng = np.random.default_rng(d + n)
+    q, k, v = values(rng, (n, H, d)), values(rng, (n, KV, d)), values(rng, (n, KV, d))
+    if kind == "any":
+        q, k, v = any_int32(rng, q.shape), any_int32(rng, k.shape), any_int32(rng, v.shape)
+    elif kind == "edge":                     # the borders of three signed bytes
+        pick = lambda s: rng.choice([8355711, 8355712, -8421504, -8421505, 32639, 32640, -32896, 127, 128, -128, -129, 0], size=s).astype(np.int32)  # noqa: E731
+        q, k, v = pick(q.shape), pick(k.shape), pick(v.shape)
+    elif kind == "wide_q":
+        q[n // 2, 0, d // 2] = (1 << 31) - 1
+    elif kind == "wide_k":
+        k[3, -1, 0] = -(1 << 31)
+    elif kind == "wide_v":
+        v[n - 1, 0, d - 1] = (1 << 31) - 1
+    else:
+        q, k, v = q * 20, k * 20, v * 20
+    for mul in (ONE, 1448):
+        assert np.array_equal(run_prompt(atlas, q, k, v, [n], mul), prompt(q, k, v, [n], mul))
+
+
+def test_prompt_scores_that_are_equal_or_far_apart(atlas):
+    rng = np.random.default_rng(9)
+    n, d = 257, 64
+    q, k, v = values(rng, (n, 1, d)), np.zeros((n, 1, d), np.int32), values(rng, (n, 1, d))
+    assert np.array_equal(run_prompt(atlas, q, k, v, [n]), prompt(q, k, v, [n]))            # all weights alike
+    k[:] = values(rng, k.shape, 3.0)
+    assert np.array_equal(run_prompt(atlas, q, k, v, [n]), prompt(q, k, v, [n]))            # one key takes all
+    k[200:] = k[17]
+    assert np.array_equal(run_prompt(atlas, q, k, v, [n]), prompt(q, k, v, [n]))            # the maximum many times
+    v[:] = (1 << 22)
+    assert np.array_equal(run_prompt(atlas, q, k, v, [n], 512), prompt(q, k, v, [n], 512))
+
+
+@pytest.mark.parametrize("d,off", [(16, 0), (64, 1), (80, 3), (33, 2), (128, 1)])
+def test_prompt_strides(atlas, d, off):
+    """q, k, v as slices of one projection's output, at offsets that no vector load likes; out inside a larger array"""
+    import jolt_atlas_amd.attention as T
+    rng = np.random.default_rng(d)
+    H, KV, lens = 4, 2, [45, 0, 70]
+    n, width = sum(lens), (H + 2 * KV) * d + 7
+    row = values(rng, (n, width))
+    R = Dev(row)
+    view = lambda at, h: R.view(at, (n, h, d), (width, d, 1))  # noqa: E731
+    part = lambda at, h: row[:, at:at + h * d].reshape(n, h, d)  # noqa: E731
+    at = T.Attention(H, KV, d, 2048)
+    outer = Dev(np.full((H, n + 2, d + 5), MARK, np.int32))                                # heads outside of tokens
+    out = outer.view((d + 5) + off, (n, H, d), (d + 5, (n + 2) * (d + 5), 1))
+    at.prompt(view(off, H), view(off + H * d, KV), view(off + (H + KV) * d, KV), Dev(np.cumsum([0] + lens).astype(np.int32)), out, workspace(at.prompt_workspace_bytes(3, n)))
+    want = prompt(part(off, H), part(off + H * d, KV), part(off + (H + KV) * d, KV), lens, 2048)
+    full = np.full((H, n + 2, d + 5), MARK, np.int32)
+    full[:, 1:n + 1, off:off + d] = want.transpose(1, 0, 2)
+    assert np.array_equal(outer.numpy(), full)
+
+
+# ------------------------------------------------------------------------------------------------------------- paged cache
+def paged(rng, keys, KV, d, block, bits, spare=3, cols=None, sigma=None):
+    """caches with random blocks for sequences of `keys`, their table, and the sequences' own keys and values"""
+    up = [-(-k // block) for k in keys]
+    n_blocks = sum(up) + spare
+    dtype = np.int16 if bits == 16 else np.int32
+    sigma = sigma or (0.4 if bits == 16 else 1.0)
+    ck, cv = (np.clip(values(rng, (n_blocks, KV, block, d), sigma), -32768, 32767 if bits == 16 else 1 << 30).astype(dtype) for _ in range(2))
+    ids = rng.permutation(n_blocks).astype(np.int32)
+    table = np.full((len(keys), cols or max(up + [1])), -1, np.int32)
+    at = 0
+    for i, u in enumerate(up):
+        table[i, :u] = ids[at:at + u]
+        at += u
+    flat = lambda c, i: c[table[i, :up[i]]].transpose(0, 2, 1, 3).reshape(-1, KV, d)[:keys[i]]  # noqa: E731
+    return ck, cv, table, flat
+
+
+def run_cached(q, ck, cv, table, keys, new, mul=ONE, causal=True, table_view=None):
+    import jolt_atlas_amd.attention as T
+    n, H, d = q.shape
+    at = T.Attention(H, ck.shape[1], d, mul, causal)
+    cache = T.KVCache(Dev(ck), Dev(cv))
+    out = Dev(np.full(q.shape, MARK, np.int32))
+    tab = table_view or Dev(table)
+    ws = workspace(at.cached_workspace_bytes(len(new), n, cache, tab.shape[1]))
+    at.cached(Dev(q), Dev(np.cumsum([0] + list(new)).astype(np.int32)), Dev(np.array(keys, np.int32)), cache, tab, out, ws)
+    return out.numpy()
+
+
+def want_cached(q, ck, cv, table, flat, keys, new, mul=ONE, causal=True):
+    out, at = np.full(q.shape, MARK, np.int32), 0
+    for i, (m, n) in enumerate(zip(keys, new)):
+        lim = [max(0, min(m, m - n + j + 1)) if causal else m for j in range(n)]
+        out[at:at + n] = attend(q[at:at + n], flat(ck, i), flat(cv, i), lim, mul)
+        at += n
+    return out
+
+
+@pytest.mark.parametrize("H,KV,d", [(1, 1, 1), (4, 4, 16), (16, 16, 64), (8, 2, 128), (8, 1, 80), (32, 4, 64), (3, 1, 256), (5, 5, 33), (40, 1, 32)])
+@pytest.mark.parametrize("bits", [32, 16])
+@pytest.mark.parametrize("block", [1, 16, 64])
+def test_cached_single_tokens(atlas, H, KV, d, bits, block):
+    rng = np.random.default_rng(H * 100 + d + block)
+    keys = [1, 2, 31, 32, 33, 100, 257, 64, 5]
+    new = [1] * len(keys)
+    ck, cv, table, flat = paged(rng, keys, KV, d, block, bits)
+    q = values(rng, (len(keys), H, d))
+    mul = int(round(ONE / np.sqrt(d)))
+    assert np.array_equal(run_cached(q, ck, cv, table, keys, new, mul), want_cached(q, ck, cv, table, flat, keys, new, mul))
+
+
+@pytest.mark.parametrize("H,KV,d,bits,block", [(4, 4, 16, 32, 16), (8, 2, 128, 32, 32), (8, 2, 64, 16, 8), (6, 2, 100, 32, 64), (2, 1, 256, 16, 128), (16, 2, 33, 32, 4)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_cached_chunks(atlas, H, KV, d, bits, block, causal):
+    """several new tokens beside single ones, a request that pauses, a prompt without a past, more new tokens than keys (rows that see nothing)"""
+    rng = np.random.default_rng(d)
+    keys, new = [90, 200, 33, 70, 300, 4, 0, 1], [17, 1, 33, 0, 70, 9, 2, 1]
+    ck, cv, table, flat = paged(rng, keys, KV, d, block, bits)
+    q = values(rng, (sum(new), H, d))
+    mul = int(round(ONE / np.sqrt(d)))
+    assert np.array_equal(run_cached(q, ck, cv, table, keys, new, mul, causal), want_cached(q, ck, cv, table, flat, keys, new, mul, causal))
+
+
+@pytest.mark.parametrize("bits", [32, 16])
+@pytest.mark.parametrize("new", [[1, 1], [3, 40]])
+def test_cached_long(atlas, bits, new):
+    rng = np.random.default_rng(11)
+    keys = [9001, 4500]
+    ck, cv, table, flat = paged(rng, keys, 2, 64, 32, bits)
+    q = values(rng, (sum(new), 4, 64))
+    assert np.array_equal(run_cached(q, ck, cv, table, keys, new, 2048), want_cached(q, ck, cv, table, flat, keys, new, 2048))
+
+
+def test_cached_pages_that_do_not_exist(atlas):
+    """a table entry outside the cache holds no keys; keys behind the table's columns do not exist; lengths that make no sense give empty rows"""
+    rng = np.random.default_rng(3)
+    for new in ([1, 1, 1, 1], [2, 5, 40, 1]):
+        keys = [100, 90, 80, 64]
+        ck, cv, table, flat = paged(rng, keys, 2, 32, 16, 32)
+        bad = table.copy()
+        bad[0, 2], bad[1, 0], bad[2, :] = -7, ck.shape[0], 2 ** 31 - 1
+        q = values(rng, (sum(new), 4, 32))
+        want, at = np.zeros(q.shape, np.int32), 0
+        for i, (m, n) in enumerate(zip(keys, new)):
+            there = np.repeat((bad[i] >= 0) & (bad[i] < ck.shape[0]), 16)[:m]
+            lim = [there & (np.arange(m) < m - n + j + 1) for j in range(n)]
+            want[at:at + n] = attend(q[at:at + n], flat(ck, i), flat(cv, i), lim, 2896)
+            at += n
+        assert np.array_equal(run_cached(q, ck, cv, bad, keys, new, 2896), want)
+        # the table cut to 3 columns: 48 keys are left of each sequence
+        cut = Dev(table).view(0, (4, 3), (table.shape[1], 1))
+        short = [48] * 4
+        got = run_cached(q, ck, cv, None, keys, new, 2896, table_view=cut)
+        assert np.array_equal(got, want_cached(q, ck, cv, table, lambda c, i: flat(c, i)[:48], short, new, 2896))
+        assert (run_cached(q, ck, cv, table, [-5, 0, -(2 ** 31), 0], new, 2896) == 0).all()
+
+
+def test_cached_of_any_int32(atlas):
+    rng = np.random.default_rng(5)
+    for new in ([1, 1], [40, 3]):
+        keys = [130, 61]
+        ck, cv, table, flat = paged(rng, keys, 2, 64, 16, 32)
+        for spoil in ("q", "k", "v", "all"):
+            k2, v2, q = ck.copy(), cv.copy(), values(rng, (sum(new), 4, 64))
+            if spoil == "q":
+                q[0, 1, 5] = -(1 << 31)
+            if spoil == "k":
+                k2[table[0, 3], 1, 2, 63] = (1 << 31) - 1
+            if spoil == "v":
+                v2[table[0, 3], 1, 2, 63] = (1 << 31) - 1
+            if spoil == "all":
+                q, k2, v2 = any_int32(rng, q.shape), any_int32(rng, ck.shape), any_int32(rng, cv.shape)
+            assert np.array_equal(run_cached(q, k2, v2, table, keys, new, 2048), want_cached(q, k2, v2, table, flat, keys, new, 2048)), spoil
+        c16 = rng.choice([-32768, 32767, 32640, 32639, 0], size=ck.shape).astype(np.int16)
+        q = values(rng, (sum(new), 4, 64), 0.01)
+        assert np.array_equal(run_cached(q, c16, c16, table, keys, new), want_cached(q, c16, c16, table, flat, keys, new))
+
+
+def test_rows_behind_the_last_sequence_stay(atlas):
+    import jolt_atlas_amd.attention as T
+    rng = np.random.default_rng(8)
+    keys, new = [50, 20], [1, 1]
+    ck, cv, table, flat = paged(rng, keys, 2, 16, 16, 32)
+    q = values(rng, (6, 4, 16))
+    at = T.Attention(4, 2, 16)
+    cache = T.KVCache(Dev(ck), Dev(cv))
+    out = Dev(np.full(q.shape, MARK, np.int32))
+    at.cached(Dev(q), Dev(np.array([0, 1, 2], np.int32)), Dev(np.array(keys, np.int32)), cache, Dev(table), out, workspace(at.cached_workspace_bytes(2, 6, cache, table.shape[1])))
+    got = out.numpy()
+    assert (got[2:] == MARK).all() and np.array_equal(got[:2], want_cached(q[:2], ck, cv, table, flat, keys, new))
+
+
+def test_cached_offsets_past_32_bits(atlas):
+    """blocks whose elements lie beyond 2^32 elements of the cache: the allocation is never touched as a whole"""
+    import jolt_atlas_amd.attention as T
+    from _dev import Buffer
+    rng = np.random.default_rng(13)
+    KV, B, d = 8, 256, 256
+    n_blocks = (1 << 32) // (KV * B * d) + 40
+    size = n_blocks * KV * B * d
+    bufs = [Buffer(2 * size) for _ in range(2)]
+    one = values(rng, (2, KV, B, d), 0.4).clip(-32768, 32767).astype(np.int16)
+    last = n_blocks - 1
+    for b, x in zip(bufs, one):
+        ok(hip().hipMemcpy(C.c_void_p(b.p.value + 2 * last * KV * B * d), np.ascontiguousarray(x).ctypes.data_as(C.c_void_p), C.c_size_t(x.nbytes), C.c_int(1)))
+    views = []
+    for b in bufs:
+        v = Dev(np.empty(0, np.int16), b, 0, (n_blocks, KV, B, d), (KV * B * d, B * d, d, 1))
+        v.total = 0
+        views.append(v)
+    cache = T.KVCache(*views)
+    for new in (1, 40):
+        at = T.Attention(KV, KV, d, 1024)
+        q = values(rng, (new, KV, d))
+        out = Dev(np.full(q.shape, MARK, np.int32))
+        at.cached(Dev(q), Dev(np.array([0, new], np.int32)), Dev(np.array([200], np.int32)), cache, Dev(np.array([[last]], np.int32)), out, workspace(at.cached_workspace_bytes(1, new, cache, 1)))
+        k, v = (x.transpose(1, 0, 2)[:200] for x in one)
+        assert np.array_equal(out.numpy(), attend(q, k, v, [200 - new + j + 1 for j in range(new)], 1024))
+    # and the write
+    k, v = values(rng, (2, KV, d), 0.4), values(rng, (2, KV, d), 0.4)
+    cache.write(Dev(k), Dev(v), Dev(np.array([last * B + 255, last * B], np.int64)))
+    ok(hip().hipDeviceSynchronize())
+    for b, x, was in zip(bufs, (k, v), one):
+        got = np.empty((KV, B, d), np.int16)
+        ok(hip().hipMemcpy(got.ctypes.data_as(C.c_void_p), C.c_void_p(b.p.value + 2 * last * KV * B * d), C.c_size_t(got.nbytes), C.c_int(2)))
+        want = was.copy()
+        want[:, 255], want[:, 0] = x[0].clip(-32768, 32767), x[1].clip(-32768, 32767)
+        assert np.array_equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------------------------- write
+@pytest.mark.parametrize("d", [1, 4, 33, 64, 128, 255])
+@pytest.mark.parametrize("bits", [32, 16])
+@pytest.mark.parametrize("block", [1, 8, 64])
+def test_write(atlas, d, bits, block):
+    import jolt_atlas_amd.attention as T
+    rng = np.random.default_rng(d)
+    KV, n, n_blocks = 3, 50, 200 // block + 2
+    dtype = np.int16 if bits == 16 else np.int32
+    ck, cv = (rng.integers(-99, 99, size=(n_blocks, KV, block, d)).astype(dtype) for _ in range(2))
+    wide = any_int32 if bits == 32 else (lambda r, s: r.integers(-32768, 32768, size=s).astype(np.int32))
+    row = wide(rng, (n, 2 * KV, d + 3))
+    R = Dev(row)
+    k, v = (R.view(o * KV * (d + 3) + 1, (n, KV, d), (2 * KV * (d + 3), d + 3, 1)) for o in (0, 1))
+    hk, hv = row[:, :KV, 1:d + 1], row[:, KV:, 1:d + 1]
+    slots = rng.permutation(n_blocks * block)[:n].astype(np.int64)
+    slots[[3, 17]] = [-1, -(1 << 40)]
+    dk, dv, status = Dev(ck), Dev(cv), Dev(np.zeros(1, np.int32))
+    cache = T.KVCache(dk, dv)
+    cache.write(k, v, Dev(slots), status)
+    cache.write(k, v, Dev(slots))
+    for host, dev, src in ((ck, dk, hk), (cv, dv, hv)):
+        want = host.copy()
+        for i, s in enumerate(slots):
+            if s >= 0:
+                want[s // block, :, s % block] = src[i]
+        assert np.array_equal(dev.numpy(), want)
+    assert status.numpy()[0] == 0
+
+
+def test_write_tells(atlas):
+    import jolt_atlas_amd.attention as T
+    ck = np.zeros((2, 1, 4, 5), np.int16)
+    k = np.zeros((3, 1, 5), np.int32)
+    k[1, 0, 4], k[2, 0, 0] = 40000, -(1 << 31)
+    v = np.zeros((3, 1, 5), np.int32)
+    dk, dv, status = Dev(ck), Dev(ck), Dev(np.zeros(1, np.int32))
+    cache = T.KVCache(dk, dv)
+    cache.write(Dev(k), Dev(v), Dev(np.array([0, 1, 7], np.int64)), status)
+    assert status.numpy()[0] == T.NARROW
+    got = dk.numpy()
+    assert got[0, 0, 1, 4] == 32767 and got[1, 0, 3, 0] == -32768 and np.count_nonzero(got) == 2 and not dv.numpy().any()
+    status = Dev(np.array([16], np.int32))
+    cache.write(Dev(v), Dev(v), Dev(np.array([0, 8, 1 << 50], np.int64)), status)
+    assert status.numpy()[0] == 16 | T.BAD_SLOT
+
+
+# -------------------------------------------------------------------------------------------------------------------- plan
+def run_plan(have, new, table, free, n_free, block, n_blocks, cap, positions=True):
+    import jolt_atlas_amd.attention as T
+    P = T.Pager(block, n_blocks)
+    n = len(have)
+    i32 = lambda x: Dev(np.asarray(x, np.int32))  # noqa: E731
+    d = dict(table=Dev(table), free=Dev(free), n_free_out=i32([77]), cu=i32([77] * (n + 1)), lens=i32([77] * n), slots=Dev(np.full(cap, 77, np.int64)), positions=i32([77] * cap), status=i32([77]))
+    P.plan(i32(have), i32(new), d["table"], d["free"], i32([n_free]), d["n_free_out"], d["cu"], d["lens"], d["slots"], d["positions"] if positions else None, d["status"],
+           workspace(P.workspace_bytes(n, cap)))
+    return {k: x.numpy() for k, x in d.items()}
+
+
+def pool(rng, have, block, n_blocks, cols):
+    ids = rng.permutation(n_blocks).astype(np.int32)
+    table = np.full((len(have), cols), -1, np.int32)
+    at = 0
+    for i, c in enumerate(have):
+        u = -(-c // block)
+        table[i, :u] = ids[at:at + u]
+        at += u
+    free = np.full(n_blocks, -9, np.int32)
+    free[:n_blocks - at] = ids[at:]
+    return table, free, n_blocks - at
+
+
+@pytest.mark.parametrize("n,longest,new,block,cap", [(1, 10, 1, 16, 1), (64, 500, 1, 64, 64), (64, 500, 1, 16, 100), (5, 0, 30, 8, 150), (1500, 60, 3, 4, 5000), (300, 40, 90, 16, 30000), (2500, 9, 1, 1, 2500),
+                                                     (3, 4000, 5000, 4096, 15000)])
+def test_plan(atlas, n, longest, new, block, cap):
+    rng = np.random.default_rng(n)
+    have = rng.integers(0, longest + 1, size=n)
+    fresh = rng.integers(0, new + 1, size=n) if new > 1 else np.ones(n, int)
+    fresh[rng.random(n) < 0.1] = -1
+    cols = -(-(longest + new) // block) + 2
+    n_blocks = int(sum(-(-(h + max(f, 0)) // block) for h, f in zip(have, fresh))) + 5
+    table, free, n_free = pool(rng, have, block, n_blocks, cols)
+    got = run_plan(have, fresh, table, free, n_free, block, n_blocks, cap)
+    want = plan(list(have), list(fresh), table, free, n_free, block, n_blocks, cap)
+    for k in want:
+        assert np.array_equal(got[k], want[k]), k
+    assert got["status"][0] == 0
+
+
+@pytest.mark.parametrize("case", ["blocks", "columns", "tokens", "length", "ended_length", "stack", "stack_negative", "many_tokens", "exact_fit", "from_the_ended"])
+def test_plan_that_does_not_fit_changes_nothing(atlas, case):
+    rng = np.random.default_rng(1)
+    have, new, block, n_blocks, cap, cols = [10, 3, 17, 0], [4, 1, -1, 20], 4, 40, 30, 10
+    table, free, n_free = pool(rng, have, block, n_blocks, cols)
+    if case == "blocks":
+        free, n_free = np.full(n_blocks, 5, np.int32), 0
+        new[2] = 0
+    if case == "columns":
+        table = np.ascontiguousarray(table[:, :4])
+        have, new = [10, 3, 9, 0], [4, 1, -1, 20]
+    if case == "tokens":
+        cap = 24
+    if case == "many_tokens":
+        cap, new, cols = 5000, [4, 1, -1, 5000], 10
+    if case == "length":
+        have[1] = -1
+    if case == "ended_length":
+        new[0] = -2
+    if case == "stack":
+        n_free = n_blocks - 4
+    if case == "stack_negative":
+        n_free = -3
+    if case == "exact_fit":
+        cap, n_free, free = 25, 1, np.arange(n_blocks, dtype=np.int32)         # 5 given back + 1 = the 6 that are needed
+    if case == "from_the_ended":
+        n_free, new = 0, [2, 1, -1, 17]
+    got = run_plan(have, new, table, free, n_free, block, n_blocks, cap)
+    want = plan(have, new, table, free, n_free, block, n_blocks, cap)
+    for k in want:
+        assert np.array_equal(got[k], want[k]), (k, got[k], want[k])
+    assert (want["status"][0] == 0) == (case in ("exact_fit", "from_the_ended"))
+
+
+def test_plan_of_nothing(atlas):
+    got = run_plan([], [], np.zeros((1, 2), np.int32), np.arange(4, dtype=np.int32), 4, 8, 4, 3, positions=False)
+    assert got["status"][0] == 0 and got["cu"][0] == 0 and got["n_free_out"][0] == 4 and (got["slots"] == -1).all() and (got["positions"] == 77).all()
+
+
+# ---------------------------------------------------------------------------------------------------- together, and the graph
+def test_attention_is_the_traced_graphs(atlas):
+    """atlas_graph_trace of the operator chain (the one atlas_prove_graph proves), and the operators over its q, k, v: the prompt at once, and token by token"""
+    from jolt_atlas_amd import graph as GG
+    from test_attention import chain
+    import jolt_atlas_amd.attention as T
+    for heads, seq, hd, mul in ((4, 64, 16, 4096), (16, 32, 64, 2048), (2, 128, 8, 5793)):
+        nodes, q, k, v = chain(heads, seq, hd, seq, mul)
+        G = GG.Graph(nodes, [nodes[-1]["idx"]])
+        try:
+            G.trace([q, k, v])
+            want = G.node_output(nodes[-1]["idx"]).reshape(seq, heads, hd)
+        finally:
+            G.free()
+        q, k, v = (x.reshape(seq, heads, hd) for x in (q, k, v))
+        assert np.array_equal(run_prompt(atlas, q, k, v, [seq], mul), want)
+        cache = T.KVCache(Dev(np.zeros((seq // 8, heads, 8, hd), np.int32)), Dev(np.zeros((seq // 8, heads, 8, hd), np.int32)))
+        table = Dev(np.arange(seq // 8, dtype=np.int32)[::-1].reshape(1, -1).copy())
+        at = T.Attention(heads, heads, hd, mul)
+        ws = workspace(at.cached_workspace_bytes(1, 1, cache, seq // 8))
+        for t in range(seq):
+            slot = (seq // 8 - 1 - t // 8) * 8 + t % 8
+            cache.write(Dev(k[t:t + 1]), Dev(v[t:t + 1]), Dev(np.array([slot], np.int64)))
+            out = Dev(np.zeros((1, heads, hd), np.int32))
+            at.cached(Dev(q[t:t + 1]), Dev(np.array([0, 1], np.int32)), Dev(np.array([t + 1], np.int32)), cache, table, out, ws)
+            assert np.array_equal(out.numpy()[0], want[t]), t
+
+
+def test_a_serving_run(atlas):
+    """requests of different lengths through plan, write and cached attention over several steps — a prompt in one chunk, in pieces, token by token, one that ends
+    and one that starts in its blocks — equal to attention over each whole sequence"""
+    import jolt_atlas_amd.attention as T
+    rng = np.random.default_rng(21)
+    H, KV, d, B, n_blocks, cols, mul = 8, 2, 64, 8, 40, 16, 2048
+    total = [70, 33, 50, 61]
+    data = [tuple(values(rng, (t, h, d)) for h in (H, KV, KV)) for t in total]
+    whole = [prompt(q, k, v, [len(q)], mul) for q, k, v in data]
+    steps = [[40, 33, 0, 1], [1, -1, 7, 0], [1, 0, 20, 30], [28, 0, 1, 1], [0, 0, 22, 29]]
+    at, pager = T.Attention(H, KV, d, mul), T.Pager(B, n_blocks)
+    cap = 80
+    cache = T.KVCache(Dev(rng.integers(-9, 9, (n_blocks, KV, B, d)).astype(np.int32)), Dev(rng.integers(-9, 9, (n_blocks, KV, B, d)).astype(np.int32)))
+    i32 = lambda x: Dev(np.asarray(x, np.int32))  # noqa: E731
+    table, free, n_free = i32(np.full((4, cols), -1)), i32(rng.permutation(n_blocks)), i32([n_blocks])
+    cu, lens, slots, positions, status = i32([0] * 5), i32([0] * 4), Dev(np.zeros(cap, np.int64)), i32([0] * cap), i32([0])
+    wp, wa = workspace(pager.workspace_bytes(4, cap)), workspace(at.cached_workspace_bytes(4, cap, cache, cols))
+    have = [0] * 4
+    for step in steps:
+        pager.plan(i32(have), i32(step), table, free, n_free, n_free, cu, lens, slots, positions, status, wp)
+        rows = [np.zeros((cap, h, d), np.int32) for h in (H, KV, KV)]
+        at_row, want = 0, np.full((cap, H, d), MARK, np.int32)
+        for i, f in enumerate(step):
+            for x, src in zip(rows, data[i]):
+                x[at_row:at_row + max(f, 0)] = src[have[i]:have[i] + max(f, 0)]
+            want[at_row:at_row + max(f, 0)] = whole[i][have[i]:have[i] + max(f, 0)]
+            at_row += max(f, 0)
+            have[i] = 0 if f < 0 else have[i] + f
+        out = Dev(np.full((cap, H, d), MARK, np.int32))
+        cache.write(Dev(rows[1]), Dev(rows[2]), slots)
+        at.cached(Dev(rows[0]), cu, lens, cache, table, out, wa)
+        assert status.numpy()[0] == 0 and list(lens.numpy()) == have
+        assert np.array_equal(out.numpy(), want)
+    assert n_free.numpy()[0] == n_blocks - sum(-(-h // B) for h in have)
+
+
+def test_pointers_that_are_no_device_memory(atlas):
+    import jolt_atlas_amd.attention as T
+    at = T.Attention(1, 1, 4)
+    x = Dev(np.zeros((2, 1, 4), np.int32))
+    host = np.zeros((2, 1, 4), np.int32)
+    fake = Dev(np.empty(0, np.int32), x.buf, 0, (2, 1, 4), (4, 4, 1))
+    fake.data_ptr = lambda: host.ctypes.data
+    for a in ((fake, x, x, x), (x, fake, x, x), (x, x, fake, x), (x, x, x, fake)):
+        with pytest.raises(atlas.AtlasError, match="device"):
+            at.prompt(a[0], a[1], a[2], Dev(np.array([0, 2], np.int32)), a[3], workspace(at.prompt_workspace_bytes(1, 2)))
+
+
+def test_captured_and_replayed_on_two_streams(atlas):
+    """a step captured into two graphs on two streams (a workspace each), replayed over changed inputs, with eager calls between; each replay against the definition"""
+    import jolt_atlas_amd.attention as T
+    h = hip()
+    rng = np.random.default_rng(4)
+    H, KV, d, B = 4, 2, 64, 16
+    up = lambda dev, x: ok(h.hipMemcpy(dev.buf.p, np.ascontiguousarray(x).ctypes.data_as(C.c_void_p), C.c_size_t(x.nbytes), C.c_int(1)))  # noqa: E731
+    sides = []
+    for side in range(2):
+        keys, new = ([300, 41], [1, 1]) if side == 0 else ([90, 130], [20, 3])
+        ck, cv, table, flat = paged(rng, keys, KV, d, B, 32)
+        S = dict(keys=keys, new=new, table=table, ck=ck, cv=cv, flat=flat, at=T.Attention(H, KV, d, 2048), q=Dev(np.zeros((sum(new), H, d), np.int32)), k=Dev(np.zeros((sum(new), KV, d), np.int32)),
+                 v=Dev(np.zeros((sum(new), KV, d), np.int32)), out=Dev(np.zeros((sum(new), H, d), np.int32)), pout=Dev(np.zeros((sum(new), H, d), np.int32)), cache=T.KVCache(Dev(ck), Dev(cv)))
+        S["lens"], S["cu"], S["dtable"] = Dev(np.array(keys, np.int32)), Dev(np.cumsum([0] + new).astype(np.int32)), Dev(table)
+        slots = []
+        for i, (m, n) in enumerate(zip(keys, new)):
+            slots += [int(table[i, p // B]) * B + p % B for p in range(m - n, m)]
+        S["slots"], S["hslots"] = Dev(np.array(slots, np.int64)), slots
+        S["ws"] = workspace(S["at"].cached_workspace_bytes(2, sum(new), S["cache"], table.shape[1]))
+        S["pws"] = workspace(S["at"].prompt_workspace_bytes(2, sum(new)))
+        S["stream"] = C.c_void_p()
+        ok(h.hipStreamCreateWithFlags(C.byref(S["stream"]), C.c_uint(1)))
+        ok(h.hipDeviceSynchronize())
+        graph, S["exec"] = C.c_void_p(), C.c_void_p()
+        ok(h.hipStreamBeginCapture(S["stream"], C.c_int(0)))
+        step(S, S["stream"].value)
+        ok(h.hipStreamEndCapture(S["stream"], C.byref(graph)))
+        ok(h.hipGraphInstantiate(C.byref(S["exec"]), graph, None, None, C.c_size_t(0)))
+        ok(h.hipGraphDestroy(graph))
+        sides.append(S)
+    for rep in range(4):
+        for S in sides:
+            S["hq"], S["hk"], S["hv"] = values(rng, S["q"].shape), values(rng, S["k"].shape), values(rng, S["v"].shape)
+            up(S["q"], S["hq"]), up(S["k"], S["hk"]), up(S["v"], S["hv"])
+        ok(h.hipDeviceSynchronize())
+        for S in sides:
+            ok(h.hipGraphLaunch(S["exec"], S["stream"]))
+        if rep % 2:                          # eager work of the program's own, on the library stream, between the replays
+            x = values(rng, (40, H, d)), values(rng, (40, KV, d)), values(rng, (40, KV, d))
+            assert np.array_equal(run_prompt(atlas, *x, [40], 2048), prompt(*x, [40], 2048))
+        ok(h.hipDeviceSynchronize())
+        for S in sides:
+            for i, s in enumerate(S["hslots"]):
+                S["ck"][s // B, :, s % B], S["cv"][s // B, :, s % B] = S["hk"][i], S["hv"][i]
+            assert np.array_equal(S["out"].numpy(), want_cached(S["hq"], S["ck"], S["cv"], S["table"], S["flat"], S["keys"], S["new"], 2048)), rep
+            assert np.array_equal(S["pout"].numpy(), prompt(S["hq"], S["hk"], S["hv"], S["new"], 2048)), rep
+    for S in sides:
+        step(S, 0)                           # HIP's default stream
+        assert np.array_equal(S["pout"].numpy(), prompt(S["hq"], S["hk"], S["hv"], S["new"], 2048))
+        ok(h.hipGraphExecDestroy(S["exec"]))
+        ok(h.hipStreamDestroy(S["stream"]))
+
+
+def step(S, stream):
+    S["cache"].write(S["k"], S["v"], S["slots"], stream=stream)
+    S["at"].cached(S["q"], S["cu"], S["lens"], S["cache"], S["dtable"], S["out"], S["ws"], stream=stream)
+    S["at"].prompt(S["q"], S["k"], S["v"], S["cu"], S["pout"], S["pws"], stream=stream)
+
+
+def test_calls_of_two_threads(atlas):
+    """two threads that share the runtime, each with its own stream and workspace, at once"""
+    import threading
+    import jolt_atlas_amd.attention as T
+    h, wrong = hip(), []
+
+    def work(seed):
+        rng = np.random.default_rng(seed)
+        st = C.c_void_p()
+        ok(h.hipSetDevice(C.c_int(0)))
+        ok(h.hipStreamCreateWithFlags(C.byref(st), C.c_uint(1)))
+        at = T.Attention(4, 2, 64, 2048)
+        q, k, v = values(rng, (90, 4, 64)), values(rng, (90, 2, 64)), values(rng, (90, 2, 64))
+        want = prompt(q, k, v, [50, 40], 2048)
+        dev, ws, cu = [Dev(x) for x in (q, k, v)], workspace(at.prompt_workspace_bytes(2, 90)), Dev(np.array([0, 50, 90], np.int32))
+        for _ in range(20):
+            out = Dev(np.zeros(q.shape, np.int32))
+            at.prompt(*dev, cu, out, ws, stream=st.value)
+            ok(h.hipStreamSynchronize(st))
+            if not np.array_equal(out.numpy(), want):
+                wrong.append(seed)
+        ok(h.hipStreamDestroy(st))
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
