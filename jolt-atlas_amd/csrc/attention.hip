@@ -4,6 +4,7 @@
 
 #include "attention_kernels.hip.h"
 #include "attention_launch.hpp"
+#include "attention_tile.hip.h"
 
 namespace {
 
@@ -19,13 +20,59 @@ Args args_of(const atlas_attn_shape_t* s, const atlas_attn_rows_t* q, const int3
     return A;
 }
 
+
+// head sizes are padded to the fragments of the tile kernel
+int padded_dim(size_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+template <class F>
+int with_dim(int dp, F f) {
+    switch (dp) {
+        case 32: return f(std::integral_constant<int, 32>{});
+        case 64: return f(std::integral_constant<int, 64>{});
+        case 128: return f(std::integral_constant<int, 128>{});
+        default: return f(std::integral_constant<int, 256>{});
+    }
+}
+
+// the digit planes of the tile kernel in a workspace; per_seq = 0: the tiles of packed prompts
+struct PlanesLayout {
+    size_t tiles, per_seq, bytes, v_at, mag_at, there_at;
+    PlanesLayout(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys) {
+        const size_t slack = 4;                                        // a step reads up to 4 tiles: its last ones may lie behind a sequence's end
+        per_seq = max_keys ? (max_keys + 31) / 32 : 0;
+        tiles = (max_keys ? n_seqs * per_seq : n_tokens / 32 + n_seqs) + slack;
+        const size_t one = tiles * s->n_kv_heads * (size_t)(padded_dim(s->head_dim) / 32 * 3072);
+        v_at = one;
+        mag_at = 2 * one;
+        there_at = mag_at + 8 * tiles * s->n_kv_heads;
+        bytes = there_at + 4 * tiles;
+    }
+    Planes at(void* ws, const atlas_attn_shape_t* s) const {
+        uint8_t* w = (uint8_t*)ws;
+        return Planes{w, w + v_at, (uint32_t*)(w + mag_at), (uint32_t*)(w + mag_at) + tiles * s->n_kv_heads, (uint32_t*)(w + there_at), (uint32_t)tiles, (uint32_t)per_seq};
+    }
+};
+bool many_rows(size_t n_seqs, size_t n_tokens) { return n_tokens > 4 * n_seqs; }
+template <class CT>
+int launch_tiles(const Args& A, const Planes& P, size_t dp, hipStream_t stream) {
+    return with_dim((int)dp, [&](auto dim) -> int {
+        constexpr int DP = decltype(dim)::value;
+        using T = TileShape<DP>;
+        k_attn_planes<CT, DP><<<dim3(P.tiles, A.KV), 256, 0, stream>>>(A, P);
+        const uint64_t wgs = ((uint64_t)A.n_tokens * A.G / T::ROWS + A.n_seqs) * A.KV;
+        if (wgs > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows for one call");
+        if (T::LDS > 65536) HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_tile<CT, DP>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS));
+        k_attn_tile<CT, DP><<<(unsigned)wgs, 256, T::LDS, stream>>>(A, P);
+        return ATLAS_OK;
+    });
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens)) return 0;
-    return 16;
+    return PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
 }
 
 int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
@@ -47,13 +94,14 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (int rc = L.on_device({q->d, k->d, v->d, d_cu_seqlens, out->d, d_workspace})) return rc;
     Args A = args_of(shape, q, d_cu_seqlens, n_seqs, n_tokens, out);
     A.k = rows_of(k); A.v = rows_of(v);
-    atlas_attn::k_attn_exact<int32_t><<<dim3((unsigned)n_tokens, A.H), 256, 0, L.stream>>>(A);
+    const PlanesLayout P(shape, n_seqs, n_tokens, 0);
+    if (int rc = launch_tiles<int32_t>(A, P.at(d_workspace, shape), padded_dim(shape->head_dim), L.stream)) return rc;
     return L.end();
 }
 
 size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
-    return 16;
+    return many_rows(n_seqs, n_tokens) ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_blocks * cache->block_size, 1)).bytes : 16;
 }
 
 int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const int32_t* d_cu_new, const int32_t* d_kv_lens, size_t n_seqs, size_t n_tokens,
@@ -76,6 +124,12 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     Args A = args_of(shape, q, d_cu_new, n_seqs, n_tokens, out);
     A.ck = cache->d_k; A.cv = cache->d_v; A.lens = d_kv_lens; A.table = d_block_table; A.table_stride = (int64_t)table_stride;
     A.n_blocks = (uint32_t)cache->n_blocks; A.log_block = log2_of(cache->block_size); A.max_keys = (uint32_t)(max_blocks * cache->block_size);
+    if (many_rows(n_seqs, n_tokens)) {
+        const PlanesLayout P(shape, n_seqs, n_tokens, std::max<size_t>(A.max_keys, 1));
+        const int dp = padded_dim(shape->head_dim);
+        if (int rc = cache->bits == 16 ? launch_tiles<int16_t>(A, P.at(d_workspace, shape), dp, L.stream) : launch_tiles<int32_t>(A, P.at(d_workspace, shape), dp, L.stream)) return rc;
+        return L.end();
+    }
     if (cache->bits == 16) atlas_attn::k_attn_exact<int16_t><<<dim3((unsigned)n_tokens, A.H), 256, 0, L.stream>>>(A);
     else atlas_attn::k_attn_exact<int32_t><<<dim3((unsigned)n_tokens, A.H), 256, 0, L.stream>>>(A);
     return L.end();

@@ -49,7 +49,7 @@ __device__ inline int64_t cache_at(const Args& A, int64_t block, uint32_t kvh, u
 __device__ inline int32_t clamp32(int64_t x) { return (int32_t)(x > 2147483647ll ? 2147483647ll : x < -2147483648ll ? -2147483648ll : x); }
 __device__ inline int32_t exp_q(uint32_t z, const int32_t* hi, const int32_t* lo) {
     z = min(z, (uint32_t)atlas::ExpTable::Z_MAX);
-    return (hi[z >> atlas::ExpTable::LOG_BASE] * lo[z & (atlas::ExpTable::BASE - 1)]) >> SCALE;      // <= 2^28
+    return (int32_t)(__umul24((uint32_t)hi[z >> atlas::ExpTable::LOG_BASE], (uint32_t)lo[z & (atlas::ExpTable::BASE - 1)]) >> SCALE);      // <= 2^28
 }
 // sums of e saturate: from 2^28 + 1 on the reciprocal floor(2^28 / sum) is 0 whatever the sum
 __device__ inline uint32_t add_sat(uint32_t a, uint32_t b) { const uint32_t s = a + b; return s < a ? 0xffffffffu : s; }

@@ -1,0 +1,387 @@
+// The matrix-core path of the quantised attention for many rows of queries: keys and values cut into signed bytes once (k_attn_planes), then one workgroup per tile of
+// query rows (k_attn_tile).
+//
+// An int32 operand in [-8421504, 8355711] is d0 + 2^8 d1 + 2^16 d2 with signed bytes d: (v + 0x808080) ^ 0x808080 holds the three of them.  A product of two
+// such operands is nine i8 products in five weights, exact in the 32-bit accumulators of v_mfma_i32_32x32x32_i8: 9 x 2 d / 5 POP/s per score against a 64-bit
+// multiply-add per element on the vector unit.  The five sums recombine without 64-bit arithmetic: with hi = a2 + 2^8 a3 + 2^16 a4 and lo = a0 + 2^8 a1,
+//     floor((2^16 hi + lo) / 2^14) = 4 hi + (lo >> 14),
+// and hi may wrap, as long as the score itself fits 32 bits: |q| |k| d < 2^45, decided per tile from the operands' magnitudes.  Tiles that do not
+// qualify (and operands beyond three bytes) are computed row by row in 64 bits (row_exact).
+//
+// The products are taken as S^T = K Q^T, so a lane holds 16 scores of ONE query row: maximum, sum and weights stay in registers, and four weights that
+// follow each other there are four bytes of the operand of O^T = V^T P^T (the keys of V's fragments are laid out in that order).  The weights
+// 0 .. 2^14 are two signed bytes; of the second, most tiles have none (p < 128) and skip it.  sum_j p <= 2^14, so an output accumulator stays below
+// 2^21 however many keys there are.
+#pragma once
+#include "attention_kernels.hip.h"
+
+namespace atlas_attn {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef int16_t i16x4 __attribute__((ext_vector_type(4), aligned(2)));
+
+constexpr uint32_t WIDE = 0x80000000u;             // in a magnitude word: an operand beyond three signed bytes
+
+// four operands that follow each other along the product's inner dimension -> a dword of each digit plane
+__device__ inline void digits4(const int32_t v0, const int32_t v1, const int32_t v2, const int32_t v3, int& p0, int& p1, int& p2, uint32_t& mag) {
+    const uint32_t u0 = v0 + 0x808080u, u1 = v1 + 0x808080u, u2 = v2 + 0x808080u, u3 = v3 + 0x808080u;
+    mag |= (uint32_t)(v0 ^ (v0 >> 31)) | (uint32_t)(v1 ^ (v1 >> 31)) | (uint32_t)(v2 ^ (v2 >> 31)) | (uint32_t)(v3 ^ (v3 >> 31));
+    if ((u0 | u1 | u2 | u3) >> 24) mag |= WIDE;
+    const uint32_t w0 = u0 ^ 0x808080u, w1 = u1 ^ 0x808080u, w2 = u2 ^ 0x808080u, w3 = u3 ^ 0x808080u;
+    const uint32_t t01 = __builtin_amdgcn_perm(w1, w0, 0x05010400u), t23 = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
+    p0 = (int)__builtin_amdgcn_perm(t23, t01, 0x05040100u);
+    p1 = (int)__builtin_amdgcn_perm(t23, t01, 0x07060302u);
+    p2 = (int)(__builtin_amdgcn_perm(w1, w0, 0x0c0c0602u) | __builtin_amdgcn_perm(w3, w2, 0x06020c0cu));
+}
+// elements [i, i + 4) of a row of d, zeros behind its end
+template <class T>
+__device__ inline void load4(const T* row, uint32_t i, uint32_t d, int32_t (&o)[4]) {
+    if (i + 4 <= d) {
+        if constexpr (sizeof(T) == 4) { const i32x4 a = *(const i32x4*)(row + i); o[0] = a[0]; o[1] = a[1]; o[2] = a[2]; o[3] = a[3]; }
+        else { const i16x4 a = *(const i16x4*)(row + i); o[0] = a[0]; o[1] = a[1]; o[2] = a[2]; o[3] = a[3]; }
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) o[e] = i + e < d ? (int32_t)row[i + e] : 0;
+    }
+}
+
+// Digit planes in the order in which the fragments are read: [kv head][tile of 32 keys][fragment of 32 dims][plane][lane][16 bytes], K's and V's each.
+//   K: lane l holds key l % 32, dims 16 (l / 32) + b;   V: lane l holds dim l % 32, byte b is key 8 (b / 4) + 4 (l / 32) + b % 4 of the tile
+struct Planes {
+    uint8_t *k, *v;
+    uint32_t *k_mag, *v_mag;       // [kv head][tile]
+    uint32_t* there;               // [tile]: which of its keys exist
+    uint32_t tiles, per_seq;       // per_seq: tiles of a sequence (cached); 0: by its offset (prompt)
+};
+// Offsets cu[s] / 32 + s are far enough apart for ceil(len / 32) tiles each: no prefix sum is needed
+__device__ inline uint32_t tile_base(const Args& A, const Planes& P, uint32_t s) { return P.per_seq ? s * P.per_seq : min((uint32_t)max(A.cu[s], 0), A.n_tokens) / 32 + s; }
+
+// largest s with base(s) <= x, base increasing
+template <class F>
+__device__ inline uint32_t last_at_most(uint32_t n, uint64_t x, F base) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) { const uint32_t mid = (lo + hi) / 2; if (base(mid) <= x) lo = mid; else hi = mid; }
+    return lo;
+}
+
+template <class CT, int DP>
+__global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
+    constexpr int F = DP / 32;
+    const uint32_t tile = blockIdx.x, kvh = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+    const uint32_t si = P.per_seq ? tile / P.per_seq : last_at_most(A.n_seqs, tile, [&](uint32_t s) { return (uint64_t)tile_base(A, P, s); });
+    if (si >= A.n_seqs) return;
+    const Seq s = seq_at(A, si);
+    const uint32_t base = tile_base(A, P, si);
+    if (tile < base || s.n_new == 0) return;
+    const uint32_t j0 = (tile - base) * 32;
+    if (j0 >= s.keys) return;
+    __shared__ uint32_t s_mag[2];
+    if (threadIdx.x < 2) s_mag[threadIdx.x] = 0;
+    __syncthreads();
+    // where each key of the tile lies (nullptr: nowhere)
+    auto row = [&](uint32_t j, bool value) -> const CT* {
+        if (j >= s.keys) return nullptr;
+        if (A.table) { const int64_t b = block_of(A, s, j); return b < 0 ? nullptr : (const CT*)(value ? A.cv : A.ck) + cache_at(A, b, kvh, j); }
+        const Rows& r = value ? A.v : A.k;
+        return (const CT*)r.d + (int64_t)(s.begin + j) * r.ts + (int64_t)kvh * r.hs;
+    };
+    const int64_t at = ((int64_t)kvh * P.tiles + tile) * (F * 3 * 1024);
+    uint32_t mk = 0, mv = 0;
+    const CT* kr = row(j0 + l32, false);
+    if (wave == 0 && kvh == 0) { const uint64_t b = __ballot(kr != nullptr); if (lane == 0) P.there[tile] = (uint32_t)b; }
+    for (int f = wave; f < F; f += 4) {
+        v4i p0, p1, p2;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            int32_t e[4] = {0, 0, 0, 0};
+            if (kr) load4(kr, f * 32 + half * 16 + c * 4, A.d, e);
+            int a, b, g;
+            digits4(e[0], e[1], e[2], e[3], a, b, g, mk);
+            p0[c] = a; p1[c] = b; p2[c] = g;
+        }
+        v4i* to = (v4i*)(P.k + at + f * 3072) + lane;
+        to[0] = p0; to[64] = p1; to[128] = p2;
+    }
+    for (int f = wave; f < F; f += 4) {
+        v4i p0, p1, p2;
+        const uint32_t i = f * 32 + l32;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            int32_t e[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) { const CT* vr = row(j0 + 8 * c + 4 * half + x, true); e[x] = vr && i < A.d ? (int32_t)vr[i] : 0; }
+            int a, b, g;
+            digits4(e[0], e[1], e[2], e[3], a, b, g, mv);
+            p0[c] = a; p1[c] = b; p2[c] = g;
+        }
+        v4i* to = (v4i*)(P.v + at + f * 3072) + lane;
+        to[0] = p0; to[64] = p1; to[128] = p2;
+    }
+    if (mk) atomicOr(&s_mag[0], mk);
+    if (mv) atomicOr(&s_mag[1], mv);
+    __syncthreads();
+    if (threadIdx.x == 0) { P.k_mag[(size_t)kvh * P.tiles + tile] = s_mag[0]; P.v_mag[(size_t)kvh * P.tiles + tile] = s_mag[1]; }
+}
+
+__device__ inline uint32_t bits_of(uint32_t mag) { return mag ? 32 - __builtin_clz(mag) : 0; }
+
+// 16 bytes per lane from global memory to LDS without a register on the way; lds: the wave's first byte
+__device__ inline void copy_to_lds(const uint8_t* src, uint8_t* lds, uint32_t bytes, uint32_t wave, uint32_t lane) {
+    for (uint32_t o = wave * 1024; o < bytes; o += 4096)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o + lane * 16), (__attribute__((address_space(3))) void*)(lds + o), 16, 0, 0);
+}
+__device__ inline void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0), the others untouched
+
+// the Mul node's rescale: floor(s c / 2^14) with 1 <= c <= 2^14, s = 2^14 a + b:  a c + floor(b c / 2^14), in 24-bit multiplications
+__device__ inline int32_t rescale(int32_t s, int32_t c) {
+    const int32_t a = s >> SCALE, b = s & (ONE - 1);
+    return __mul24(a, c) + (int32_t)(__umul24((uint32_t)b, (uint32_t)c) >> SCALE);
+}
+
+template <int DP>
+struct TileShape {
+    static constexpr int F = DP / 32;                         // fragments of 32 dims
+    static constexpr int SPLIT = DP <= 64 ? 1 : DP / 64;      // waves that share 32 query rows: each scores its own keys and carries 64 of the output's dims
+    static constexpr int GROUPS = 4 / SPLIT, ROWS = 32 * GROUPS;
+    static constexpr int SUBS = SPLIT < 2 ? 2 : SPLIT;        // key sub-tiles of 32 per step
+    static constexpr int KEYS = 32 * SUBS, MY_SUBS = SUBS / SPLIT;
+    static constexpr int OF = F / SPLIT;                      // output fragments of a wave
+    static constexpr uint32_t TILE = F * 3072, STEP = TILE * SUBS;
+    static constexpr int BUFS = DP == 256 ? 1 : 2;            // 160 KB of LDS hold one step of 256 dims
+    static constexpr uint32_t LUT = 4096, P_BYTES = SPLIT > 1 ? GROUPS * SUBS * 2048 : 0;
+    static constexpr uint32_t LDS = LUT + P_BYTES + STEP * BUFS + 1024;
+};
+
+template <class CT, int DP>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Planes P) {
+    using T = TileShape<DP>;
+    constexpr int F = T::F, SPLIT = T::SPLIT, SUBS = T::SUBS;
+    extern __shared__ __align__(16) uint8_t lds[];
+    int32_t* s_hi = (int32_t*)lds;
+    int32_t* s_lo = s_hi + 512;
+    uint8_t* s_p = lds + T::LUT;
+    uint8_t* s_a = s_p + T::P_BYTES;
+    uint8_t* s_b = s_a + (T::BUFS == 2 ? T::STEP : 0);
+    uint32_t* s_red = (uint32_t*)(s_a + T::STEP * T::BUFS);        // 256 words
+    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+    const uint32_t group = wave / SPLIT, part = wave % SPLIT;
+    // the kv head runs fastest: with 8 of them each XCD's L2 sees one head's planes; late tiles (many keys under the causal mask) start first
+    const uint32_t kvh = blockIdx.x % A.KV, qt = gridDim.x / A.KV - 1 - blockIdx.x / A.KV;
+    auto q_base = [&](uint32_t s) { return (uint64_t)min((uint32_t)max(A.cu[s], 0), A.n_tokens) * A.G / T::ROWS + s; };
+    const uint32_t si = last_at_most(A.n_seqs, qt, q_base);
+    const Seq s = seq_at(A, si);
+    const uint64_t first = (uint64_t)(qt - q_base(si)) * T::ROWS;
+    const uint32_t n_rows = s.n_new * A.G;
+    if (qt < q_base(si) || first >= n_rows) return;
+    const uint32_t row0 = (uint32_t)first, rows = min((uint32_t)T::ROWS, n_rows - row0);
+    const uint32_t base = tile_base(A, P, si);
+    // my row
+    const uint32_t r = row0 + group * 32 + l32;
+    const bool mine = r < n_rows;
+    const uint32_t rr = mine ? r : n_rows - 1, tok = rr / A.G, head = kvh * A.G + rr % A.G;
+    const uint32_t limit = min(key_limit(A, s, tok), s.keys);
+    const uint32_t most = min(key_limit(A, s, (row0 + rows - 1) / A.G), s.keys), n_steps = (most + T::KEYS - 1) / T::KEYS;
+
+    for (uint32_t i = tid; i < 512; i += 256) { s_hi[i] = g_exp.hi[i]; s_lo[i] = g_exp.lo[i]; }
+    if (tid < 3) s_red[tid] = 0;
+    __syncthreads();
+    v4i q0[F], q1[F], q2[F];
+    uint32_t mq = 0, mk = 0, mv = 0;
+    {
+        const int32_t* q = A.q.d + (int64_t)(s.begin + tok) * A.q.ts + (int64_t)head * A.q.hs;
+#pragma unroll
+        for (int f = 0; f < F; f++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                int32_t e[4];
+                load4(q, f * 32 + half * 16 + c * 4, A.d, e);
+                int a, b, g;
+                digits4(e[0], e[1], e[2], e[3], a, b, g, mq);
+                q0[f][c] = a; q1[f][c] = b; q2[f][c] = g;
+            }
+        const uint32_t tiles = (most + 31) / 32;
+        for (uint32_t i = tid; i < tiles; i += 256) { mk |= P.k_mag[(size_t)kvh * P.tiles + base + i]; mv |= P.v_mag[(size_t)kvh * P.tiles + base + i]; }
+        if (mq) atomicOr(&s_red[0], mq);
+        if (mk) atomicOr(&s_red[1], mk);
+        if (mv) atomicOr(&s_red[2], mv);
+        __syncthreads();
+        mq = s_red[0]; mk = s_red[1]; mv = s_red[2];
+        __syncthreads();
+    }
+    if (((mq | mk | mv) & WIDE) || bits_of(mq) + bits_of(mk) + bits_of(A.d - 1) > 45) {
+        int32_t* x_q = (int32_t*)s_a;                                  // 1 KB, 1 KB, 2 KB of the tile buffer
+        for (uint32_t x = 0; x < rows; x++) row_exact<CT>(A, s, (row0 + x) / A.G, kvh * A.G + (row0 + x) % A.G, x_q, x_q + 256, (uint64_t*)(x_q + 512));
+        return;
+    }
+
+    const uint8_t* gk = P.k + ((int64_t)kvh * P.tiles + base) * T::TILE;
+    const uint8_t* gv = P.v + ((int64_t)kvh * P.tiles + base) * T::TILE;
+    // the scores of sub-tile `sub` of the step in `buf`, in one sweep over the fragments with five accumulators
+    auto scores = [&](const uint8_t* buf, int sub, v16i& x) {
+        v16i a0 = {}, a1 = {}, a2 = {}, a3 = {}, a4 = {};
+        const v4i* kf = (const v4i*)(buf + sub * T::TILE) + lane;
+#pragma unroll
+        for (int f = 0; f < F; f++) {
+            const v4i k0 = kf[f * 192], k1 = kf[f * 192 + 64], k2 = kf[f * 192 + 128];
+            a4 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q2[f], a4, 0, 0, 0);
+            a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q1[f], a3, 0, 0, 0);
+            a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q0[f], a2, 0, 0, 0);
+            a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q0[f], a1, 0, 0, 0);
+            a0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q0[f], a0, 0, 0, 0);
+            a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q2[f], a3, 0, 0, 0);
+            a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q1[f], a2, 0, 0, 0);
+            a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q1[f], a1, 0, 0, 0);
+            a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q2[f], a2, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int32_t hi = (int32_t)((uint32_t)a2[i] + ((uint32_t)a3[i] << 8) + ((uint32_t)a4[i] << 16));
+            // 256 dims: 2^8 a1 may pass 32 bits, so the low part is shifted down first (the floors nest)
+            const int32_t lo = DP == 256 ? ((a0[i] >> 8) + a1[i]) >> 6 : (a0[i] + (int32_t)((uint32_t)a1[i] << 8)) >> SCALE;
+            int32_t v = (int32_t)(((uint32_t)hi << 2) + (uint32_t)lo);
+            if (A.mul != ONE) v = rescale(v, A.mul);
+            x[i] = v;
+        }
+    };
+    // which of a lane's 16 keys of a sub-tile count: bit i; `all`: every one of the wave's does
+    auto seen = [&](uint32_t step, int sub, bool& all) -> uint32_t {
+        const uint32_t j0 = step * T::KEYS + sub * 32, t = j0 / 32;
+        const uint32_t there = j0 < s.keys ? P.there[base + t] : 0;
+        uint32_t in = limit >= j0 + 32 ? ~0u : limit > j0 ? (1u << (limit - j0)) - 1 : 0;
+        in &= there;
+        all = __all(in == ~0u);
+        const uint32_t w = in >> (4 * half);                           // byte c: keys 8 c + 4 half ..
+        return (w & 0xf) | ((w >> 4) & 0xf0) | ((w >> 8) & 0xf00) | ((w >> 12) & 0xf000);
+    };
+
+    // ---- pass 1: the maximum, pass 2: the sum
+    int32_t m = INT32_MIN;
+    uint32_t sum = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+        if (T::BUFS == 2 && n_steps) copy_to_lds(gk, s_a, T::STEP, wave, lane);
+#pragma unroll 1
+        for (uint32_t step = 0; step < n_steps; step++) {
+            uint8_t* buf = T::BUFS == 2 && (step & 1) ? s_b : s_a;
+            if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gk + (int64_t)step * T::STEP, buf, T::STEP, wave, lane); }
+            wait_loads();
+            __syncthreads();
+            if (T::BUFS == 2 && step + 1 < n_steps) copy_to_lds(gk + (int64_t)(step + 1) * T::STEP, (step & 1) ? s_a : s_b, T::STEP, wave, lane);
+#pragma unroll 1
+            for (int y = 0; y < T::MY_SUBS; y++) {
+                const int sub = part * T::MY_SUBS + y;
+                bool all;
+                const uint32_t in = seen(step, sub, all);
+                if (!__any(in != 0)) continue;
+                v16i x;
+                scores(buf, sub, x);
+                if (pass == 0) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) { const int32_t v = all || ((in >> i) & 1) ? x[i] : INT32_MIN; m = max(m, v); }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int32_t e = exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo);
+                        sum = __builtin_elementwise_add_sat(sum, all || ((in >> i) & 1) ? (uint32_t)e : 0u);
+                    }
+                }
+            }
+        }
+        // the other half-wave has the rest of the row's keys, and so have the waves that share the rows
+        if (pass == 0) m = max(m, __shfl_xor(m, 32)); else sum = __builtin_elementwise_add_sat(sum, (uint32_t)__shfl_xor((int)sum, 32));
+        __syncthreads();
+        if (SPLIT > 1) {
+            if (half == 0) s_red[wave * 32 + l32] = pass == 0 ? (uint32_t)m : sum;
+            __syncthreads();
+            for (int p = 0; p < SPLIT; p++) {
+                const uint32_t o = s_red[(group * SPLIT + p) * 32 + l32];
+                if (p != (int)part) { if (pass == 0) m = max(m, (int32_t)o); else sum = __builtin_elementwise_add_sat(sum, o); }
+            }
+            __syncthreads();
+        }
+    }
+    const uint32_t inv = sum ? (1u << (2 * SCALE)) / sum : 0;
+
+    // ---- pass 3: the weights again, and their product with the values.  o[.][f]: the sums with the values' digit 0, 1, 2
+    v16i o0[T::OF] = {}, o1[T::OF] = {}, o2[T::OF] = {};
+    if (T::BUFS == 2 && n_steps) copy_to_lds(gk, s_a, T::STEP, wave, lane);
+#pragma unroll 1
+    for (uint32_t step = 0; step < n_steps; step++) {
+        if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gk + (int64_t)step * T::STEP, s_a, T::STEP, wave, lane); }
+        wait_loads();
+        __syncthreads();
+        if (T::BUFS == 2) copy_to_lds(gv + (int64_t)step * T::STEP, s_b, T::STEP, wave, lane);
+        v4i w0[T::MY_SUBS], w1[T::MY_SUBS];
+#pragma unroll
+        for (int y = 0; y < T::MY_SUBS; y++) {
+            const int sub = part * T::MY_SUBS + y;
+            bool all;
+            const uint32_t in = seen(step, sub, all);
+            w0[y] = v4i{}; w1[y] = v4i{};
+            if (__any(in != 0)) {
+                v16i x;
+                scores(s_a, sub, x);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t p[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t e = (uint32_t)exp_q((uint32_t)m - (uint32_t)x[4 * c + i], s_hi, s_lo);
+                        p[i] = all || ((in >> (4 * c + i)) & 1) ? __umul24(e, inv) >> SCALE : 0;
+                    }
+                    // p = (signed byte) p + 2^8 ((p + 128) >> 8)
+                    const uint32_t a = p[0] | (p[1] << 16), b = p[2] | (p[3] << 16);
+                    w0[y][c] = (int)__builtin_amdgcn_perm(b, a, 0x06040200u);
+                    w1[y][c] = (int)__builtin_amdgcn_perm(b + 0x00800080u, a + 0x00800080u, 0x07050301u);
+                }
+            }
+            if (SPLIT > 1) {
+                v4i* to = (v4i*)(s_p + (group * SUBS + sub) * 2048) + lane;
+                to[0] = w0[y]; to[64] = w1[y];
+            }
+        }
+        if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gv + (int64_t)step * T::STEP, s_b, T::STEP, wave, lane); }
+        wait_loads();
+        __syncthreads();
+        if (T::BUFS == 2 && step + 1 < n_steps) copy_to_lds(gk + (int64_t)(step + 1) * T::STEP, s_a, T::STEP, wave, lane);
+#pragma unroll
+        for (int sub = 0; sub < SUBS; sub++) {
+            v4i b0, b1;
+            if (SPLIT > 1) { const v4i* from = (const v4i*)(s_p + (group * SUBS + sub) * 2048) + lane; b0 = from[0]; b1 = from[64]; }
+            else { b0 = w0[sub]; b1 = w1[sub]; }
+            const bool second = __any((b1[0] | b1[1] | b1[2] | b1[3]) != 0);
+            if (!second && !__any((b0[0] | b0[1] | b0[2] | b0[3]) != 0)) continue;
+            const v4i* vf = (const v4i*)(s_b + sub * T::TILE + part * T::OF * 3072) + lane;
+#pragma unroll
+            for (int f = 0; f < T::OF; f++) {
+                const v4i x0 = vf[f * 192], x1 = vf[f * 192 + 64], x2 = vf[f * 192 + 128];
+                o0[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x0, b0, o0[f], 0, 0, 0);
+                o1[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x1, b0, o1[f], 0, 0, 0);
+                o2[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x2, b0, o2[f], 0, 0, 0);
+                if (second) {
+                    const v16i y0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x0, b1, v16i{}, 0, 0, 0), y1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x1, b1, v16i{}, 0, 0, 0),
+                               y2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x2, b1, v16i{}, 0, 0, 0);
+                    o0[f] += y0 * 256; o1[f] += y1 * 256; o2[f] += y2 * 256;
+                }
+            }
+        }
+    }
+    // floor((o0 + 2^8 o1 + 2^16 o2) / 2^14): a lane holds dims 8 c + 4 half .. + 3 of its row
+    if (!mine) return;
+    int32_t* out = A.out.d + (int64_t)(s.begin + tok) * A.out.ts + (int64_t)head * A.out.hs;
+#pragma unroll
+    for (int f = 0; f < T::OF; f++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const uint32_t i = (part * T::OF + f) * 32 + 8 * c + 4 * half;
+            i32x4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = (int32_t)(((int64_t)o0[f][4 * c + e] + ((int64_t)o1[f][4 * c + e] << 8) + ((int64_t)o2[f][4 * c + e] << 16)) >> SCALE);
+            if (i + 4 <= A.d) *(i32x4*)(out + i) = y;
+            else for (uint32_t e = 0; e < 4; e++) if (i + e < A.d) out[i + e] = y[e];
+        }
+}
+
+}  // namespace atlas_attn
