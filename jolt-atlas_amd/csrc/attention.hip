@@ -4,6 +4,7 @@
 
 #include "attention_kernels.hip.h"
 #include "attention_launch.hpp"
+#include "attention_split.hip.h"
 #include "attention_tile.hip.h"
 
 namespace {
@@ -66,6 +67,53 @@ int launch_tiles(const Args& A, const Planes& P, size_t dp, hipStream_t stream) 
     });
 }
 
+// Few rows: the workspace of the split path.  A chunk is 128 keys or more: as many as keep the launch below about 8192 workgroups at the table's capacity
+struct SplitLayout {
+    Split S{};
+    size_t bytes, segments;
+    SplitLayout(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys, void* ws) {
+        const size_t G = s->n_heads / s->n_kv_heads, tiles = n_tokens * G / TILE_ROWS + n_seqs, rows = n_tokens * s->n_heads;
+        size_t chunk = 128;
+        while (chunk < SEGMENT && tiles * s->n_kv_heads * ((max_keys + chunk - 1) / chunk) > 8192) chunk *= 2;
+        const size_t chunks = std::max<size_t>((max_keys + chunk - 1) / chunk, 1), pitch = chunks * chunk;
+        segments = std::max<size_t>((max_keys + SEGMENT - 1) / SEGMENT, 1);
+        size_t at = 0;
+        auto take = [&](size_t n) { const size_t was = at; at += (n + 15) / 16 * 16; return (uint8_t*)ws + was; };
+        S.chunk = (uint32_t)chunk; S.n_chunks = (uint32_t)chunks; S.n_tiles = (uint32_t)tiles; S.n_rows = (uint32_t)rows; S.pitch = (int64_t)pitch;
+        S.scores = (int32_t*)take(rows * pitch * 4);
+        S.part = (int64_t*)take(chunks * rows * s->head_dim * 8);
+        S.cmax = (int32_t*)take(chunks * rows * 4);
+        S.csum = (uint32_t*)take(segments * rows * 4);
+        S.rmax = (int32_t*)take(rows * 4);
+        S.q_mag = (uint32_t*)take(tiles * s->n_kv_heads * 4);
+        S.k_mag = (uint32_t*)take(chunks * tiles * s->n_kv_heads * 4);
+        S.v_mag = (uint32_t*)take(chunks * tiles * s->n_kv_heads * 4);
+        bytes = at + 16;
+    }
+};
+template <class CT>
+int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
+    const uint64_t wgs = (uint64_t)L.S.n_tiles * A.KV;
+    if (wgs > 0x7fffffff || L.S.n_chunks > 65535 || L.segments > 65535) return fail(ATLAS_EINVAL, "attention: too many rows or keys for one call");
+    const dim3 grid((unsigned)wgs, L.S.n_chunks);
+    auto run = [&](auto ks, auto quad) {
+        k_split_scores<CT, decltype(ks)::value, decltype(quad)::value><<<grid, 256, 0, stream>>>(A, L.S);
+        k_split_sums<<<dim3(L.S.n_rows, (unsigned)L.segments), 256, 0, stream>>>(A, L.S);
+        k_split_values<CT, decltype(ks)::value, decltype(quad)::value><<<grid, 256, 0, stream>>>(A, L.S);
+    };
+    auto dims = [&](auto quad) {
+        switch ((A.d + 63) / 64) {
+            case 1: run(std::integral_constant<int, 1>{}, quad); break;
+            case 2: run(std::integral_constant<int, 2>{}, quad); break;
+            case 3: run(std::integral_constant<int, 3>{}, quad); break;
+            default: run(std::integral_constant<int, 4>{}, quad);
+        }
+    };
+    if (A.d % 4 == 0) dims(std::true_type{}); else dims(std::false_type{});
+    k_split_join<CT><<<(unsigned)wgs, 256, 0, stream>>>(A, L.S);
+    return ATLAS_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -101,7 +149,8 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
 
 size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
-    return many_rows(n_seqs, n_tokens) ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_blocks * cache->block_size, 1)).bytes : 16;
+    return many_rows(n_seqs, n_tokens) ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_blocks * cache->block_size, 1)).bytes
+                                       : SplitLayout(shape, n_seqs, n_tokens, max_blocks * cache->block_size, nullptr).bytes;
 }
 
 int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const int32_t* d_cu_new, const int32_t* d_kv_lens, size_t n_seqs, size_t n_tokens,
@@ -130,8 +179,8 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
         if (int rc = cache->bits == 16 ? launch_tiles<int16_t>(A, P.at(d_workspace, shape), dp, L.stream) : launch_tiles<int32_t>(A, P.at(d_workspace, shape), dp, L.stream)) return rc;
         return L.end();
     }
-    if (cache->bits == 16) atlas_attn::k_attn_exact<int16_t><<<dim3((unsigned)n_tokens, A.H), 256, 0, L.stream>>>(A);
-    else atlas_attn::k_attn_exact<int32_t><<<dim3((unsigned)n_tokens, A.H), 256, 0, L.stream>>>(A);
+    const SplitLayout P(shape, n_seqs, n_tokens, A.max_keys, d_workspace);
+    if (int rc = cache->bits == 16 ? launch_split<int16_t>(A, P, L.stream) : launch_split<int32_t>(A, P, L.stream)) return rc;
     return L.end();
 }
 

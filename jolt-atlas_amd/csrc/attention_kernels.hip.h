@@ -1,4 +1,4 @@
-// Device side of the quantised attention (attention.hip): what every kernel of it shares, and the kernel that is right for any int32 operand.
+// Device side of the quantised attention (attention.hip): what every kernel of it shares, and the row that is right for any int32 operand.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -54,7 +54,7 @@ __device__ inline int32_t exp_q(uint32_t z, const int32_t* hi, const int32_t* lo
 // sums of e saturate: from 2^28 + 1 on the reciprocal floor(2^28 / sum) is 0 whatever the sum
 __device__ inline uint32_t add_sat(uint32_t a, uint32_t b) { const uint32_t s = a + b; return s < a ? 0xffffffffu : s; }
 
-// ---- any operands: one workgroup per (token, head), 64-bit products one by one, the scores recomputed in each of the three passes.
+// ---- any operands: a workgroup takes one (token, head), 64-bit products one by one, the scores recomputed in each of the three passes.
 // The softmax's floors are taken under the FINAL maximum and sum, so partial results cannot be rescaled as a float softmax's are: a pass for the
 // maximum, one for the sum, one for the product.
 template <class CT>
@@ -125,17 +125,6 @@ __device__ inline uint32_t find_seq(const int32_t* cu, uint32_t n_seqs, uint32_t
     uint32_t lo = 0, hi = n_seqs;                                    // cu[lo] <= t < cu[hi]
     while (hi - lo > 1) { const uint32_t mid = (lo + hi) / 2; if ((int64_t)t >= cu[mid]) lo = mid; else hi = mid; }
     return lo;
-}
-
-template <class CT>
-__global__ __launch_bounds__(256) void k_attn_exact(Args A) {
-    __shared__ int32_t s_q[256], s_p[256];
-    __shared__ uint64_t s_red[256];
-    const uint32_t t = blockIdx.x, h = blockIdx.y, si = find_seq(A.cu, A.n_seqs, t);
-    if (si >= A.n_seqs) return;
-    const Seq s = seq_at(A, si);
-    if (t < s.begin || t - s.begin >= s.n_new) return;
-    row_exact<CT>(A, s, t - s.begin, h, s_q, s_p, s_red);
 }
 
 }  // namespace atlas_attn

@@ -1,7 +1,7 @@
 // The matrix-core path of the quantised attention for many rows of queries: keys and values cut into signed bytes once (k_attn_planes), then one workgroup per tile of
 // query rows (k_attn_tile).
 //
-// An int32 operand in [-8421504, 8355711] is d0 + 2^8 d1 + 2^16 d2 with signed bytes d: (v + 0x808080) ^ 0x808080 holds the three of them.  A product of two
+// An int32 operand in [-8421504, 8355711] is d0 + 2^8 d1 + 2^16 d2 with signed bytes d: the bytes of v + 0x808080, each less 128.  A product of two
 // such operands is nine i8 products in five weights, exact in the 32-bit accumulators of v_mfma_i32_32x32x32_i8: 9 x 2 d / 5 POP/s per score against a 64-bit
 // multiply-add per element on the vector unit.  The five sums recombine without 64-bit arithmetic: with hi = a2 + 2^8 a3 + 2^16 a4 and lo = a0 + 2^8 a1,
 //     floor((2^16 hi + lo) / 2^14) = 4 hi + (lo >> 14),
@@ -24,16 +24,23 @@ typedef int16_t i16x4 __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr uint32_t WIDE = 0x80000000u;             // in a magnitude word: an operand beyond three signed bytes
 
-// four operands that follow each other along the product's inner dimension -> a dword of each digit plane
-__device__ inline void digits4(const int32_t v0, const int32_t v1, const int32_t v2, const int32_t v3, int& p0, int& p1, int& p2, uint32_t& mag) {
+// the extremes of the operands seen
+struct Range {
+    int32_t hi = 0, lo = 0;
+    // bits of the largest magnitude as a mask, WIDE where three signed bytes do not hold an operand
+    __device__ uint32_t word() const { return (uint32_t)hi | (uint32_t)(lo ^ (lo >> 31)) | (hi > 8355711 || lo < -8421504 ? WIDE : 0); }
+};
+// four operands that follow each other along the product's inner dimension -> a dword of each digit plane.  The extremes are taken at once (the empty asm):
+// left to itself the compiler keeps every operand to do it later, and spills.
+__device__ inline void digits4(const int32_t v0, const int32_t v1, const int32_t v2, const int32_t v3, int& p0, int& p1, int& p2, Range& g) {
+    g.hi = max(max(g.hi, max(v0, v1)), max(v2, v3));
+    g.lo = min(min(g.lo, min(v0, v1)), min(v2, v3));
+    asm volatile("" : "+v"(g.hi), "+v"(g.lo));
     const uint32_t u0 = v0 + 0x808080u, u1 = v1 + 0x808080u, u2 = v2 + 0x808080u, u3 = v3 + 0x808080u;
-    mag |= (uint32_t)(v0 ^ (v0 >> 31)) | (uint32_t)(v1 ^ (v1 >> 31)) | (uint32_t)(v2 ^ (v2 >> 31)) | (uint32_t)(v3 ^ (v3 >> 31));
-    if ((u0 | u1 | u2 | u3) >> 24) mag |= WIDE;
-    const uint32_t w0 = u0 ^ 0x808080u, w1 = u1 ^ 0x808080u, w2 = u2 ^ 0x808080u, w3 = u3 ^ 0x808080u;
-    const uint32_t t01 = __builtin_amdgcn_perm(w1, w0, 0x05010400u), t23 = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
-    p0 = (int)__builtin_amdgcn_perm(t23, t01, 0x05040100u);
-    p1 = (int)__builtin_amdgcn_perm(t23, t01, 0x07060302u);
-    p2 = (int)(__builtin_amdgcn_perm(w1, w0, 0x0c0c0602u) | __builtin_amdgcn_perm(w3, w2, 0x06020c0cu));
+    const uint32_t t01 = __builtin_amdgcn_perm(u1, u0, 0x05010400u), t23 = __builtin_amdgcn_perm(u3, u2, 0x05010400u);
+    p0 = (int)(__builtin_amdgcn_perm(t23, t01, 0x05040100u) ^ 0x80808080u);
+    p1 = (int)(__builtin_amdgcn_perm(t23, t01, 0x07060302u) ^ 0x80808080u);
+    p2 = (int)((__builtin_amdgcn_perm(u1, u0, 0x0c0c0602u) | __builtin_amdgcn_perm(u3, u2, 0x06020c0cu)) ^ 0x80808080u);
 }
 // elements [i, i + 4) of a row of d, zeros behind its end
 template <class T>
@@ -88,7 +95,7 @@ __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
         return (const CT*)r.d + (int64_t)(s.begin + j) * r.ts + (int64_t)kvh * r.hs;
     };
     const int64_t at = ((int64_t)kvh * P.tiles + tile) * (F * 3 * 1024);
-    uint32_t mk = 0, mv = 0;
+    Range rk, rv;
     const CT* kr = row(j0 + l32, false);
     if (wave == 0 && kvh == 0) { const uint64_t b = __ballot(kr != nullptr); if (lane == 0) P.there[tile] = (uint32_t)b; }
     for (int f = wave; f < F; f += 4) {
@@ -98,7 +105,7 @@ __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
             int32_t e[4] = {0, 0, 0, 0};
             if (kr) load4(kr, f * 32 + half * 16 + c * 4, A.d, e);
             int a, b, g;
-            digits4(e[0], e[1], e[2], e[3], a, b, g, mk);
+            digits4(e[0], e[1], e[2], e[3], a, b, g, rk);
             p0[c] = a; p1[c] = b; p2[c] = g;
         }
         v4i* to = (v4i*)(P.k + at + f * 3072) + lane;
@@ -113,14 +120,14 @@ __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
 #pragma unroll
             for (int x = 0; x < 4; x++) { const CT* vr = row(j0 + 8 * c + 4 * half + x, true); e[x] = vr && i < A.d ? (int32_t)vr[i] : 0; }
             int a, b, g;
-            digits4(e[0], e[1], e[2], e[3], a, b, g, mv);
+            digits4(e[0], e[1], e[2], e[3], a, b, g, rv);
             p0[c] = a; p1[c] = b; p2[c] = g;
         }
         v4i* to = (v4i*)(P.v + at + f * 3072) + lane;
         to[0] = p0; to[64] = p1; to[128] = p2;
     }
-    if (mk) atomicOr(&s_mag[0], mk);
-    if (mv) atomicOr(&s_mag[1], mv);
+    atomicOr(&s_mag[0], rk.word());
+    atomicOr(&s_mag[1], rv.word());
     __syncthreads();
     if (threadIdx.x == 0) { P.k_mag[(size_t)kvh * P.tiles + tile] = s_mag[0]; P.v_mag[(size_t)kvh * P.tiles + tile] = s_mag[1]; }
 }
@@ -138,6 +145,15 @@ __device__ inline void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }     
 __device__ inline int32_t rescale(int32_t s, int32_t c) {
     const int32_t a = s >> SCALE, b = s & (ONE - 1);
     return __mul24(a, c) + (int32_t)(__umul24((uint32_t)b, (uint32_t)c) >> SCALE);
+}
+
+// floor((a0 + 2^8 a1 + 2^16 a2 + 2^24 a3 + 2^32 a4) / 2^14), which fits 32 bits; LONG: more than 128 dims, where 2^8 a1 may not, so that the low part is
+// shifted down first (the floors nest)
+template <bool LONG>
+__device__ inline int32_t combine(int32_t a0, int32_t a1, int32_t a2, int32_t a3, int32_t a4) {
+    const uint32_t hi = (uint32_t)a2 + ((uint32_t)a3 << 8) + ((uint32_t)a4 << 16);
+    const int32_t lo = LONG ? ((a0 >> 8) + a1) >> 6 : (a0 + (int32_t)((uint32_t)a1 << 8)) >> SCALE;
+    return (int32_t)((hi << 2) + (uint32_t)lo);
 }
 
 template <int DP>
@@ -190,6 +206,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
     v4i q0[F], q1[F], q2[F];
     uint32_t mq = 0, mk = 0, mv = 0;
     {
+        Range rq;
         const int32_t* q = A.q.d + (int64_t)(s.begin + tok) * A.q.ts + (int64_t)head * A.q.hs;
 #pragma unroll
         for (int f = 0; f < F; f++)
@@ -198,12 +215,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
                 int32_t e[4];
                 load4(q, f * 32 + half * 16 + c * 4, A.d, e);
                 int a, b, g;
-                digits4(e[0], e[1], e[2], e[3], a, b, g, mq);
+                digits4(e[0], e[1], e[2], e[3], a, b, g, rq);
                 q0[f][c] = a; q1[f][c] = b; q2[f][c] = g;
             }
         const uint32_t tiles = (most + 31) / 32;
         for (uint32_t i = tid; i < tiles; i += 256) { mk |= P.k_mag[(size_t)kvh * P.tiles + base + i]; mv |= P.v_mag[(size_t)kvh * P.tiles + base + i]; }
-        if (mq) atomicOr(&s_red[0], mq);
+        atomicOr(&s_red[0], rq.word());
         if (mk) atomicOr(&s_red[1], mk);
         if (mv) atomicOr(&s_red[2], mv);
         __syncthreads();
@@ -237,10 +254,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const int32_t hi = (int32_t)((uint32_t)a2[i] + ((uint32_t)a3[i] << 8) + ((uint32_t)a4[i] << 16));
-            // 256 dims: 2^8 a1 may pass 32 bits, so the low part is shifted down first (the floors nest)
-            const int32_t lo = DP == 256 ? ((a0[i] >> 8) + a1[i]) >> 6 : (a0[i] + (int32_t)((uint32_t)a1[i] << 8)) >> SCALE;
-            int32_t v = (int32_t)(((uint32_t)hi << 2) + (uint32_t)lo);
+            int32_t v = combine<DP == 256>(a0[i], a1[i], a2[i], a3[i], a4[i]);
             if (A.mul != ONE) v = rescale(v, A.mul);
             x[i] = v;
         }
