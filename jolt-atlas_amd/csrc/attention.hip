@@ -91,6 +91,17 @@ struct SplitLayout {
         bytes = at + 16;
     }
 };
+template <class CT, class F>
+void with_steps(uint32_t d, F f) {
+    auto dims = [&](auto quad) {
+        switch ((d + 63) / 64) {
+            case 1: f(std::integral_constant<int, 1>{}, quad); break;
+            case 2: f(std::integral_constant<int, 2>{}, quad); break;
+            default: f(std::integral_constant<int, 4>{}, quad);
+        }
+    };
+    if (d % 4 == 0) dims(std::true_type{}); else dims(std::false_type{});
+}
 template <class CT>
 int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
     const uint64_t wgs = (uint64_t)L.S.n_tiles * A.KV;
@@ -101,17 +112,25 @@ int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
         k_split_sums<<<dim3(L.S.n_rows, (unsigned)L.segments), 256, 0, stream>>>(A, L.S);
         k_split_values<CT, decltype(ks)::value, decltype(quad)::value><<<grid, 256, 0, stream>>>(A, L.S);
     };
-    auto dims = [&](auto quad) {
-        switch ((A.d + 63) / 64) {
-            case 1: run(std::integral_constant<int, 1>{}, quad); break;
-            case 2: run(std::integral_constant<int, 2>{}, quad); break;
-            case 3: run(std::integral_constant<int, 3>{}, quad); break;
-            default: run(std::integral_constant<int, 4>{}, quad);
-        }
-    };
-    if (A.d % 4 == 0) dims(std::true_type{}); else dims(std::false_type{});
+    with_steps<CT>(A.d, run);
     k_split_join<CT><<<(unsigned)wgs, 256, 0, stream>>>(A, L.S);
     return ATLAS_OK;
+}
+
+bool fused(size_t max_keys, size_t d) { return max_keys <= fused_keys(d); }
+template <class CT>
+int launch_fused(const Args& A, size_t max_keys, hipStream_t stream) {
+    const uint64_t wgs = ((uint64_t)A.n_tokens * A.G / TILE_ROWS + A.n_seqs) * A.KV;
+    if (wgs > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows for one call");
+    int rc = ATLAS_OK;
+    with_steps<CT>(A.d, [&](auto ks, auto quad) {
+        constexpr int KS = decltype(ks)::value;
+        auto* k = &k_attn_fused<CT, KS, decltype(quad)::value>;
+        const size_t lds = fused_lds(max_keys, KS);
+        if (lds > 65536 - 6144 && hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) { rc = fail(ATLAS_ENODEV, "attention: LDS"); return; }
+        k<<<(unsigned)wgs, FUSED_WAVES * 64, lds, stream>>>(A, (uint32_t)fused_pitch(max_keys));
+    });
+    return rc;
 }
 
 }  // namespace
@@ -120,7 +139,7 @@ extern "C" {
 
 size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens)) return 0;
-    return PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
+    return fused(n_tokens, shape->head_dim) ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
 }
 
 int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
@@ -142,6 +161,10 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (int rc = L.on_device({q->d, k->d, v->d, d_cu_seqlens, out->d, d_workspace})) return rc;
     Args A = args_of(shape, q, d_cu_seqlens, n_seqs, n_tokens, out);
     A.k = rows_of(k); A.v = rows_of(v);
+    if (fused(n_tokens, A.d)) {
+        if (int rc = launch_fused<int32_t>(A, n_tokens, L.stream)) return rc;
+        return L.end();
+    }
     const PlanesLayout P(shape, n_seqs, n_tokens, 0);
     if (int rc = launch_tiles<int32_t>(A, P.at(d_workspace, shape), padded_dim(shape->head_dim), L.stream)) return rc;
     return L.end();
@@ -149,6 +172,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
 
 size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
+    if (fused(max_blocks * cache->block_size, shape->head_dim)) return 16;
     return many_rows(n_seqs, n_tokens) ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_blocks * cache->block_size, 1)).bytes
                                        : SplitLayout(shape, n_seqs, n_tokens, max_blocks * cache->block_size, nullptr).bytes;
 }
@@ -173,6 +197,10 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     Args A = args_of(shape, q, d_cu_new, n_seqs, n_tokens, out);
     A.ck = cache->d_k; A.cv = cache->d_v; A.lens = d_kv_lens; A.table = d_block_table; A.table_stride = (int64_t)table_stride;
     A.n_blocks = (uint32_t)cache->n_blocks; A.log_block = log2_of(cache->block_size); A.max_keys = (uint32_t)(max_blocks * cache->block_size);
+    if (fused(A.max_keys, A.d)) {
+        if (int rc = cache->bits == 16 ? launch_fused<int16_t>(A, A.max_keys, L.stream) : launch_fused<int32_t>(A, A.max_keys, L.stream)) return rc;
+        return L.end();
+    }
     if (many_rows(n_seqs, n_tokens)) {
         const PlanesLayout P(shape, n_seqs, n_tokens, std::max<size_t>(A.max_keys, 1));
         const int dp = padded_dim(shape->head_dim);

@@ -75,36 +75,36 @@ __device__ inline int32_t score_exact(const Args& A, const Seq& s, uint32_t kvh,
     return clamp32(((int64_t)x * A.mul) >> SCALE);
 }
 
-template <class CT>
+template <class CT, uint32_t NT = 256>
 __device__ void row_exact(const Args& A, const Seq& s, uint32_t i, uint32_t h, int32_t* s_q, int32_t* s_p, uint64_t* s_red) {
     const uint32_t tid = threadIdx.x, kvh = h / A.G, limit = min(key_limit(A, s, i), s.keys);
     const int32_t* q = A.q.d + (int64_t)(s.begin + i) * A.q.ts + (int64_t)h * A.q.hs;
-    for (uint32_t t = tid; t < A.d; t += 256) s_q[t] = q[t];
+    for (uint32_t t = tid; t < A.d; t += NT) s_q[t] = q[t];
     __syncthreads();
     int64_t m = INT64_MIN;
-    for (uint32_t j = tid; j < limit; j += 256) { bool there; const int32_t x = score_exact<CT>(A, s, kvh, s_q, j, there); if (there && x > m) m = x; }
+    for (uint32_t j = tid; j < limit; j += NT) { bool there; const int32_t x = score_exact<CT>(A, s, kvh, s_q, j, there); if (there && x > m) m = x; }
     s_red[tid] = (uint64_t)m;
     __syncthreads();
-    for (uint32_t w = 128; w > 0; w >>= 1) { if (tid < w) s_red[tid] = (uint64_t)max((int64_t)s_red[tid], (int64_t)s_red[tid + w]); __syncthreads(); }
+    for (uint32_t w = NT / 2; w > 0; w >>= 1) { if (tid < w) s_red[tid] = (uint64_t)max((int64_t)s_red[tid], (int64_t)s_red[tid + w]); __syncthreads(); }
     m = (int64_t)s_red[0];
     __syncthreads();
     uint64_t part = 0;
-    for (uint32_t j = tid; j < limit; j += 256) { bool there; const int32_t x = score_exact<CT>(A, s, kvh, s_q, j, there); if (there) part += exp_q((uint32_t)(m - x), g_exp.hi, g_exp.lo); }
+    for (uint32_t j = tid; j < limit; j += NT) { bool there; const int32_t x = score_exact<CT>(A, s, kvh, s_q, j, there); if (there) part += exp_q((uint32_t)(m - x), g_exp.hi, g_exp.lo); }
     s_red[tid] = part;
     __syncthreads();
-    for (uint32_t w = 128; w > 0; w >>= 1) { if (tid < w) s_red[tid] += s_red[tid + w]; __syncthreads(); }
+    for (uint32_t w = NT / 2; w > 0; w >>= 1) { if (tid < w) s_red[tid] += s_red[tid + w]; __syncthreads(); }
     const uint64_t sum = s_red[0];
     __syncthreads();
     const uint32_t inv = sum ? (uint32_t)((1ull << (2 * SCALE)) / sum) : 0;
     uint64_t acc = 0;
-    for (uint32_t j0 = 0; j0 < limit; j0 += 256) {
+    for (uint32_t j0 = 0; j0 < limit; j0 += NT) {
         const uint32_t j = j0 + tid;
         int32_t p = 0;
         if (j < limit) { bool there; const int32_t x = score_exact<CT>(A, s, kvh, s_q, j, there); if (there) p = (int32_t)(((uint32_t)exp_q((uint32_t)(m - x), g_exp.hi, g_exp.lo) * inv) >> SCALE); }
         s_p[tid] = p;
         __syncthreads();
         if (tid < A.d) {
-            const uint32_t n = min(256u, limit - j0);
+            const uint32_t n = min(NT, limit - j0);
             for (uint32_t t = 0; t < n; t++) {
                 if (!s_p[t]) continue;
                 int64_t v;

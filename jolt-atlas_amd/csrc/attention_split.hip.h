@@ -6,6 +6,8 @@
 // (16 dims of one key: 64 contiguous bytes) and are cut into digits in registers, values the same with 4 dims of 16 keys per lane; nothing
 // passes through LDS.  About 4.3 vector operations per element against 32 that the memory's rate leaves room for.
 #pragma once
+#include <algorithm>
+
 #include "attention_tile.hip.h"
 
 namespace atlas_attn {
@@ -54,8 +56,264 @@ __device__ inline RowTile row_tile(const Args& A, uint32_t x) {
 }
 __device__ inline uint32_t row_id(const Args& A, const RowTile& t, uint32_t r) { return (t.s.begin + r / A.G) * A.H + t.kvh * A.G + r % A.G; }
 
-template <class CT, int KS, bool QUAD>      // KS: steps of 64 dims
-__global__ __launch_bounds__(256, KS > 2 ? 1 : 2) void k_split_scores(Args A, Split S) {
+// ---- what the split and the fused kernels share; g = lane / 16, l = lane % 16 throughout: a lane has query row l
+template <int KS>
+struct Query { v4i q0[KS], q1[KS], q2[KS]; Range range; };
+template <int KS, bool QUAD>
+__device__ inline void load_query(const Args& A, const RowTile& R, uint32_t r, bool mine, uint32_t g, Query<KS>& Q) {
+    const int32_t* q = A.q.d + (int64_t)(R.s.begin + (mine ? r / A.G : 0)) * A.q.ts + (int64_t)(R.kvh * A.G + (mine ? r % A.G : 0)) * A.q.hs;
+#pragma unroll
+    for (int f = 0; f < KS; f++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            int32_t e[4];
+            const uint32_t i = f * 64 + g * 16 + x * 4;
+            fetch4<QUAD>(q, i, A.d, e);
+#pragma unroll
+            for (uint32_t y = 0; y < 4; y++) e[y] = mine && i + y < A.d ? e[y] : 0;
+            int a, b, d;
+            digits4(e[0], e[1], e[2], e[3], a, b, d, Q.range);
+            Q.q0[f][x] = a; Q.q1[f][x] = b; Q.q2[f][x] = d;
+        }
+}
+// where key j's row begins (value: among the values); a block that does not exist: block 0, whose scores and weights do not count
+template <class CT>
+__device__ inline const CT* key_row(const Args& A, const RowTile& R, uint32_t j, bool value, bool& there) {
+    if (A.table) {
+        const int64_t b = block_of(A, R.s, j);
+        there = b >= 0;
+        return (const CT*)(value ? A.cv : A.ck) + cache_at(A, max(b, (int64_t)0), R.kvh, j);
+    }
+    there = true;
+    const Rows& x = value ? A.v : A.k;
+    return (const CT*)x.d + (int64_t)(R.s.begin + j) * x.ts + (int64_t)R.kvh * x.hs;
+}
+// the scores of the 64 keys from j0 on (those below k1 count), x[t][i]: key 16 t + 4 g + i
+template <class CT, int KS, bool QUAD>
+__device__ inline void score64(const Args& A, const RowTile& R, const Query<KS>& Q, uint32_t j0, uint32_t k1, uint32_t limit, uint32_t g, uint32_t l, Range& range, v4i (&x)[4]) {
+    const CT* row[4];
+    uint32_t in[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        bool there;
+        row[t] = key_row<CT>(A, R, min(j0 + 16 * t + l, k1 - 1), false, there);      // behind the end: the last key again
+        in[t] = (uint32_t)__ballot(there && j0 + 16 * t + l < k1) & 0xffff;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        if (t == 2) __builtin_amdgcn_sched_barrier(0);               // two sub-tiles' loads in flight; all four would spill
+        v4i a0 = {}, a1 = {}, a2 = {}, a3 = {}, a4 = {};
+#pragma unroll
+        for (int f = 0; f < KS; f++) {
+            v4i p0, p1, p2;
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                int32_t e[4];
+                fetch4<QUAD>(row[t], f * 64 + g * 16 + y * 4, A.d, e);
+                int a, b, d;
+                digits4(e[0], e[1], e[2], e[3], a, b, d, range);
+                p0[y] = a; p1[y] = b; p2[y] = d;
+            }
+            a4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, Q.q2[f], a4, 0, 0, 0);
+            a3 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, Q.q1[f], a3, 0, 0, 0);
+            a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, Q.q0[f], a2, 0, 0, 0);
+            a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, Q.q0[f], a1, 0, 0, 0);
+            a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, Q.q0[f], a0, 0, 0, 0);
+            a3 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, Q.q2[f], a3, 0, 0, 0);
+            a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, Q.q1[f], a2, 0, 0, 0);
+            a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, Q.q1[f], a1, 0, 0, 0);
+            a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, Q.q2[f], a2, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            int32_t v = combine<KS >= 3>(a0[i], a1[i], a2[i], a3[i], a4[i]);
+            if (A.mul != ONE) v = rescale(v, A.mul);
+            const uint32_t at = 4 * g + i;
+            x[t][i] = ((in[t] >> at) & 1) && j0 + 16 * t + at < limit ? v : GONE;
+        }
+    }
+}
+// four weights 0 .. 2^14 as signed bytes: p = (signed byte) p + 2^8 ((p + 128) >> 8)
+__device__ inline void weight_bytes(const uint32_t (&p)[4], int& lo, int& hi) {
+    const uint32_t a = p[0] | (p[1] << 16), b = p[2] | (p[3] << 16);
+    lo = (int)__builtin_amdgcn_perm(b, a, 0x06040200u);
+    hi = (int)__builtin_amdgcn_perm(b + 0x00800080u, a + 0x00800080u, 0x07050301u);
+}
+// The sums with the values' digits 0, 1, 2: o[4 f + e], dims 64 (f0 + f) + 4 (4 g + i) + e of row l.  At most 128 dims at a time (VS = 2): the sums of 256 would take
+// 192 registers, and where it then spills hipcc 7.2 copies a matrix instruction's result two instructions behind it, without the wait (seen in the assembly, and
+// as wrong sums).
+constexpr int value_steps(int ks) { return ks < 2 ? ks : 2; }
+template <int VS>
+struct Product { v4i o0[VS * 4] = {}, o1[VS * 4] = {}, o2[VS * 4] = {}; };
+template <class CT, int VS, bool QUAD>
+__device__ inline void values64(const Args& A, const RowTile& R, int f0, v4i w0, v4i w1, uint32_t j0, uint32_t k1, uint32_t g, uint32_t l, Product<VS>& P, Range& range) {
+    const bool second = __any((w1[0] | w1[1] | w1[2] | w1[3]) != 0);
+    const CT* vr[4][4];
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t j = j0 + 16 * t + 4 * g + i;
+            bool there;
+            if (i > 0 && j < k1 && (!A.table || A.log_block >= 2)) vr[t][i] = vr[t][0] + (int64_t)i * (A.table ? (int64_t)A.d : A.v.ts);
+            else vr[t][i] = key_row<CT>(A, R, min(j, k1 - 1), true, there);          // behind the end: any values, their weights are 0
+        }
+#pragma unroll
+    for (int f = 0; f < VS; f++) {
+        if (f) __builtin_amdgcn_sched_barrier(0);
+        int32_t v[4][4][4];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) fetch4<QUAD>(vr[t][i], (f0 + f) * 64 + l * 4, A.d, v[t][i]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v4i p0, p1, p2;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                int a, b, d;
+                digits4(v[t][0][e], v[t][1][e], v[t][2][e], v[t][3][e], a, b, d, range);
+                p0[t] = a; p1[t] = b; p2[t] = d;
+            }
+            const int x = f * 4 + e;
+            P.o0[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, w0, P.o0[x], 0, 0, 0);
+            P.o1[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, w0, P.o1[x], 0, 0, 0);
+            P.o2[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, w0, P.o2[x], 0, 0, 0);
+            if (second) {
+                P.o0[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, w1, v4i{}, 0, 0, 0) * 256;
+                P.o1[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, w1, v4i{}, 0, 0, 0) * 256;
+                P.o2[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, w1, v4i{}, 0, 0, 0) * 256;
+            }
+        }
+    }
+}
+// adds a wave's products to the workgroup's sums [row][dims]
+template <int VS>
+__device__ inline void add_product(const Product<VS>& P, int f0, int dims, uint32_t g, uint32_t l, unsigned long long* s_o) {
+#pragma unroll
+    for (int x = 0; x < VS * 4; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t y = (int64_t)P.o0[x][i] + ((int64_t)P.o1[x][i] << 8) + ((int64_t)P.o2[x][i] << 16);
+            atomicAdd(&s_o[l * dims + (f0 + x / 4) * 64 + (4 * g + i) * 4 + x % 4], (unsigned long long)y);
+        }
+}
+
+// ---- everything in one launch where a row's scores fit into LDS (up to FUSED_KEYS keys): 8 waves take 64 keys each in turn, the scores of 16 rows stay in LDS as scores, then
+// as e, and the rows' maxima and sums are joined there.  Few launches for short contexts and prompts, one pass over the keys instead of three.
+constexpr uint32_t FUSED_WAVES = 8;
+inline size_t fused_keys(size_t d) { return d > 128 ? 1024 : 2048; }
+inline size_t fused_pitch(size_t max_keys) { return (max_keys + 63) / 64 * 64 + 4; }
+// the scores of 16 rows and behind them the products' sums; row_exact needs 8 KB
+inline size_t fused_lds(size_t max_keys, size_t steps) { return std::max<size_t>(TILE_ROWS * fused_pitch(max_keys) * 4 + (steps > 2 ? TILE_ROWS * steps * 512 : 0), std::max<size_t>(8192, TILE_ROWS * steps * 512)); }
+
+template <class CT, int KS, bool QUAD>
+__global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint32_t pitch) {
+    constexpr int D = KS * 64;
+    extern __shared__ __align__(16) int32_t s_x[];                 // [16][pitch] scores; the sums of the products afterwards
+    __shared__ int32_t s_hi[512], s_lo[512], s_m[FUSED_WAVES][16];
+    __shared__ uint32_t s_s[FUSED_WAVES][16], s_mag[3];
+    const RowTile R = row_tile(A, blockIdx.x);
+    if (!R.any) return;
+    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, l = lane & 15;
+    const uint32_t r = R.row0 + l, rows = min(TILE_ROWS, R.n_rows - R.row0);
+    const bool mine = r < R.n_rows;
+    const uint32_t limit = mine ? min(key_limit(A, R.s, r / A.G), R.s.keys) : 0;
+    const uint32_t k1 = min(key_limit(A, R.s, (R.row0 + rows - 1) / A.G), R.s.keys);      // the most that a row of the tile sees
+    s_hi[tid] = g_exp.hi[tid]; s_lo[tid] = g_exp.lo[tid];
+    if (tid < 3) s_mag[tid] = 0;
+    __syncthreads();
+    Range rk;
+    int32_t m = GONE;
+    if (wave * 64 < k1) {
+        Query<KS> Q;
+        load_query<KS, QUAD>(A, R, r, mine, g, Q);
+#pragma unroll 1
+        for (uint32_t j0 = wave * 64; j0 < k1; j0 += FUSED_WAVES * 64) {
+            v4i x[4];
+            score64<CT, KS, QUAD>(A, R, Q, j0, k1, limit, g, l, rk, x);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                *(v4i*)(s_x + l * pitch + j0 + 16 * t + 4 * g) = x[t];
+                m = max(max(m, max(x[t][0], x[t][1])), max(x[t][2], x[t][3]));
+            }
+        }
+        atomicOr(&s_mag[0], Q.range.word());
+        atomicOr(&s_mag[1], rk.word());
+    }
+    m = max(m, __shfl_xor(m, 16));
+    m = max(m, __shfl_xor(m, 32));
+    if (g == 0) s_m[wave][l] = m;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < FUSED_WAVES; w++) m = max(m, s_m[w][l]);
+    const bool exact = ((s_mag[0] | s_mag[1]) & WIDE) || bits_of(s_mag[0]) + bits_of(s_mag[1]) + bits_of(A.d - 1) > SPLIT_BITS;
+    uint32_t sum = 0;
+#pragma unroll 1
+    for (uint32_t j0 = wave * 64; j0 < k1; j0 += FUSED_WAVES * 64)
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            v4i* at = (v4i*)(s_x + l * pitch + j0 + 16 * t + 4 * g);
+            v4i x = *at;
+#pragma unroll
+            for (int i = 0; i < 4; i++) { x[i] = x[i] == GONE ? 0 : exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo); sum += (uint32_t)x[i]; }
+            *at = x;
+        }
+    sum += (uint32_t)__shfl_xor((int)sum, 16);
+    sum += (uint32_t)__shfl_xor((int)sum, 32);
+    if (g == 0) s_s[wave][l] = sum;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < FUSED_WAVES; w++) sum += s_s[w][l];       // <= 2^25
+    const uint32_t inv = sum ? (1u << (2 * SCALE)) / sum : 0;
+    // up to 128 dims the sums take the scores' place; more dims are two sweeps over the weights, their sums lie behind the scores
+    constexpr int VS = value_steps(KS);
+    unsigned long long* s_o = (unsigned long long*)(s_x + (KS > 2 ? TILE_ROWS * pitch : 0));
+    if (KS > 2) for (uint32_t i = tid; i < rows * D; i += FUSED_WAVES * 64) s_o[i] = 0;
+    if (KS > 2) __syncthreads();
+    Range rv;
+#pragma unroll 1
+    for (int f0 = 0; f0 < KS; f0 += VS) {
+        Product<VS> P;
+#pragma unroll 1
+        for (uint32_t j0 = wave * 64; j0 < k1 && !exact; j0 += FUSED_WAVES * 64) {
+            v4i w0, w1;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const v4i e = *(const v4i*)(s_x + l * pitch + j0 + 16 * t + 4 * g);
+                uint32_t p[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[i] = __umul24((uint32_t)e[i], inv) >> SCALE;
+                int a, b;
+                weight_bytes(p, a, b);
+                w0[t] = a; w1[t] = b;
+            }
+            values64<CT, VS, QUAD>(A, R, f0, w0, w1, j0, k1, g, l, P, rv);
+        }
+        if (KS <= 2) {
+            __syncthreads();                                        // the weights have been read
+            for (uint32_t i = tid; i < rows * D; i += FUSED_WAVES * 64) s_o[i] = 0;
+            __syncthreads();
+        }
+        if (mine && wave * 64 < k1) add_product<VS>(P, f0, D, g, l, s_o);
+    }
+    atomicOr(&s_mag[2], rv.word());
+    __syncthreads();
+    if (exact || (s_mag[2] & WIDE)) {
+        for (uint32_t x = 0; x < rows; x++)
+            row_exact<CT, FUSED_WAVES * 64>(A, R.s, (R.row0 + x) / A.G, R.kvh * A.G + (R.row0 + x) % A.G, s_x, s_x + 512, (uint64_t*)(s_x + 1024));
+        return;
+    }
+    for (uint32_t i = tid; i < rows * D; i += FUSED_WAVES * 64) {
+        const uint32_t x = R.row0 + i / D, y = i % D;
+        if (y < A.d) A.out.d[(int64_t)(R.s.begin + x / A.G) * A.out.ts + (int64_t)(R.kvh * A.G + x % A.G) * A.out.hs + y] = (int32_t)((int64_t)s_o[i] >> SCALE);
+    }
+}
+
+// ---- longer contexts: four launches
+template <class CT, int KS, bool QUAD>      // KS: steps of 64 dims: 1, 2 or 4
+__global__ __launch_bounds__(256, 2) void k_split_scores(Args A, Split S) {
     const RowTile R = row_tile(A, blockIdx.x);
     const uint32_t c = blockIdx.y, k0 = c * S.chunk;
     if (!R.any || k0 >= R.s.keys) return;
@@ -67,77 +325,25 @@ __global__ __launch_bounds__(256, KS > 2 ? 1 : 2) void k_split_scores(Args A, Sp
     __shared__ uint32_t s_mag[2];
     if (tid < 2) s_mag[tid] = 0;
     __syncthreads();
-    v4i q0[KS], q1[KS], q2[KS];
-    Range rq, rk;
-    {
-        const int32_t* q = A.q.d + (int64_t)(R.s.begin + (mine ? r / A.G : 0)) * A.q.ts + (int64_t)(R.kvh * A.G + (mine ? r % A.G : 0)) * A.q.hs;
-#pragma unroll
-        for (int f = 0; f < KS; f++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                int32_t e[4];
-                const uint32_t i = f * 64 + g * 16 + x * 4;
-                fetch4<QUAD>(q, i, A.d, e);
-#pragma unroll
-                for (uint32_t y = 0; y < 4; y++) e[y] = mine && i + y < A.d ? e[y] : 0;
-                int a, b, d;
-                digits4(e[0], e[1], e[2], e[3], a, b, d, rq);
-                q0[f][x] = a; q1[f][x] = b; q2[f][x] = d;
-            }
-    }
+    Query<KS> Q;
+    load_query<KS, QUAD>(A, R, r, mine, g, Q);
+    Range rk;
     int32_t m = GONE;
     const uint32_t k1 = min(k0 + S.chunk, R.s.keys);
 #pragma unroll 1
     for (uint32_t j0 = k0 + wave * 64; j0 < k1; j0 += 256) {
-        const CT* row[4];
-        uint32_t there[4];
+        v4i x[4];
+        score64<CT, KS, QUAD>(A, R, Q, j0, k1, limit, g, l, rk, x);
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const uint32_t j = min(j0 + 16 * t + l, k1 - 1);              // behind the end: the last key again, its score does not count
-            const int64_t b = block_of(A, R.s, j);
-            row[t] = (const CT*)A.ck + cache_at(A, max(b, (int64_t)0), R.kvh, j);
-            there[t] = (uint32_t)__ballot(b >= 0 && j0 + 16 * t + l < k1) & 0xffff;
-        }
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            if (t == 2) __builtin_amdgcn_sched_barrier(0);               // two sub-tiles' loads in flight; all four would spill
-            v4i a0 = {}, a1 = {}, a2 = {}, a3 = {}, a4 = {};
-#pragma unroll
-            for (int f = 0; f < KS; f++) {
-                v4i p0, p1, p2;
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    int32_t e[4];
-                    fetch4<QUAD>(row[t], f * 64 + g * 16 + x * 4, A.d, e);
-                    int a, b, d;
-                    digits4(e[0], e[1], e[2], e[3], a, b, d, rk);
-                    p0[x] = a; p1[x] = b; p2[x] = d;
-                }
-                a4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, q2[f], a4, 0, 0, 0);
-                a3 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, q1[f], a3, 0, 0, 0);
-                a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, q0[f], a2, 0, 0, 0);
-                a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, q0[f], a1, 0, 0, 0);
-                a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, q0[f], a0, 0, 0, 0);
-                a3 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, q2[f], a3, 0, 0, 0);
-                a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, q1[f], a2, 0, 0, 0);
-                a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, q1[f], a1, 0, 0, 0);
-                a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, q2[f], a2, 0, 0, 0);
-            }
-            v4i x;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int32_t v = A.mul != ONE ? rescale(combine<KS == 4>(a0[i], a1[i], a2[i], a3[i], a4[i]), A.mul) : combine<KS == 4>(a0[i], a1[i], a2[i], a3[i], a4[i]);
-                const uint32_t at = 4 * g + i;
-                x[i] = ((there[t] >> at) & 1) && j0 + 16 * t + at < limit ? v : GONE;
-                m = max(m, x[i]);
-            }
-            if (mine) *(v4i*)(S.scores + (int64_t)id * S.pitch + j0 + 16 * t + 4 * g) = x;
+            m = max(max(m, max(x[t][0], x[t][1])), max(x[t][2], x[t][3]));
+            if (mine) *(v4i*)(S.scores + (int64_t)id * S.pitch + j0 + 16 * t + 4 * g) = x[t];
         }
     }
     m = max(m, __shfl_xor(m, 16));
     m = max(m, __shfl_xor(m, 32));
     if (g == 0) s_max[wave][l] = m;
-    atomicOr(&s_mag[0], rq.word());
+    atomicOr(&s_mag[0], Q.range.word());
     atomicOr(&s_mag[1], rk.word());
     __syncthreads();
     if (tid < 16 && mine) S.cmax[(int64_t)c * S.n_rows + id] = max(max(s_max[0][l], s_max[1][l]), max(s_max[2][l], s_max[3][l]));
@@ -175,7 +381,7 @@ __global__ __launch_bounds__(256) void k_split_sums(Args A, Split S) {
 }
 
 template <class CT, int KS, bool QUAD>
-__global__ __launch_bounds__(256, KS > 2 ? 1 : 2) void k_split_values(Args A, Split S) {
+__global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
     const RowTile R = row_tile(A, blockIdx.x);
     const uint32_t c = blockIdx.y, k0 = c * S.chunk;
     if (!R.any || k0 >= R.s.keys) return;
@@ -199,74 +405,32 @@ __global__ __launch_bounds__(256, KS > 2 ? 1 : 2) void k_split_values(Args A, Sp
         inv = sum ? (1u << (2 * SCALE)) / sum : 0;
     }
     __syncthreads();
-    v4i o0[KS * 4] = {}, o1[KS * 4] = {}, o2[KS * 4] = {};
+    constexpr int VS = value_steps(KS);
     Range rv;
     const uint32_t k1 = min(k0 + S.chunk, R.s.keys);
 #pragma unroll 1
-    for (uint32_t j0 = k0 + wave * 64; j0 < k1; j0 += 256) {
-        v4i w0 = {}, w1 = {};
-        if (mine) {
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const v4i x = *(const v4i*)(S.scores + (int64_t)id * S.pitch + j0 + 16 * t + 4 * g);
-                uint32_t p[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) p[i] = x[i] == GONE ? 0 : __umul24((uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
-                const uint32_t a = p[0] | (p[1] << 16), b = p[2] | (p[3] << 16);
-                w0[t] = (int)__builtin_amdgcn_perm(b, a, 0x06040200u);
-                w1[t] = (int)__builtin_amdgcn_perm(b + 0x00800080u, a + 0x00800080u, 0x07050301u);
-            }
-        }
-        const bool second = __any((w1[0] | w1[1] | w1[2] | w1[3]) != 0);
-        // the rows of this lane's 16 keys: 16 t + 4 g + i
-        const CT* vr[4][4];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t j = min(j0 + 16 * t + 4 * g + i, k1 - 1);      // behind the end, and in blocks that do not exist: any values, their weights are 0
-                if (i > 0 && A.log_block >= 2 && j0 + 16 * t + 4 * g + i < k1) vr[t][i] = vr[t][0] + (int64_t)i * A.d;
-                else vr[t][i] = (const CT*)A.cv + cache_at(A, max(block_of(A, R.s, j), (int64_t)0), R.kvh, j);
-            }
-#pragma unroll
-        for (int f = 0; f < KS; f++) {
-            if (f) __builtin_amdgcn_sched_barrier(0);
-            int32_t v[4][4][4];
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) fetch4<QUAD>(vr[t][i], f * 64 + l * 4, A.d, v[t][i]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v4i p0, p1, p2;
+    for (int f0 = 0; f0 < KS; f0 += VS) {
+        Product<VS> P;
+#pragma unroll 1
+        for (uint32_t j0 = k0 + wave * 64; j0 < k1; j0 += 256) {
+            v4i w0 = {}, w1 = {};
+            if (mine) {
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    int a, b, d;
-                    digits4(v[t][0][e], v[t][1][e], v[t][2][e], v[t][3][e], a, b, d, rv);
-                    p0[t] = a; p1[t] = b; p2[t] = d;
-                }
-                const int x = f * 4 + e;
-                o0[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, w0, o0[x], 0, 0, 0);
-                o1[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, w0, o1[x], 0, 0, 0);
-                o2[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, w0, o2[x], 0, 0, 0);
-                if (second) {
-                    o0[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, w1, v4i{}, 0, 0, 0) * 256;
-                    o1[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, w1, v4i{}, 0, 0, 0) * 256;
-                    o2[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, w1, v4i{}, 0, 0, 0) * 256;
+                    const v4i x = *(const v4i*)(S.scores + (int64_t)id * S.pitch + j0 + 16 * t + 4 * g);
+                    uint32_t p[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p[i] = x[i] == GONE ? 0 : __umul24((uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
+                    int a, b;
+                    weight_bytes(p, a, b);
+                    w0[t] = a; w1[t] = b;
                 }
             }
+            values64<CT, VS, QUAD>(A, R, f0, w0, w1, j0, k1, g, l, P, rv);
         }
+        if (mine) add_product<VS>(P, f0, D, g, l, s_o);
     }
     atomicOr(&s_mag, rv.word());
-    if (mine) {
-#pragma unroll
-        for (int x = 0; x < KS * 4; x++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int64_t y = (int64_t)o0[x][i] + ((int64_t)o1[x][i] << 8) + ((int64_t)o2[x][i] << 16);
-                atomicAdd(&s_o[l * D + (x / 4) * 64 + (4 * g + i) * 4 + x % 4], (unsigned long long)y);
-            }
-    }
     __syncthreads();
     const uint32_t rows = min(TILE_ROWS, R.n_rows - R.row0);
     for (uint32_t i = tid; i < rows * D; i += 256) {
