@@ -91,28 +91,29 @@ struct SplitLayout {
         bytes = at + 16;
     }
 };
+// f(steps of 64 dims, FAST)
 template <class CT, class F>
-void with_steps(uint32_t d, F f) {
-    auto dims = [&](auto quad) {
-        switch ((d + 63) / 64) {
-            case 1: f(std::integral_constant<int, 1>{}, quad); break;
-            case 2: f(std::integral_constant<int, 2>{}, quad); break;
-            default: f(std::integral_constant<int, 4>{}, quad);
+void with_steps(const Args& A, F f) {
+    auto dims = [&](auto fast) {
+        switch ((A.d + 63) / 64) {
+            case 1: f(std::integral_constant<int, 1>{}, fast); break;
+            case 2: f(std::integral_constant<int, 2>{}, fast); break;
+            default: f(std::integral_constant<int, 4>{}, fast);
         }
     };
-    if (d % 4 == 0) dims(std::true_type{}); else dims(std::false_type{});
+    if (A.d % 4 == 0 && (!A.table || A.log_block >= 4)) dims(std::true_type{}); else dims(std::false_type{});
 }
 template <class CT>
 int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
     const uint64_t wgs = (uint64_t)L.S.n_tiles * A.KV;
     if (wgs > 0x7fffffff || L.S.n_chunks > 65535 || L.segments > 65535) return fail(ATLAS_EINVAL, "attention: too many rows or keys for one call");
     const dim3 grid((unsigned)wgs, L.S.n_chunks);
-    auto run = [&](auto ks, auto quad) {
-        k_split_scores<CT, decltype(ks)::value, decltype(quad)::value><<<grid, 256, 0, stream>>>(A, L.S);
+    auto run = [&](auto ks, auto fast) {
+        k_split_scores<CT, decltype(ks)::value, decltype(fast)::value><<<grid, 256, 0, stream>>>(A, L.S);
         k_split_sums<<<dim3(L.S.n_rows, (unsigned)L.segments), 256, 0, stream>>>(A, L.S);
-        k_split_values<CT, decltype(ks)::value, decltype(quad)::value><<<grid, 256, 0, stream>>>(A, L.S);
+        k_split_values<CT, decltype(ks)::value, decltype(fast)::value><<<grid, 256, 0, stream>>>(A, L.S);
     };
-    with_steps<CT>(A.d, run);
+    with_steps<CT>(A, run);
     k_split_join<CT><<<(unsigned)wgs, 256, 0, stream>>>(A, L.S);
     return ATLAS_OK;
 }
@@ -123,9 +124,9 @@ int launch_fused(const Args& A, size_t max_keys, hipStream_t stream) {
     const uint64_t wgs = ((uint64_t)A.n_tokens * A.G / TILE_ROWS + A.n_seqs) * A.KV;
     if (wgs > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows for one call");
     int rc = ATLAS_OK;
-    with_steps<CT>(A.d, [&](auto ks, auto quad) {
+    with_steps<CT>(A, [&](auto ks, auto fast) {
         constexpr int KS = decltype(ks)::value;
-        auto* k = &k_attn_fused<CT, KS, decltype(quad)::value>;
+        auto* k = &k_attn_fused<CT, KS, decltype(fast)::value>;
         const size_t lds = fused_lds(max_keys, KS);
         if (lds > 65536 - 6144 && hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) { rc = fail(ATLAS_ENODEV, "attention: LDS"); return; }
         k<<<(unsigned)wgs, FUSED_WAVES * 64, lds, stream>>>(A, (uint32_t)fused_pitch(max_keys));

@@ -26,10 +26,10 @@ constexpr int32_t GONE = INT32_MIN;       // no score of this path reaches it: |
 constexpr uint32_t SPLIT_BITS = 44, SEGMENT = 4096, TILE_ROWS = 16;
 
 // Four elements of a row from i on, without a branch around the load: places behind the row's end get elements of the row again (they meet zeros of the
-// query, or outputs that nobody stores).  QUAD: head_dim is a multiple of 4, one vector load
-template <bool QUAD, class T>
+// query, or outputs that nobody stores).  FAST: head_dim is a multiple of 4, one vector load
+template <bool FAST, class T>
 __device__ inline void fetch4(const T* row, uint32_t i, uint32_t d, int32_t (&o)[4]) {
-    if constexpr (QUAD) {
+    if constexpr (FAST) {
         i = min(i, d - 4);
         if constexpr (sizeof(T) == 4) { const i32x4 a = *(const i32x4*)(row + i); o[0] = a[0]; o[1] = a[1]; o[2] = a[2]; o[3] = a[3]; }
         else { const i16x4 a = *(const i16x4*)(row + i); o[0] = a[0]; o[1] = a[1]; o[2] = a[2]; o[3] = a[3]; }
@@ -56,62 +56,73 @@ __device__ inline RowTile row_tile(const Args& A, uint32_t x) {
 }
 __device__ inline uint32_t row_id(const Args& A, const RowTile& t, uint32_t r) { return (t.s.begin + r / A.G) * A.H + t.kvh * A.G + r % A.G; }
 
-// ---- what the split and the fused kernels share; g = lane / 16, l = lane % 16 throughout: a lane has query row l
+// ---- what the split and the fused kernels share; g = lane / 16, l = lane % 16 throughout: a lane has query row l.
+// FAST: head_dim is a multiple of 4 and 16 keys from a multiple of 16 on lie behind each other (prompts; blocks of 16 or more): one scalar look-up for them
 template <int KS>
 struct Query { v4i q0[KS], q1[KS], q2[KS]; Range range; };
-template <int KS, bool QUAD>
+template <int KS, bool FAST>
 __device__ inline void load_query(const Args& A, const RowTile& R, uint32_t r, bool mine, uint32_t g, Query<KS>& Q) {
     const int32_t* q = A.q.d + (int64_t)(R.s.begin + (mine ? r / A.G : 0)) * A.q.ts + (int64_t)(R.kvh * A.G + (mine ? r % A.G : 0)) * A.q.hs;
+    int32_t e[KS][4][4];
+#pragma unroll
+    for (int f = 0; f < KS; f++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) fetch4<FAST>(q, f * 64 + g * 16 + x * 4, A.d, e[f][x]);
 #pragma unroll
     for (int f = 0; f < KS; f++)
 #pragma unroll
         for (int x = 0; x < 4; x++) {
-            int32_t e[4];
             const uint32_t i = f * 64 + g * 16 + x * 4;
-            fetch4<QUAD>(q, i, A.d, e);
 #pragma unroll
-            for (uint32_t y = 0; y < 4; y++) e[y] = mine && i + y < A.d ? e[y] : 0;
+            for (uint32_t y = 0; y < 4; y++) e[f][x][y] = mine && i + y < A.d ? e[f][x][y] : 0;
             int a, b, d;
-            digits4(e[0], e[1], e[2], e[3], a, b, d, Q.range);
+            digits4(e[f][x][0], e[f][x][1], e[f][x][2], e[f][x][3], a, b, d, Q.range);
             Q.q0[f][x] = a; Q.q1[f][x] = b; Q.q2[f][x] = d;
         }
 }
-// where key j's row begins (value: among the values); a block that does not exist: block 0, whose scores and weights do not count
-template <class CT>
-__device__ inline const CT* key_row(const Args& A, const RowTile& R, uint32_t j, bool value, bool& there) {
+// where key j's row begins; a block that does not exist: block 0, whose scores and weights do not count
+template <class CT, bool VALUE>
+__device__ inline const CT* key_row(const Args& A, const RowTile& R, uint32_t j, bool& there) {
     if (A.table) {
         const int64_t b = block_of(A, R.s, j);
         there = b >= 0;
-        return (const CT*)(value ? A.cv : A.ck) + cache_at(A, max(b, (int64_t)0), R.kvh, j);
+        return (const CT*)(VALUE ? A.cv : A.ck) + cache_at(A, max(b, (int64_t)0), R.kvh, j);
     }
     there = true;
-    const Rows& x = value ? A.v : A.k;
+    const Rows& x = VALUE ? A.v : A.k;
     return (const CT*)x.d + (int64_t)(R.s.begin + j) * x.ts + (int64_t)R.kvh * x.hs;
 }
-// the scores of the 64 keys from j0 on (those below k1 count), x[t][i]: key 16 t + 4 g + i
-template <class CT, int KS, bool QUAD>
-__device__ inline void score64(const Args& A, const RowTile& R, const Query<KS>& Q, uint32_t j0, uint32_t k1, uint32_t limit, uint32_t g, uint32_t l, Range& range, v4i (&x)[4]) {
-    const CT* row[4];
-    uint32_t in[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
+// 16 keys from j (a multiple of 16, below k1) as they come from memory: lane l has key j + l, dims 16 g + .. of each step; in: which of them count
+template <class CT, int KS, bool FAST>
+struct Keys16 {
+    int32_t e[KS][4][4];
+    uint32_t in;
+    __device__ void fetch(const Args& A, const RowTile& R, uint32_t j, uint32_t k1, uint32_t g, uint32_t l) {
+        const uint32_t n = min(k1 - j, 16u), o = min(l, n - 1);                 // behind the end: the last key again
+        const CT* row;
         bool there;
-        row[t] = key_row<CT>(A, R, min(j0 + 16 * t + l, k1 - 1), false, there);      // behind the end: the last key again
-        in[t] = (uint32_t)__ballot(there && j0 + 16 * t + l < k1) & 0xffff;
-    }
+        if constexpr (FAST) {
+            row = key_row<CT, false>(A, R, j, there) + (int64_t)o * (A.table ? (int64_t)A.d : A.k.ts);
+            in = there ? (1u << n) - 1 : 0;
+        } else {
+            row = key_row<CT, false>(A, R, j + o, there);
+            in = (uint32_t)__ballot(there && l < n) & 0xffff;
+        }
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-        if (t == 2) __builtin_amdgcn_sched_barrier(0);               // two sub-tiles' loads in flight; all four would spill
+        for (int f = 0; f < KS; f++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) fetch4<FAST>(row, f * 64 + g * 16 + y * 4, A.d, e[f][y]);
+    }
+    // the scores of keys j + 4 g + i against row l, GONE where one does not count
+    __device__ v4i scores(const Args& A, const Query<KS>& Q, uint32_t j, uint32_t limit, uint32_t g, Range& range) const {
         v4i a0 = {}, a1 = {}, a2 = {}, a3 = {}, a4 = {};
 #pragma unroll
         for (int f = 0; f < KS; f++) {
             v4i p0, p1, p2;
 #pragma unroll
             for (int y = 0; y < 4; y++) {
-                int32_t e[4];
-                fetch4<QUAD>(row[t], f * 64 + g * 16 + y * 4, A.d, e);
                 int a, b, d;
-                digits4(e[0], e[1], e[2], e[3], a, b, d, range);
+                digits4(e[f][y][0], e[f][y][1], e[f][y][2], e[f][y][3], a, b, d, range);
                 p0[y] = a; p1[y] = b; p2[y] = d;
             }
             a4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, Q.q2[f], a4, 0, 0, 0);
@@ -124,13 +135,31 @@ __device__ inline void score64(const Args& A, const RowTile& R, const Query<KS>&
             a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, Q.q1[f], a1, 0, 0, 0);
             a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, Q.q2[f], a2, 0, 0, 0);
         }
+        const uint32_t at = 4 * g, see = limit > j ? min(limit - j, 16u) : 0, mask = (in & ((1u << see) - 1)) >> at;
+        v4i x;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            int32_t v = combine<KS >= 3>(a0[i], a1[i], a2[i], a3[i], a4[i]);
-            if (A.mul != ONE) v = rescale(v, A.mul);
-            const uint32_t at = 4 * g + i;
-            x[t][i] = ((in[t] >> at) & 1) && j0 + 16 * t + at < limit ? v : GONE;
-        }
+        for (int i = 0; i < 4; i++) x[i] = (mask >> i) & 1 ? rescale(combine<KS == 4>(a0[i], a1[i], a2[i], a3[i], a4[i]), A.mul) : GONE;      // 2^14: the same score
+        return x;
+    }
+};
+// Every 16 keys of a wave's 64 at a time (64 of every `stride` from j0 on, below k1): the next ones are on their way while the scores of these are taken.  take(j, x)
+template <class CT, int KS, bool FAST, class F>
+__device__ inline void each_score(const Args& A, const RowTile& R, const Query<KS>& Q, uint32_t j0, uint32_t stride, uint32_t k1, uint32_t limit, uint32_t g, uint32_t l, Range& range, F take) {
+    auto next = [&](uint32_t j) { return (j & 63) == 48 ? j + 16 + stride - 64 : j + 16; };
+    Keys16<CT, KS, FAST> a, b;
+    uint32_t j = j0;
+    if (j >= k1) return;
+    a.fetch(A, R, j, k1, g, l);
+#pragma unroll 1
+    for (;;) {
+        const uint32_t j1 = next(j);
+        if (j1 < k1) b.fetch(A, R, j1, k1, g, l);
+        take(j, a.scores(A, Q, j, limit, g, range));
+        if (j1 >= k1) break;
+        j = next(j1);
+        if (j < k1) a.fetch(A, R, j, k1, g, l);
+        take(j1, b.scores(A, Q, j1, limit, g, range));
+        if (j >= k1) break;
     }
 }
 // four weights 0 .. 2^14 as signed bytes: p = (signed byte) p + 2^8 ((p + 128) >> 8)
@@ -145,27 +174,30 @@ __device__ inline void weight_bytes(const uint32_t (&p)[4], int& lo, int& hi) {
 constexpr int value_steps(int ks) { return ks < 2 ? ks : 2; }
 template <int VS>
 struct Product { v4i o0[VS * 4] = {}, o1[VS * 4] = {}, o2[VS * 4] = {}; };
-template <class CT, int VS, bool QUAD>
+// the values of the 64 keys from j0 on against the weights' bytes: byte 4 t + i of lane group g is key 16 t + 4 g + i, a lane loads 4 dims of each of its 16 keys
+template <class CT, int VS, bool FAST>
 __device__ inline void values64(const Args& A, const RowTile& R, int f0, v4i w0, v4i w1, uint32_t j0, uint32_t k1, uint32_t g, uint32_t l, Product<VS>& P, Range& range) {
     const bool second = __any((w1[0] | w1[1] | w1[2] | w1[3]) != 0);
-    const CT* vr[4][4];
+    const CT* row[4];                     // of key 16 t + 4 g (FAST)
+    const int64_t stride = A.table ? (int64_t)A.d : A.v.ts;
+    if constexpr (FAST) {
 #pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t j = j0 + 16 * t + 4 * g + i;
+        for (int t = 0; t < 4; t++) {
             bool there;
-            if (i > 0 && j < k1 && (!A.table || A.log_block >= 2)) vr[t][i] = vr[t][0] + (int64_t)i * (A.table ? (int64_t)A.d : A.v.ts);
-            else vr[t][i] = key_row<CT>(A, R, min(j, k1 - 1), true, there);          // behind the end: any values, their weights are 0
+            row[t] = key_row<CT, true>(A, R, min(j0 + 16 * t, (k1 - 1) & ~15u), there);
         }
+    }
 #pragma unroll
     for (int f = 0; f < VS; f++) {
-        if (f) __builtin_amdgcn_sched_barrier(0);
         int32_t v[4][4][4];
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) fetch4<QUAD>(vr[t][i], (f0 + f) * 64 + l * 4, A.d, v[t][i]);
+            for (int i = 0; i < 4; i++) {
+                // behind the end, and in blocks that do not exist: any values, their weights are 0
+                if constexpr (FAST) fetch4<true>(row[t] + (int64_t)min(4 * g + i, k1 - 1 - min(j0 + 16 * t, (k1 - 1) & ~15u)) * stride, (f0 + f) * 64 + l * 4, A.d, v[t][i]);
+                else { bool there; fetch4<false>(key_row<CT, true>(A, R, min(j0 + 16 * t + 4 * g + i, k1 - 1), there), (f0 + f) * 64 + l * 4, A.d, v[t][i]); }
+            }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             v4i p0, p1, p2;
@@ -207,7 +239,7 @@ inline size_t fused_pitch(size_t max_keys) { return (max_keys + 63) / 64 * 64 + 
 // the scores of 16 rows and behind them the products' sums; row_exact needs 8 KB
 inline size_t fused_lds(size_t max_keys, size_t steps) { return std::max<size_t>(TILE_ROWS * fused_pitch(max_keys) * 4 + (steps > 2 ? TILE_ROWS * steps * 512 : 0), std::max<size_t>(8192, TILE_ROWS * steps * 512)); }
 
-template <class CT, int KS, bool QUAD>
+template <class CT, int KS, bool FAST>
 __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint32_t pitch) {
     constexpr int D = KS * 64;
     extern __shared__ __align__(16) int32_t s_x[];                 // [16][pitch] scores; the sums of the products afterwards
@@ -215,7 +247,7 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
     __shared__ uint32_t s_s[FUSED_WAVES][16], s_mag[3];
     const RowTile R = row_tile(A, blockIdx.x);
     if (!R.any) return;
-    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, l = lane & 15;
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, l = lane & 15;
     const uint32_t r = R.row0 + l, rows = min(TILE_ROWS, R.n_rows - R.row0);
     const bool mine = r < R.n_rows;
     const uint32_t limit = mine ? min(key_limit(A, R.s, r / A.G), R.s.keys) : 0;
@@ -227,17 +259,13 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
     int32_t m = GONE;
     if (wave * 64 < k1) {
         Query<KS> Q;
-        load_query<KS, QUAD>(A, R, r, mine, g, Q);
-#pragma unroll 1
-        for (uint32_t j0 = wave * 64; j0 < k1; j0 += FUSED_WAVES * 64) {
-            v4i x[4];
-            score64<CT, KS, QUAD>(A, R, Q, j0, k1, limit, g, l, rk, x);
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                *(v4i*)(s_x + l * pitch + j0 + 16 * t + 4 * g) = x[t];
-                m = max(max(m, max(x[t][0], x[t][1])), max(x[t][2], x[t][3]));
-            }
-        }
+        load_query<KS, FAST>(A, R, r, mine, g, Q);
+        each_score<CT, KS, FAST>(A, R, Q, wave * 64, FUSED_WAVES * 64, k1, limit, g, l, rk, [&](uint32_t j, v4i x) {
+            *(v4i*)(s_x + l * pitch + j + 4 * g) = x;
+            m = max(max(m, max(x[0], x[1])), max(x[2], x[3]));
+        });
+        for (uint32_t j = (k1 + 15) & ~15u; j & 63; j += 16)                    // up to the next multiple of 64: no keys
+            if (wave == j / 64 % FUSED_WAVES) *(v4i*)(s_x + l * pitch + j + 4 * g) = v4i{GONE, GONE, GONE, GONE};
         atomicOr(&s_mag[0], Q.range.word());
         atomicOr(&s_mag[1], rk.word());
     }
@@ -256,7 +284,7 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
             v4i* at = (v4i*)(s_x + l * pitch + j0 + 16 * t + 4 * g);
             v4i x = *at;
 #pragma unroll
-            for (int i = 0; i < 4; i++) { x[i] = x[i] == GONE ? 0 : exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo); sum += (uint32_t)x[i]; }
+            for (int i = 0; i < 4; i++) { x[i] = exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo); sum += (uint32_t)x[i]; }      // GONE lies 2^30 below: 0
             *at = x;
         }
     sum += (uint32_t)__shfl_xor((int)sum, 16);
@@ -266,7 +294,7 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
     sum = 0;
 #pragma unroll
     for (uint32_t w = 0; w < FUSED_WAVES; w++) sum += s_s[w][l];       // <= 2^25
-    const uint32_t inv = sum ? (1u << (2 * SCALE)) / sum : 0;
+    const uint32_t inv = m == GONE ? 0 : (1u << (2 * SCALE)) / sum;       // a row that sees no key: no weights
     // up to 128 dims the sums take the scores' place; more dims are two sweeps over the weights, their sums lie behind the scores
     constexpr int VS = value_steps(KS);
     unsigned long long* s_o = (unsigned long long*)(s_x + (KS > 2 ? TILE_ROWS * pitch : 0));
@@ -289,7 +317,7 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
                 weight_bytes(p, a, b);
                 w0[t] = a; w1[t] = b;
             }
-            values64<CT, VS, QUAD>(A, R, f0, w0, w1, j0, k1, g, l, P, rv);
+            values64<CT, VS, FAST>(A, R, f0, w0, w1, j0, k1, g, l, P, rv);
         }
         if (KS <= 2) {
             __syncthreads();                                        // the weights have been read
@@ -312,12 +340,12 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
 }
 
 // ---- longer contexts: four launches
-template <class CT, int KS, bool QUAD>      // KS: steps of 64 dims: 1, 2 or 4
+template <class CT, int KS, bool FAST>      // KS: steps of 64 dims: 1, 2 or 4
 __global__ __launch_bounds__(256, 2) void k_split_scores(Args A, Split S) {
     const RowTile R = row_tile(A, blockIdx.x);
     const uint32_t c = blockIdx.y, k0 = c * S.chunk;
     if (!R.any || k0 >= R.s.keys) return;
-    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, l = lane & 15;
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, l = lane & 15;
     const uint32_t r = R.row0 + l;
     const bool mine = r < R.n_rows;
     const uint32_t id = mine ? row_id(A, R, r) : 0, limit = mine ? min(key_limit(A, R.s, r / A.G), R.s.keys) : 0;
@@ -326,20 +354,17 @@ __global__ __launch_bounds__(256, 2) void k_split_scores(Args A, Split S) {
     if (tid < 2) s_mag[tid] = 0;
     __syncthreads();
     Query<KS> Q;
-    load_query<KS, QUAD>(A, R, r, mine, g, Q);
+    load_query<KS, FAST>(A, R, r, mine, g, Q);
     Range rk;
     int32_t m = GONE;
     const uint32_t k1 = min(k0 + S.chunk, R.s.keys);
-#pragma unroll 1
-    for (uint32_t j0 = k0 + wave * 64; j0 < k1; j0 += 256) {
-        v4i x[4];
-        score64<CT, KS, QUAD>(A, R, Q, j0, k1, limit, g, l, rk, x);
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            m = max(max(m, max(x[t][0], x[t][1])), max(x[t][2], x[t][3]));
-            if (mine) *(v4i*)(S.scores + (int64_t)id * S.pitch + j0 + 16 * t + 4 * g) = x[t];
-        }
-    }
+    int32_t* to = S.scores + (int64_t)id * S.pitch + 4 * g;
+    each_score<CT, KS, FAST>(A, R, Q, k0 + wave * 64, 256, k1, limit, g, l, rk, [&](uint32_t j, v4i x) {
+        if (mine) *(v4i*)(to + j) = x;
+        m = max(max(m, max(x[0], x[1])), max(x[2], x[3]));
+    });
+    for (uint32_t j = (k1 + 15) & ~15u; j & 63; j += 16)                        // up to the next multiple of 64: no keys
+        if (mine && wave == (j - k0) / 64 % 4) *(v4i*)(to + j) = v4i{GONE, GONE, GONE, GONE};
     m = max(m, __shfl_xor(m, 16));
     m = max(m, __shfl_xor(m, 32));
     if (g == 0) s_max[wave][l] = m;
@@ -372,20 +397,20 @@ __global__ __launch_bounds__(256) void k_split_sums(Args A, Split S) {
     for (uint32_t j = seg * SEGMENT + tid * 4; j < end; j += 1024) {
         const v4i x = *(const v4i*)(S.scores + (int64_t)id * S.pitch + j);      // behind the last key: GONE up to the next multiple of 64
 #pragma unroll
-        for (int i = 0; i < 4; i++) sum += x[i] == GONE ? 0u : (uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo);      // 16 e <= 2^18 per thread
+        for (int i = 0; i < 4; i++) sum += (uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo);      // 16 e <= 2^18 per thread
     }
     for (int o = 32; o; o >>= 1) sum += (uint32_t)__shfl_xor((int)sum, o);
     if ((tid & 63) == 0) s_s[tid >> 6] = sum;
     __syncthreads();
-    if (tid == 0) { S.csum[(int64_t)seg * S.n_rows + id] = s_s[0] + s_s[1] + s_s[2] + s_s[3]; if (seg == 0) S.rmax[id] = m; }      // <= 2^26
+    if (tid == 0) { S.csum[(int64_t)seg * S.n_rows + id] = m == GONE ? 0 : s_s[0] + s_s[1] + s_s[2] + s_s[3]; if (seg == 0) S.rmax[id] = m; }      // <= 2^26
 }
 
-template <class CT, int KS, bool QUAD>
+template <class CT, int KS, bool FAST>
 __global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
     const RowTile R = row_tile(A, blockIdx.x);
     const uint32_t c = blockIdx.y, k0 = c * S.chunk;
     if (!R.any || k0 >= R.s.keys) return;
-    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, l = lane & 15;
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, l = lane & 15;
     constexpr int D = KS * 64;
     __shared__ int32_t s_hi[512], s_lo[512];
     __shared__ unsigned long long s_o[TILE_ROWS * D];
@@ -420,13 +445,13 @@ __global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
                     const v4i x = *(const v4i*)(S.scores + (int64_t)id * S.pitch + j0 + 16 * t + 4 * g);
                     uint32_t p[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) p[i] = x[i] == GONE ? 0 : __umul24((uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
+                    for (int i = 0; i < 4; i++) p[i] = __umul24((uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
                     int a, b;
                     weight_bytes(p, a, b);
                     w0[t] = a; w1[t] = b;
                 }
             }
-            values64<CT, VS, QUAD>(A, R, f0, w0, w1, j0, k1, g, l, P, rv);
+            values64<CT, VS, FAST>(A, R, f0, w0, w1, j0, k1, g, l, P, rv);
         }
         if (mine) add_product<VS>(P, f0, D, g, l, s_o);
     }

@@ -76,7 +76,7 @@ __device__ inline uint32_t last_at_most(uint32_t n, uint64_t x, F base) {
 template <class CT, int DP>
 __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
     constexpr int F = DP / 32;
-    const uint32_t tile = blockIdx.x, kvh = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+    const uint32_t tile = blockIdx.x, kvh = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     const uint32_t si = P.per_seq ? tile / P.per_seq : last_at_most(A.n_seqs, tile, [&](uint32_t s) { return (uint64_t)tile_base(A, P, s); });
     if (si >= A.n_seqs) return;
     const Seq s = seq_at(A, si);
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
     uint8_t* s_a = s_p + T::P_BYTES;
     uint8_t* s_b = s_a + (T::BUFS == 2 ? T::STEP : 0);
     uint32_t* s_red = (uint32_t*)(s_a + T::STEP * T::BUFS);        // 256 words
-    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
     const uint32_t group = wave / SPLIT, part = wave % SPLIT;
     // the kv head runs fastest: with 8 of them each XCD's L2 sees one head's planes; late tiles (many keys under the causal mask) start first
     const uint32_t kvh = blockIdx.x % A.KV, qt = gridDim.x / A.KV - 1 - blockIdx.x / A.KV;
@@ -253,11 +253,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
             a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q2[f], a2, 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            int32_t v = combine<DP == 256>(a0[i], a1[i], a2[i], a3[i], a4[i]);
-            if (A.mul != ONE) v = rescale(v, A.mul);
-            x[i] = v;
-        }
+        for (int i = 0; i < 16; i++) x[i] = combine<DP == 256>(a0[i], a1[i], a2[i], a3[i], a4[i]);
+        if (A.mul != ONE)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = rescale(x[i], A.mul);
     };
     // which of a lane's 16 keys of a sub-tile count: bit i; `all`: every one of the wave's does
     auto seen = [&](uint32_t step, int sub, bool& all) -> uint32_t {
