@@ -67,14 +67,14 @@ int launch_tiles(const Args& A, const Planes& P, size_t dp, hipStream_t stream) 
     });
 }
 
-// Few rows: the workspace of the split path.  A chunk is 128 keys or more: as many as keep the launch below about 8192 workgroups at the table's capacity
+// Few rows: the workspace of the split path.  A chunk is 128 keys or more: as many as keep the launch below about 4096 workgroups at the table's capacity
 struct SplitLayout {
     Split S{};
     size_t bytes, segments;
     SplitLayout(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys, void* ws) {
         const size_t G = s->n_heads / s->n_kv_heads, tiles = n_tokens * G / TILE_ROWS + n_seqs, rows = n_tokens * s->n_heads;
         size_t chunk = 128;
-        while (chunk < SEGMENT && tiles * s->n_kv_heads * ((max_keys + chunk - 1) / chunk) > 8192) chunk *= 2;
+        while (chunk < SEGMENT && tiles * s->n_kv_heads * ((max_keys + chunk - 1) / chunk) > 4096) chunk *= 2;
         const size_t chunks = std::max<size_t>((max_keys + chunk - 1) / chunk, 1), pitch = chunks * chunk;
         segments = std::max<size_t>((max_keys + SEGMENT - 1) / SEGMENT, 1);
         size_t at = 0;
@@ -114,7 +114,7 @@ int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
         k_split_values<CT, decltype(ks)::value, decltype(fast)::value><<<grid, 256, 0, stream>>>(A, L.S);
     };
     with_steps<CT>(A, run);
-    k_split_join<CT><<<(unsigned)wgs, 256, 0, stream>>>(A, L.S);
+    k_split_join<CT><<<L.S.n_rows, 256, 0, stream>>>(A, L.S, (uint32_t)padded_dim(A.d));
     return ATLAS_OK;
 }
 

@@ -80,15 +80,17 @@ __device__ inline void load_query(const Args& A, const RowTile& R, uint32_t r, b
             Q.q0[f][x] = a; Q.q1[f][x] = b; Q.q2[f][x] = d;
         }
 }
-// where key j's row begins; a block that does not exist: block 0, whose scores and weights do not count
+// the page table's entry for key j as a scalar load (j is uniform over the wave), -1 for a block that does not exist; prompts have no table: 0
+__device__ inline int32_t look_up(const Args& A, const RowTile& R, uint32_t j) {
+    if (!A.table) return 0;
+    const auto* t = (const __attribute__((address_space(4))) int32_t*)(A.table + (int64_t)R.s.idx * A.table_stride);
+    const int32_t b = t[__builtin_amdgcn_readfirstlane(j >> A.log_block)];
+    return (uint32_t)b < A.n_blocks ? b : -1;
+}
+// where key j's row begins, its block being known; a block that does not exist: block 0, whose scores and weights do not count
 template <class CT, bool VALUE>
-__device__ inline const CT* key_row(const Args& A, const RowTile& R, uint32_t j, bool& there) {
-    if (A.table) {
-        const int64_t b = block_of(A, R.s, j);
-        there = b >= 0;
-        return (const CT*)(VALUE ? A.cv : A.ck) + cache_at(A, max(b, (int64_t)0), R.kvh, j);
-    }
-    there = true;
+__device__ inline const CT* key_row(const Args& A, const RowTile& R, uint32_t j, int64_t block) {
+    if (A.table) return (const CT*)(VALUE ? A.cv : A.ck) + cache_at(A, max(block, (int64_t)0), R.kvh, j);
     const Rows& x = VALUE ? A.v : A.k;
     return (const CT*)x.d + (int64_t)(R.s.begin + j) * x.ts + (int64_t)R.kvh * x.hs;
 }
@@ -97,16 +99,16 @@ template <class CT, int KS, bool FAST>
 struct Keys16 {
     int32_t e[KS][4][4];
     uint32_t in;
-    __device__ void fetch(const Args& A, const RowTile& R, uint32_t j, uint32_t k1, uint32_t g, uint32_t l) {
+    __device__ void fetch(const Args& A, const RowTile& R, uint32_t j, int32_t block, uint32_t k1, uint32_t g, uint32_t l) {
         const uint32_t n = min(k1 - j, 16u), o = min(l, n - 1);                 // behind the end: the last key again
         const CT* row;
-        bool there;
         if constexpr (FAST) {
-            row = key_row<CT, false>(A, R, j, there) + (int64_t)o * (A.table ? (int64_t)A.d : A.k.ts);
-            in = there ? (1u << n) - 1 : 0;
+            row = key_row<CT, false>(A, R, j, block) + (int64_t)o * (A.table ? (int64_t)A.d : A.k.ts);
+            in = block >= 0 ? (1u << n) - 1 : 0;
         } else {
-            row = key_row<CT, false>(A, R, j + o, there);
-            in = (uint32_t)__ballot(there && l < n) & 0xffff;
+            const int64_t b = A.table ? block_of(A, R.s, j + o) : 0;
+            row = key_row<CT, false>(A, R, j + o, b);
+            in = (uint32_t)__ballot(b >= 0 && l < n) & 0xffff;
         }
 #pragma unroll
         for (int f = 0; f < KS; f++)
@@ -135,29 +137,39 @@ struct Keys16 {
             a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, Q.q1[f], a1, 0, 0, 0);
             a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, Q.q2[f], a2, 0, 0, 0);
         }
-        const uint32_t at = 4 * g, see = limit > j ? min(limit - j, 16u) : 0, mask = (in & ((1u << see) - 1)) >> at;
+        const uint32_t see = limit > j ? min(limit - j, 16u) : 0, mask = (in & ((1u << see) - 1)) >> (4 * g);
         v4i x;
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = (mask >> i) & 1 ? rescale(combine<KS == 4>(a0[i], a1[i], a2[i], a3[i], a4[i]), A.mul) : GONE;      // 2^14: the same score
+        for (int i = 0; i < 4; i++) {
+            const int32_t v = rescale(combine<KS == 4>(a0[i], a1[i], a2[i], a3[i], a4[i]), A.mul);       // 2^14: the same score
+            const int32_t keep = (int32_t)(mask << (31 - i)) >> 31;                                       // no branch
+            x[i] = (v & keep) | (GONE & ~keep);
+        }
         return x;
     }
 };
-// Every 16 keys of a wave's 64 at a time (64 of every `stride` from j0 on, below k1): the next ones are on their way while the scores of these are taken.  take(j, x)
+// Every 16 keys of a wave's 64 at a time (64 of every `stride` from j0 on, below k1): the next ones are on their way while the scores of these are taken, the
+// page of those behind them is being looked up.  take(j, x)
 template <class CT, int KS, bool FAST, class F>
 __device__ inline void each_score(const Args& A, const RowTile& R, const Query<KS>& Q, uint32_t j0, uint32_t stride, uint32_t k1, uint32_t limit, uint32_t g, uint32_t l, Range& range, F take) {
     auto next = [&](uint32_t j) { return (j & 63) == 48 ? j + 16 + stride - 64 : j + 16; };
+    auto look = [&](uint32_t j) { return FAST ? look_up(A, R, min(j, k1 - 1)) : 0; };
     Keys16<CT, KS, FAST> a, b;
     uint32_t j = j0;
     if (j >= k1) return;
-    a.fetch(A, R, j, k1, g, l);
+    int32_t page = look(j);
+    a.fetch(A, R, j, page, k1, g, l);
+    page = look(next(j));
 #pragma unroll 1
     for (;;) {
         const uint32_t j1 = next(j);
-        if (j1 < k1) b.fetch(A, R, j1, k1, g, l);
+        if (j1 < k1) b.fetch(A, R, j1, page, k1, g, l);
+        page = look(next(j1));
         take(j, a.scores(A, Q, j, limit, g, range));
         if (j1 >= k1) break;
         j = next(j1);
-        if (j < k1) a.fetch(A, R, j, k1, g, l);
+        if (j < k1) a.fetch(A, R, j, page, k1, g, l);
+        page = look(next(j));
         take(j1, b.scores(A, Q, j1, limit, g, range));
         if (j >= k1) break;
     }
@@ -174,47 +186,75 @@ __device__ inline void weight_bytes(const uint32_t (&p)[4], int& lo, int& hi) {
 constexpr int value_steps(int ks) { return ks < 2 ? ks : 2; }
 template <int VS>
 struct Product { v4i o0[VS * 4] = {}, o1[VS * 4] = {}, o2[VS * 4] = {}; };
-// the values of the 64 keys from j0 on against the weights' bytes: byte 4 t + i of lane group g is key 16 t + 4 g + i, a lane loads 4 dims of each of its 16 keys
-template <class CT, int VS, bool FAST>
-__device__ inline void values64(const Args& A, const RowTile& R, int f0, v4i w0, v4i w1, uint32_t j0, uint32_t k1, uint32_t g, uint32_t l, Product<VS>& P, Range& range) {
-    const bool second = __any((w1[0] | w1[1] | w1[2] | w1[3]) != 0);
-    const CT* row[4];                     // of key 16 t + 4 g (FAST)
-    const int64_t stride = A.table ? (int64_t)A.d : A.v.ts;
-    if constexpr (FAST) {
+// The products of 64 weights and values at a time (64 keys of every `stride` from j0 on, below k1): byte 4 t + i of lane group g is key 16 t + 4 g + i, a lane loads
+// 4 dims of each of its 16 keys.  The values of the next step are on their way from when a half's digits are taken.  weights(j, w0, w1): the weights' bytes
+template <class CT, int VS, bool FAST, class F>
+__device__ inline void each_product(const Args& A, const RowTile& R, int f0, uint32_t j0, uint32_t stride, uint32_t k1, uint32_t g, uint32_t l, Product<VS>& P, Range& range, F weights) {
+    if (j0 >= k1) return;
+    int32_t v[4][4][4];
+    int32_t page[4];
+    const int64_t step = A.table ? (int64_t)A.d : A.v.ts;
+    const uint32_t last = (k1 - 1) & ~15u;
+    auto look = [&](uint32_t j) {
+        if constexpr (FAST)
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            bool there;
-            row[t] = key_row<CT, true>(A, R, min(j0 + 16 * t, (k1 - 1) & ~15u), there);
-        }
-    }
+            for (int t = 0; t < 4; t++) page[t] = look_up(A, R, min(j + 16 * t, last));
+    };
+    // behind the end, and in blocks that do not exist: any values, their weights are 0
+    auto load = [&](uint32_t j, int f, int half) {
 #pragma unroll
-    for (int f = 0; f < VS; f++) {
-        int32_t v[4][4][4];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int t = 2 * half; t < 2 * half + 2; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                // behind the end, and in blocks that do not exist: any values, their weights are 0
-                if constexpr (FAST) fetch4<true>(row[t] + (int64_t)min(4 * g + i, k1 - 1 - min(j0 + 16 * t, (k1 - 1) & ~15u)) * stride, (f0 + f) * 64 + l * 4, A.d, v[t][i]);
-                else { bool there; fetch4<false>(key_row<CT, true>(A, R, min(j0 + 16 * t + 4 * g + i, k1 - 1), there), (f0 + f) * 64 + l * 4, A.d, v[t][i]); }
+                if constexpr (FAST) {
+                    const uint32_t jt = min(j + 16 * t, last);
+                    fetch4<true>(key_row<CT, true>(A, R, jt, page[t]) + (int64_t)min(4 * g + i, k1 - 1 - jt) * step, (f0 + f) * 64 + l * 4, A.d, v[t][i]);
+                } else {
+                    const uint32_t jt = min(j + 16 * t + 4 * g + i, k1 - 1);
+                    fetch4<false>(key_row<CT, true>(A, R, jt, A.table ? block_of(A, R.s, jt) : 0), (f0 + f) * 64 + l * 4, A.d, v[t][i]);
+                }
+            }
+    };
+    look(j0);
+    load(j0, 0, 0);
+    load(j0, 0, 1);
+#pragma unroll 1
+    for (uint32_t j = j0; j < k1; j += stride) {
+        v4i w0, w1;
+        weights(j, w0, w1);
+        const bool second = __any((w1[0] | w1[1] | w1[2] | w1[3]) != 0);
+#pragma unroll
+        for (int f = 0; f < VS; f++) {
+            v4i p[4][3];
+            if (f + 1 == VS) look(min(j + stride, last));
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int t = 2 * half; t < 2 * half + 2; t++) {
+                        int a, b, d;
+                        digits4(v[t][0][e], v[t][1][e], v[t][2][e], v[t][3][e], a, b, d, range);
+                        p[e][0][t] = a; p[e][1][t] = b; p[e][2][t] = d;
+                    }
+                if (f + 1 < VS) load(j, f + 1, half);
+                else if (j + stride < k1) load(j + stride, 0, half);
             }
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            v4i p0, p1, p2;
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                int a, b, d;
-                digits4(v[t][0][e], v[t][1][e], v[t][2][e], v[t][3][e], a, b, d, range);
-                p0[t] = a; p1[t] = b; p2[t] = d;
+            for (int e = 0; e < 4; e++) {
+                const int x = f * 4 + e;
+                P.o0[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p[e][0], w0, P.o0[x], 0, 0, 0);
+                P.o1[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p[e][1], w0, P.o1[x], 0, 0, 0);
+                P.o2[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p[e][2], w0, P.o2[x], 0, 0, 0);
             }
-            const int x = f * 4 + e;
-            P.o0[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, w0, P.o0[x], 0, 0, 0);
-            P.o1[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, w0, P.o1[x], 0, 0, 0);
-            P.o2[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, w0, P.o2[x], 0, 0, 0);
             if (second) {
-                P.o0[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p0, w1, v4i{}, 0, 0, 0) * 256;
-                P.o1[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p1, w1, v4i{}, 0, 0, 0) * 256;
-                P.o2[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p2, w1, v4i{}, 0, 0, 0) * 256;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int x = f * 4 + e;
+                    P.o0[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p[e][0], w1, v4i{}, 0, 0, 0) * 256;
+                    P.o1[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p[e][1], w1, v4i{}, 0, 0, 0) * 256;
+                    P.o2[x] += __builtin_amdgcn_mfma_i32_16x16x64_i8(p[e][2], w1, v4i{}, 0, 0, 0) * 256;
+                }
             }
         }
     }
@@ -304,21 +344,19 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
 #pragma unroll 1
     for (int f0 = 0; f0 < KS; f0 += VS) {
         Product<VS> P;
-#pragma unroll 1
-        for (uint32_t j0 = wave * 64; j0 < k1 && !exact; j0 += FUSED_WAVES * 64) {
-            v4i w0, w1;
+        if (!exact)
+            each_product<CT, VS, FAST>(A, R, f0, wave * 64, FUSED_WAVES * 64, k1, g, l, P, rv, [&](uint32_t j, v4i& w0, v4i& w1) {
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const v4i e = *(const v4i*)(s_x + l * pitch + j0 + 16 * t + 4 * g);
-                uint32_t p[4];
+                for (int t = 0; t < 4; t++) {
+                    const v4i e = *(const v4i*)(s_x + l * pitch + j + 16 * t + 4 * g);
+                    uint32_t p[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) p[i] = __umul24((uint32_t)e[i], inv) >> SCALE;
-                int a, b;
-                weight_bytes(p, a, b);
-                w0[t] = a; w1[t] = b;
-            }
-            values64<CT, VS, FAST>(A, R, f0, w0, w1, j0, k1, g, l, P, rv);
-        }
+                    for (int i = 0; i < 4; i++) p[i] = __umul24((uint32_t)e[i], inv) >> SCALE;
+                    int a, b;
+                    weight_bytes(p, a, b);
+                    w0[t] = a; w1[t] = b;
+                }
+            });
         if (KS <= 2) {
             __syncthreads();                                        // the weights have been read
             for (uint32_t i = tid; i < rows * D; i += FUSED_WAVES * 64) s_o[i] = 0;
@@ -420,7 +458,7 @@ __global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
     if (tid == 0) s_mag = 0;
     const uint32_t r = R.row0 + l;
     const bool mine = r < R.n_rows;
-    const uint32_t id = mine ? row_id(A, R, r) : 0;
+    const uint32_t id = row_id(A, R, mine ? r : R.row0);
     int32_t m = 0;
     uint32_t inv = 0;
     if (mine) {
@@ -436,23 +474,18 @@ __global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
 #pragma unroll 1
     for (int f0 = 0; f0 < KS; f0 += VS) {
         Product<VS> P;
-#pragma unroll 1
-        for (uint32_t j0 = k0 + wave * 64; j0 < k1; j0 += 256) {
-            v4i w0 = {}, w1 = {};
-            if (mine) {
+        each_product<CT, VS, FAST>(A, R, f0, k0 + wave * 64, 256, k1, g, l, P, rv, [&](uint32_t j, v4i& w0, v4i& w1) {
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const v4i x = *(const v4i*)(S.scores + (int64_t)id * S.pitch + j0 + 16 * t + 4 * g);
-                    uint32_t p[4];
+            for (int t = 0; t < 4; t++) {
+                const v4i x = *(const v4i*)(S.scores + (int64_t)id * S.pitch + j + 16 * t + 4 * g);      // lanes without a row: another's, inv is 0
+                uint32_t p[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) p[i] = __umul24((uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
-                    int a, b;
-                    weight_bytes(p, a, b);
-                    w0[t] = a; w1[t] = b;
-                }
+                for (int i = 0; i < 4; i++) p[i] = __umul24((uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
+                int a, b;
+                weight_bytes(p, a, b);
+                w0[t] = a; w1[t] = b;
             }
-            values64<CT, VS, FAST>(A, R, f0, w0, w1, j0, k1, g, l, P, rv);
-        }
+        });
         if (mine) add_product<VS>(P, f0, D, g, l, s_o);
     }
     atomicOr(&s_mag, rv.word());
@@ -465,33 +498,39 @@ __global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
     if (tid == 0) S.v_mag[(int64_t)c * gridDim.x + blockIdx.x] = s_mag;
 }
 
-// the chunks' products added up; where the operands did not fit the digits, the rows again in 64 bits
+// One workgroup per row: the chunks' products added up, every dim by 256 / DP threads; where the operands did not fit the digits, the row again in 64 bits
 template <class CT>
-__global__ __launch_bounds__(256) void k_split_join(Args A, Split S) {
-    const RowTile R = row_tile(A, blockIdx.x);
-    if (!R.any) return;
-    const uint32_t tid = threadIdx.x, chunks = (R.s.keys + S.chunk - 1) / S.chunk, rows = min(TILE_ROWS, R.n_rows - R.row0);
+__global__ __launch_bounds__(256) void k_split_join(Args A, Split S, uint32_t dp) {
+    const uint32_t id = blockIdx.x, t = id / A.H, h = id % A.H, tid = threadIdx.x, kvh = h / A.G;
+    const uint32_t si = find_seq(A.cu, A.n_seqs, t);
+    if (si >= A.n_seqs) return;
+    const Seq s = seq_at(A, si);
+    if (t < s.begin || t - s.begin >= s.n_new) return;
+    const uint32_t chunks = (s.keys + S.chunk - 1) / S.chunk;
+    const uint32_t tile = (uint32_t)((uint64_t)s.begin * A.G / TILE_ROWS) + si + ((t - s.begin) * A.G + h % A.G) / TILE_ROWS, at = tile * A.KV + kvh, tiles = S.n_tiles * A.KV;
     __shared__ uint32_t s_mag[3];
     __shared__ int32_t s_q[256], s_p[256];
     __shared__ uint64_t s_red[256];
     if (tid < 3) s_mag[tid] = 0;
     __syncthreads();
     for (uint32_t c = tid; c < chunks; c += 256) {
-        atomicOr(&s_mag[1], S.k_mag[(int64_t)c * gridDim.x + blockIdx.x]);
-        atomicOr(&s_mag[2], S.v_mag[(int64_t)c * gridDim.x + blockIdx.x]);
-        if (c == 0) atomicOr(&s_mag[0], S.q_mag[blockIdx.x]);
+        atomicOr(&s_mag[1], S.k_mag[(int64_t)c * tiles + at]);
+        atomicOr(&s_mag[2], S.v_mag[(int64_t)c * tiles + at]);
+        if (c == 0) atomicOr(&s_mag[0], S.q_mag[at]);
     }
+    const uint32_t y = tid & (dp - 1), parts = 256 / dp;
+    int64_t sum = 0;
+    if (y < A.d) for (uint32_t c = tid / dp; c < chunks; c += parts) sum += S.part[((int64_t)c * S.n_rows + id) * A.d + y];
+    s_red[tid] = (uint64_t)sum;
     __syncthreads();
     const uint32_t mq = s_mag[0], mk = s_mag[1], mv = s_mag[2];
     if (((mq | mk | mv) & WIDE) || bits_of(mq) + bits_of(mk) + bits_of(A.d - 1) > SPLIT_BITS) {
-        for (uint32_t x = 0; x < rows; x++) row_exact<CT>(A, R.s, (R.row0 + x) / A.G, R.kvh * A.G + (R.row0 + x) % A.G, s_q, s_p, s_red);
+        row_exact<CT>(A, s, t - s.begin, h, s_q, s_p, s_red);
         return;
     }
-    for (uint32_t i = tid; i < rows * A.d; i += 256) {
-        const uint32_t x = R.row0 + i / A.d, y = i % A.d, id = row_id(A, R, x);
-        int64_t sum = 0;
-        for (uint32_t c = 0; c < chunks; c++) sum += S.part[((int64_t)c * S.n_rows + id) * A.d + y];
-        A.out.d[(int64_t)(R.s.begin + x / A.G) * A.out.ts + (int64_t)(R.kvh * A.G + x % A.G) * A.out.hs + y] = (int32_t)(sum >> SCALE);
+    if (tid < A.d) {
+        for (uint32_t p = 1; p < parts; p++) sum += (int64_t)s_red[p * dp + tid];
+        A.out.d[(int64_t)t * A.out.ts + (int64_t)h * A.out.hs + tid] = (int32_t)(sum >> SCALE);
     }
 }
 

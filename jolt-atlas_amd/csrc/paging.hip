@@ -134,9 +134,13 @@ __device__ void plan_scan(const PlanArgs& P) {
             P.cu[i + 1] = bad ? 0 : (int32_t)(before.a + inc.a);
             P.lens[i] = bad ? c : P.fresh[i] < 0 ? 0 : c + (int32_t)r.tokens;
             P.ws[4 + i] = (uint32_t)(before.b + inc.b - r.need);
-            // the blocks of an ended request: its own thread copies them (they are few, and such requests too)
-            const int64_t to = n_free + (int64_t)(before.c + inc.c - r.back);
-            for (uint32_t b = 0; b < r.back; b++) P.free_[to + b] = P.table[(int64_t)i * P.table_stride + b];
+        }
+        // the blocks of ended requests: their waves copy them, 64 entries at a time (one thread per request took 85 us where 120 of 4000 requests ended)
+        for (uint64_t todo = __ballot(r.back != 0); todo; todo &= todo - 1) {
+            const int from = __builtin_ctzll(todo);
+            const uint32_t who = i0 + (tid & ~63u) + from, n = __shfl(r.back, from);
+            const int64_t to = n_free + (int64_t)__shfl((unsigned long long)(before.c + inc.c - r.back), from);
+            for (uint32_t b = tid & 63; b < n; b += 64) P.free_[to + b] = P.table[(int64_t)who * P.table_stride + b];
         }
         before.a += all.a; before.b += all.b; before.c += all.c;
     }
