@@ -67,27 +67,25 @@ int launch_tiles(const Args& A, const Planes& P, size_t dp, hipStream_t stream) 
     });
 }
 
-// Few rows: the workspace of the split path.  A chunk is 128 keys or more: as many as keep the launch below about 4096 workgroups at the table's capacity
+// Few rows: the workspace of the split path
 struct SplitLayout {
     Split S{};
-    size_t bytes, segments;
+    size_t bytes;
     SplitLayout(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys, void* ws) {
-        const size_t G = s->n_heads / s->n_kv_heads, tiles = n_tokens * G / TILE_ROWS + n_seqs, rows = n_tokens * s->n_heads;
-        size_t chunk = 128;
-        while (chunk < SEGMENT && tiles * s->n_kv_heads * ((max_keys + chunk - 1) / chunk) > 4096) chunk *= 2;
-        const size_t chunks = std::max<size_t>((max_keys + chunk - 1) / chunk, 1), pitch = chunks * chunk;
-        segments = std::max<size_t>((max_keys + SEGMENT - 1) / SEGMENT, 1);
+        const size_t G = s->n_heads / s->n_kv_heads, tiles = n_tokens * G / TILE_ROWS + n_seqs, rows = n_tokens * s->n_heads, parts = WGS * TILE_ROWS + rows, mags = WGS + tiles * s->n_kv_heads;
+        const size_t pitch = (max_keys + 63) / 64 * 64;
         size_t at = 0;
         auto take = [&](size_t n) { const size_t was = at; at += (n + 15) / 16 * 16; return (uint8_t*)ws + was; };
-        S.chunk = (uint32_t)chunk; S.n_chunks = (uint32_t)chunks; S.n_tiles = (uint32_t)tiles; S.n_rows = (uint32_t)rows; S.pitch = (int64_t)pitch;
+        S.n_tiles = (uint32_t)tiles; S.n_rows = (uint32_t)rows; S.pitch = (int64_t)pitch;
         S.scores = (int32_t*)take(rows * pitch * 4);
-        S.part = (int64_t*)take(chunks * rows * s->head_dim * 8);
-        S.cmax = (int32_t*)take(chunks * rows * 4);
-        S.csum = (uint32_t*)take(segments * rows * 4);
-        S.rmax = (int32_t*)take(rows * 4);
-        S.q_mag = (uint32_t*)take(tiles * s->n_kv_heads * 4);
-        S.k_mag = (uint32_t*)take(chunks * tiles * s->n_kv_heads * 4);
-        S.v_mag = (uint32_t*)take(chunks * tiles * s->n_kv_heads * 4);
+        S.part = (int64_t*)take(parts * s->head_dim * 8);
+        S.cmax = (int32_t*)take(parts * 4);
+        S.csum = (uint32_t*)take(parts * 4);
+        S.q_mag = (uint32_t*)take(mags * 4);
+        S.k_mag = (uint32_t*)take(mags * 4);
+        S.v_mag = (uint32_t*)take(mags * 4);
+        S.units = (uint32_t*)take((tiles + 1) * 4);
+        S.rows = (uint32_t*)take((tiles + 1) * 4);
         bytes = at + 16;
     }
 };
@@ -105,20 +103,25 @@ void with_steps(const Args& A, F f) {
 }
 template <class CT>
 int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
-    const uint64_t wgs = (uint64_t)L.S.n_tiles * A.KV;
-    if (wgs > 0x7fffffff || L.S.n_chunks > 65535 || L.segments > 65535) return fail(ATLAS_EINVAL, "attention: too many rows or keys for one call");
-    const dim3 grid((unsigned)wgs, L.S.n_chunks);
-    auto run = [&](auto ks, auto fast) {
-        k_split_scores<CT, decltype(ks)::value, decltype(fast)::value><<<grid, 256, 0, stream>>>(A, L.S);
-        k_split_sums<<<dim3(L.S.n_rows, (unsigned)L.segments), 256, 0, stream>>>(A, L.S);
-        k_split_values<CT, decltype(ks)::value, decltype(fast)::value><<<grid, 256, 0, stream>>>(A, L.S);
-    };
-    with_steps<CT>(A, run);
+    // rows, parts, magnitudes and units are counted in 32 bits
+    const uint64_t tiles = (uint64_t)A.n_tokens * A.G / TILE_ROWS + A.n_seqs, units = ((uint64_t)A.max_keys + UNIT - 1) / UNIT;
+    if ((uint64_t)A.n_tokens * A.H > 0x40000000 || tiles * A.KV > 0x40000000 || tiles * A.KV * units > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows and keys for one call");
+    k_split_plan<<<1, 1024, 0, stream>>>(A, L.S);
+    with_steps<CT>(A, [&](auto ks, auto fast) {
+        k_split_scores<CT, decltype(ks)::value, decltype(fast)::value><<<WGS, 256, 0, stream>>>(A, L.S);
+        k_split_sums<<<WGS, 256, 0, stream>>>(A, L.S);
+        k_split_values<CT, decltype(ks)::value, decltype(fast)::value><<<WGS, 256, 0, stream>>>(A, L.S);
+    });
     k_split_join<CT><<<L.S.n_rows, 256, 0, stream>>>(A, L.S, (uint32_t)padded_dim(A.d));
     return ATLAS_OK;
 }
 
-bool fused(size_t max_keys, size_t d) { return max_keys <= fused_keys(d); }
+// One launch while LDS holds the scores — up to 1024 keys, beyond that only where there are workgroups enough for the chip: 16 heads of 64 over 1000 / 2000 keys
+// take 27 / 42 us in one launch of 16 workgroups and 30 / 31 us in the split path's five launches
+bool fused(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys) {
+    const size_t wgs = (n_tokens * (s->n_heads / s->n_kv_heads) / TILE_ROWS + n_seqs) * s->n_kv_heads;
+    return max_keys <= 1024 || (max_keys <= fused_keys(s->head_dim) && wgs >= 256);
+}
 template <class CT>
 int launch_fused(const Args& A, size_t max_keys, hipStream_t stream) {
     const uint64_t wgs = ((uint64_t)A.n_tokens * A.G / TILE_ROWS + A.n_seqs) * A.KV;
@@ -140,7 +143,7 @@ extern "C" {
 
 size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens)) return 0;
-    return fused(n_tokens, shape->head_dim) ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
+    return fused(shape, n_seqs, n_tokens, n_tokens) ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
 }
 
 int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
@@ -162,7 +165,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (int rc = L.on_device({q->d, k->d, v->d, d_cu_seqlens, out->d, d_workspace})) return rc;
     Args A = args_of(shape, q, d_cu_seqlens, n_seqs, n_tokens, out);
     A.k = rows_of(k); A.v = rows_of(v);
-    if (fused(n_tokens, A.d)) {
+    if (fused(shape, n_seqs, n_tokens, n_tokens)) {
         if (int rc = launch_fused<int32_t>(A, n_tokens, L.stream)) return rc;
         return L.end();
     }
@@ -173,7 +176,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
 
 size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
-    if (fused(max_blocks * cache->block_size, shape->head_dim)) return 16;
+    if (fused(shape, n_seqs, n_tokens, max_blocks * cache->block_size)) return 16;
     return many_rows(n_seqs, n_tokens) ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_blocks * cache->block_size, 1)).bytes
                                        : SplitLayout(shape, n_seqs, n_tokens, max_blocks * cache->block_size, nullptr).bytes;
 }
@@ -198,7 +201,7 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     Args A = args_of(shape, q, d_cu_new, n_seqs, n_tokens, out);
     A.ck = cache->d_k; A.cv = cache->d_v; A.lens = d_kv_lens; A.table = d_block_table; A.table_stride = (int64_t)table_stride;
     A.n_blocks = (uint32_t)cache->n_blocks; A.log_block = log2_of(cache->block_size); A.max_keys = (uint32_t)(max_blocks * cache->block_size);
-    if (fused(A.max_keys, A.d)) {
+    if (fused(shape, n_seqs, n_tokens, A.max_keys)) {
         if (int rc = cache->bits == 16 ? launch_fused<int16_t>(A, A.max_keys, L.stream) : launch_fused<int32_t>(A, A.max_keys, L.stream)) return rc;
         return L.end();
     }

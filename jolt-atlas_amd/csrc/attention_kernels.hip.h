@@ -119,12 +119,23 @@ __device__ void row_exact(const Args& A, const Seq& s, uint32_t i, uint32_t h, i
     __syncthreads();
 }
 
-// the last sequence whose offset is <= t, or n_seqs where t lies behind the last one
+// The largest s below n with base(s) <= x (base increasing, base(0) <= x), by all 64 lanes of a wave: 64 places per dependent load (one binary search
+// per workgroup was 3 us of every launch).  Offsets that do not increase give some s below n.
+template <class F>
+__device__ inline uint32_t last_at_most(uint32_t n, uint64_t x, F base) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = 0;
+    while (n > 1) {
+        const uint32_t step = (n + 63) / 64, at = lane * step;
+        const uint32_t hit = (uint32_t)__popcll(__ballot(at < n && base(lo + at) <= x)), skip = (hit ? hit - 1 : 0) * step;
+        lo += skip;
+        n = min(step, n - skip);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+// the sequence that token t (uniform over the wave) belongs to, or n_seqs where it lies behind the last one
 __device__ inline uint32_t find_seq(const int32_t* cu, uint32_t n_seqs, uint32_t t) {
-    if ((int64_t)t >= cu[n_seqs]) return n_seqs;
-    uint32_t lo = 0, hi = n_seqs;                                    // cu[lo] <= t < cu[hi]
-    while (hi - lo > 1) { const uint32_t mid = (lo + hi) / 2; if ((int64_t)t >= cu[mid]) lo = mid; else hi = mid; }
-    return lo;
+    return (int64_t)t >= cu[n_seqs] ? n_seqs : last_at_most(n_seqs, t, [&](uint32_t s) { return (uint64_t)max(cu[s], 0); });
 }
 
 }  // namespace atlas_attn

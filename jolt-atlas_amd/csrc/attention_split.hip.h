@@ -1,10 +1,10 @@
-// The quantised attention of few query rows over long caches (decoding): bound by reading the cache once.  The keys of a sequence are split over workgroups in chunks,
-// and four launches join them: k_split_scores (reads the keys, keeps the scores and each chunk's maximum), k_split_sums, k_split_values (reads the values), k_split_join.
-// Splitting costs nothing in exactness: maxima and integer sums do not depend on the order.
+// The quantised attention of few query rows (decoding): bound by reading the cache once.  Up to 16 rows (the heads that share a kv head, times the new tokens) are the
+// columns of v_mfma_i32_16x16x64_i8.  Keys go from memory into the fragments' own lanes (16 dims of one key: 64 contiguous bytes) and are cut into digits in
+// registers, values the same with 4 dims of 16 keys per lane; nothing passes through LDS.
 //
-// Up to 16 rows (the heads that share a kv head, times the new tokens) are the columns of v_mfma_i32_16x16x64_i8.  Keys go from memory into the fragments' own lanes
-// (16 dims of one key: 64 contiguous bytes) and are cut into digits in registers, values the same with 4 dims of 16 keys per lane; nothing
-// passes through LDS.  About 4.3 vector operations per element against 32 that the memory's rate leaves room for.
+// Short contexts take one launch (k_attn_fused).  Longer ones five: k_split_plan lays the keys of all row tiles and kv heads behind each other in units of 256 and
+// k_split_scores, k_split_sums and k_split_values give each of WGS workgroups the same share of that line, wherever sequences begin and end; k_split_join adds the
+// shares of a row up.  Splitting costs nothing in exactness: maxima and integer sums do not depend on the order.
 #pragma once
 #include <algorithm>
 
@@ -13,17 +13,17 @@
 namespace atlas_attn {
 
 struct Split {
-    int32_t* scores;             // [row][pitch]; row = token * heads + head; GONE where no key counts
-    int32_t* cmax;               // [chunk][row]
-    uint32_t* csum;              // [segment][row]
-    int32_t* rmax;               // [row]
-    uint32_t *q_mag, *k_mag, *v_mag;      // [row tile * kv heads + kv head], the latter two by chunk in front
-    int64_t* part;               // [chunk][row][d]
-    uint32_t chunk, n_chunks, n_tiles, n_rows;
+    uint32_t *units, *rows;      // [tile]: units of 256 keys, rows, of one kv head before this tile; one entry more
+    int32_t* scores;             // [row][pitch], rows in the line's order; GONE where no key counts
+    int32_t* cmax;               // [part]: a share's rows follow each other at part_at()
+    uint32_t* csum;              // [part]
+    int64_t* part;               // [part][d]
+    uint32_t *q_mag, *k_mag, *v_mag;      // [workgroup + stretch]
+    uint32_t n_tiles, n_rows;
     int64_t pitch;
 };
 constexpr int32_t GONE = INT32_MIN;       // no score of this path reaches it: |score| < 2^30 (SPLIT_BITS)
-constexpr uint32_t SPLIT_BITS = 44, SEGMENT = 4096, TILE_ROWS = 16;
+constexpr uint32_t SPLIT_BITS = 44, UNIT = 256, WGS = 1024, TILE_ROWS = 16;
 
 // Four elements of a row from i on, without a branch around the load: places behind the row's end get elements of the row again (they meet zeros of the
 // query, or outputs that nobody stores).  FAST: head_dim is a multiple of 4, one vector load
@@ -40,21 +40,20 @@ __device__ inline void fetch4(const T* row, uint32_t i, uint32_t d, int32_t (&o)
 }
 
 // the rows of a workgroup: 16 (token, head of the group) pairs of one sequence
-struct RowTile { Seq s; uint32_t row0, n_rows, tile, kvh; bool any; };
-__device__ inline RowTile row_tile(const Args& A, uint32_t x) {
+struct RowTile { Seq s; uint32_t row0, n_rows, kvh; bool any; };
+__device__ inline RowTile row_tile(const Args& A, uint32_t tile, uint32_t kvh) {
     RowTile t;
-    t.kvh = x % A.KV; t.tile = x / A.KV;
+    t.kvh = kvh;
     auto base = [&](uint32_t s) { return (uint64_t)min((uint32_t)max(A.cu[s], 0), A.n_tokens) * A.G / TILE_ROWS + s; };
-    const uint32_t si = last_at_most(A.n_seqs, t.tile, base);
+    const uint32_t si = last_at_most(A.n_seqs, tile, base);
     t.s = seq_at(A, si);
     t.n_rows = t.s.n_new * A.G;
     const uint64_t b = base(si);
-    const uint64_t first = t.tile >= b ? (t.tile - b) * TILE_ROWS : ~0ull;
+    const uint64_t first = tile >= b ? (tile - b) * TILE_ROWS : ~0ull;
     t.any = first < t.n_rows;
     t.row0 = (uint32_t)first;
     return t;
 }
-__device__ inline uint32_t row_id(const Args& A, const RowTile& t, uint32_t r) { return (t.s.begin + r / A.G) * A.H + t.kvh * A.G + r % A.G; }
 
 // ---- what the split and the fused kernels share; g = lane / 16, l = lane % 16 throughout: a lane has query row l.
 // FAST: head_dim is a multiple of 4 and 16 keys from a multiple of 16 on lie behind each other (prompts; blocks of 16 or more): one scalar look-up for them
@@ -285,7 +284,7 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
     extern __shared__ __align__(16) int32_t s_x[];                 // [16][pitch] scores; the sums of the products afterwards
     __shared__ int32_t s_hi[512], s_lo[512], s_m[FUSED_WAVES][16];
     __shared__ uint32_t s_s[FUSED_WAVES][16], s_mag[3];
-    const RowTile R = row_tile(A, blockIdx.x);
+    const RowTile R = row_tile(A, blockIdx.x / A.KV, blockIdx.x % A.KV);
     if (!R.any) return;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, l = lane & 15;
     const uint32_t r = R.row0 + l, rows = min(TILE_ROWS, R.n_rows - R.row0);
@@ -377,150 +376,226 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
     }
 }
 
-// ---- longer contexts: four launches
-template <class CT, int KS, bool FAST>      // KS: steps of 64 dims: 1, 2 or 4
-__global__ __launch_bounds__(256, 2) void k_split_scores(Args A, Split S) {
-    const RowTile R = row_tile(A, blockIdx.x);
-    const uint32_t c = blockIdx.y, k0 = c * S.chunk;
-    if (!R.any || k0 >= R.s.keys) return;
-    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, l = lane & 15;
-    const uint32_t r = R.row0 + l;
-    const bool mine = r < R.n_rows;
-    const uint32_t id = mine ? row_id(A, R, r) : 0, limit = mine ? min(key_limit(A, R.s, r / A.G), R.s.keys) : 0;
-    __shared__ int32_t s_max[4][16];
-    __shared__ uint32_t s_mag[2];
-    if (tid < 2) s_mag[tid] = 0;
-    __syncthreads();
-    Query<KS> Q;
-    load_query<KS, FAST>(A, R, r, mine, g, Q);
-    Range rk;
-    int32_t m = GONE;
-    const uint32_t k1 = min(k0 + S.chunk, R.s.keys);
-    int32_t* to = S.scores + (int64_t)id * S.pitch + 4 * g;
-    each_score<CT, KS, FAST>(A, R, Q, k0 + wave * 64, 256, k1, limit, g, l, rk, [&](uint32_t j, v4i x) {
-        if (mine) *(v4i*)(to + j) = x;
-        m = max(max(m, max(x[0], x[1])), max(x[2], x[3]));
-    });
-    for (uint32_t j = (k1 + 15) & ~15u; j & 63; j += 16)                        // up to the next multiple of 64: no keys
-        if (mine && wave == (j - k0) / 64 % 4) *(v4i*)(to + j) = v4i{GONE, GONE, GONE, GONE};
-    m = max(m, __shfl_xor(m, 16));
-    m = max(m, __shfl_xor(m, 32));
-    if (g == 0) s_max[wave][l] = m;
-    atomicOr(&s_mag[0], Q.range.word());
-    atomicOr(&s_mag[1], rk.word());
-    __syncthreads();
-    if (tid < 16 && mine) S.cmax[(int64_t)c * S.n_rows + id] = max(max(s_max[0][l], s_max[1][l]), max(s_max[2][l], s_max[3][l]));
-    if (tid == 0) { S.k_mag[(int64_t)c * gridDim.x + blockIdx.x] = s_mag[1]; if (c == 0) S.q_mag[blockIdx.x] = s_mag[0]; }
+// ---- longer contexts
+// One workgroup: the prefix sums of the tiles' units and rows
+__global__ __launch_bounds__(1024) void k_split_plan(Args A, Split S) {
+    __shared__ uint32_t s_u[16], s_r[16];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t u0 = 0, r0 = 0;
+    for (uint32_t i0 = 0; i0 < S.n_tiles; i0 += 1024) {
+        const uint32_t i = i0 + tid;
+        uint32_t u = 0, r = 0;
+        if (i < S.n_tiles) {
+            auto base = [&](uint32_t s) { return (uint64_t)min((uint32_t)max(A.cu[s], 0), A.n_tokens) * A.G / TILE_ROWS + s; };
+            uint32_t lo = 0, hi = A.n_seqs;                        // every thread has a tile of its own: a binary search each
+            while (hi - lo > 1) { const uint32_t mid = (lo + hi) / 2; if (base(mid) <= i) lo = mid; else hi = mid; }
+            const Seq s = seq_at(A, lo);
+            const uint64_t b = base(lo), first = i >= b ? (i - b) * TILE_ROWS : ~0ull;
+            if (first < (uint64_t)s.n_new * A.G) { r = min(TILE_ROWS, s.n_new * A.G - (uint32_t)first); u = (s.keys + UNIT - 1) / UNIT; }
+        }
+        const uint32_t u_mine = u, r_mine = r;
+#pragma unroll
+        for (uint32_t o = 1; o < 64; o <<= 1) { const uint32_t a = __shfl_up(u, o), b = __shfl_up(r, o); if (lane >= o) { u += a; r += b; } }
+        if (lane == 63) { s_u[wave] = u; s_r[wave] = r; }
+        __syncthreads();
+        uint32_t ut = 0, rt = 0;
+        for (uint32_t w = 0; w < 16; w++) { if (w < wave) { u += s_u[w]; r += s_r[w]; } ut += s_u[w]; rt += s_r[w]; }
+        if (i < S.n_tiles) { S.units[i] = u0 + u - u_mine; S.rows[i] = r0 + r - r_mine; }
+        u0 += ut; r0 += rt;
+        __syncthreads();
+    }
+    if (tid == 0) { S.units[S.n_tiles] = u0; S.rows[S.n_tiles] = r0; }
+}
+// The line's units over the workgroups: n of them have a share, the first `more` of them per + 1 units and the others per
+struct Line {
+    uint32_t n, per, more;
+    __device__ Line(const Args& A, const Split& S) { const uint32_t U = S.units[S.n_tiles] * A.KV; n = max(min(U, WGS), 1u); per = U / n; more = U % n; }
+    __device__ uint32_t begin(uint32_t w) const { return min(w, n) * per + min(w, more); }
+    __device__ uint32_t owner(uint32_t u) const { const uint32_t x = more * (per + 1); return u < x ? u / (per + 1) : more + (u - x) / per; }
+};
+// a stretch of the line: keys [k0, k1) of a row tile under one kv head
+struct Stretch {
+    RowTile R;
+    uint32_t tile, units, k0, k1, part, row, mag, n;      // part: of its first row in cmax, csum, part; row: of its first row in scores; mag: its place in the magnitudes; n: its rows
+};
+// what workgroup w has from unit u on (u < end, the end of its share)
+__device__ inline Stretch stretch_at(const Args& A, const Split& S, uint32_t w, uint32_t u, uint32_t end) {
+    Stretch x;
+    const uint32_t t = x.tile = last_at_most(S.n_tiles, u, [&](uint32_t i) { return (uint64_t)S.units[i] * A.KV; });
+    const uint32_t per = max(S.units[t + 1] - S.units[t], 1u), rel = u - S.units[t] * A.KV, kvh = min(rel / per, A.KV - 1), at = rel % per;
+    x.R = row_tile(A, t, kvh);
+    x.units = min(per - at, end - u);
+    x.k0 = at * UNIT;
+    x.k1 = min((at + x.units) * UNIT, x.R.s.keys);
+    x.n = S.rows[t + 1] - S.rows[t];
+    x.row = S.rows[t] * A.KV + kvh * x.n;
+    x.part = w * TILE_ROWS + x.row;          // a next stretch of w lies n further, the same rows' share of w + 1 16 further: no two overlap
+    x.mag = w + t * A.KV + kvh;
+    return x;
 }
 
-// one workgroup per row and segment of 4096 keys
-__global__ __launch_bounds__(256) void k_split_sums(Args A, Split S) {
-    const uint32_t id = blockIdx.x, t = id / A.H, seg = blockIdx.y, tid = threadIdx.x;
-    const uint32_t si = find_seq(A.cu, A.n_seqs, t);
-    if (si >= A.n_seqs) return;
-    const Seq s = seq_at(A, si);
-    if (t < s.begin || t - s.begin >= s.n_new || seg * SEGMENT >= s.keys) return;
-    __shared__ int32_t s_hi[512], s_lo[512], s_m[4];
-    __shared__ uint32_t s_s[4];
-    for (uint32_t i = tid; i < 512; i += 256) { s_hi[i] = g_exp.hi[i]; s_lo[i] = g_exp.lo[i]; }
-    const uint32_t chunks = (s.keys + S.chunk - 1) / S.chunk;
-    int32_t m = GONE;
-    for (uint32_t c = tid; c < chunks; c += 256) m = max(m, S.cmax[(int64_t)c * S.n_rows + id]);
-    for (int o = 32; o; o >>= 1) m = max(m, __shfl_xor(m, o));
-    if ((tid & 63) == 0) s_m[tid >> 6] = m;
-    __syncthreads();
-    m = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3]));
-    const uint32_t end = min((seg + 1) * SEGMENT, s.keys);
-    uint32_t sum = 0;
-    for (uint32_t j = seg * SEGMENT + tid * 4; j < end; j += 1024) {
-        const v4i x = *(const v4i*)(S.scores + (int64_t)id * S.pitch + j);      // behind the last key: GONE up to the next multiple of 64
-#pragma unroll
-        for (int i = 0; i < 4; i++) sum += (uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo);      // 16 e <= 2^18 per thread
+template <class CT, int KS, bool FAST>      // KS: steps of 64 dims: 1, 2 or 4
+__global__ __launch_bounds__(256, 2) void k_split_scores(Args A, Split S) {
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, l = lane & 15;
+    __shared__ int32_t s_max[4][16];
+    __shared__ uint32_t s_mag[2];
+    const Line line(A, S);
+    const uint32_t end = line.begin(blockIdx.x + 1);
+#pragma unroll 1
+    for (uint32_t u = line.begin(blockIdx.x); u < end;) {
+        const Stretch X = stretch_at(A, S, blockIdx.x, u, end);
+        const RowTile& R = X.R;
+        u += X.units;
+        const uint32_t r = R.row0 + l;
+        const bool mine = l < X.n;
+        const uint32_t limit = mine ? min(key_limit(A, R.s, r / A.G), R.s.keys) : 0;
+        if (tid < 2) s_mag[tid] = 0;
+        __syncthreads();
+        Query<KS> Q;
+        load_query<KS, FAST>(A, R, r, mine, g, Q);
+        Range rk;
+        int32_t m = GONE;
+        int32_t* to = S.scores + (int64_t)(X.row + (mine ? l : 0)) * S.pitch + 4 * g;
+        each_score<CT, KS, FAST>(A, R, Q, X.k0 + wave * 64, UNIT, X.k1, limit, g, l, rk, [&](uint32_t j, v4i x) {
+            if (mine) *(v4i*)(to + j) = x;
+            m = max(max(m, max(x[0], x[1])), max(x[2], x[3]));
+        });
+        for (uint32_t j = (X.k1 + 15) & ~15u; j & 63; j += 16)                      // up to the next multiple of 64: no keys
+            if (mine && wave == j / 64 % 4) *(v4i*)(to + j) = v4i{GONE, GONE, GONE, GONE};
+        m = max(m, __shfl_xor(m, 16));
+        m = max(m, __shfl_xor(m, 32));
+        if (g == 0) s_max[wave][l] = m;
+        atomicOr(&s_mag[0], Q.range.word());
+        atomicOr(&s_mag[1], rk.word());
+        __syncthreads();
+        if (tid < X.n) S.cmax[X.part + tid] = max(max(s_max[0][l], s_max[1][l]), max(s_max[2][l], s_max[3][l]));
+        if (tid == 0) { S.q_mag[X.mag] = s_mag[0]; S.k_mag[X.mag] = s_mag[1]; }
+        __syncthreads();
     }
-    for (int o = 32; o; o >>= 1) sum += (uint32_t)__shfl_xor((int)sum, o);
-    if ((tid & 63) == 0) s_s[tid >> 6] = sum;
+}
+
+// A row's value over the shares of its stretch: `with` over the places of the shares' parts
+template <class F>
+__device__ inline void each_share(const Args& A, const Split& S, uint32_t t, uint32_t kvh, uint32_t first, uint32_t step, F with) {
+    const uint32_t per = S.units[t + 1] - S.units[t], n = S.rows[t + 1] - S.rows[t];
+    if (per == 0) return;
+    const Line line(A, S);
+    const uint32_t p = S.units[t] * A.KV + kvh * per, w1 = line.owner(p + per - 1);
+    for (uint32_t w = line.owner(p) + first; w <= w1; w += step) with(w * TILE_ROWS + S.rows[t] * A.KV + kvh * n, w + t * A.KV + kvh);
+}
+
+// a wave takes a row of the share at a time, 256 keys by 4 per lane
+__global__ __launch_bounds__(256) void k_split_sums(Args A, Split S) {
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    __shared__ int32_t s_hi[512], s_lo[512];
+    for (uint32_t i = tid; i < 512; i += 256) { s_hi[i] = g_exp.hi[i]; s_lo[i] = g_exp.lo[i]; }
     __syncthreads();
-    if (tid == 0) { S.csum[(int64_t)seg * S.n_rows + id] = m == GONE ? 0 : s_s[0] + s_s[1] + s_s[2] + s_s[3]; if (seg == 0) S.rmax[id] = m; }      // <= 2^26
+    const Line line(A, S);
+    const uint32_t end = line.begin(blockIdx.x + 1);
+#pragma unroll 1
+    for (uint32_t u = line.begin(blockIdx.x); u < end;) {
+        const Stretch X = stretch_at(A, S, blockIdx.x, u, end);
+        u += X.units;
+        const uint32_t t = X.tile;
+        for (uint32_t r = wave; r < X.n; r += 4) {
+            int32_t m = GONE;
+            each_share(A, S, t, X.R.kvh, lane, 64, [&](uint32_t part, uint32_t) { m = max(m, S.cmax[part + r]); });
+            for (int o = 32; o; o >>= 1) m = max(m, __shfl_xor(m, o));
+            uint32_t sum = 0;
+            for (uint32_t j = X.k0 + lane * 4; j < X.k1; j += 256) {
+                const v4i x = *(const v4i*)(S.scores + (int64_t)(X.row + r) * S.pitch + j);      // behind the last key: GONE up to the next multiple of 64
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum = __builtin_elementwise_add_sat(sum, (uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo));
+            }
+            for (int o = 32; o; o >>= 1) sum = __builtin_elementwise_add_sat(sum, (uint32_t)__shfl_xor((int)sum, o));
+            if (lane == 0) S.csum[X.part + r] = m == GONE ? 0 : sum;
+        }
+    }
 }
 
 template <class CT, int KS, bool FAST>
 __global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
-    const RowTile R = row_tile(A, blockIdx.x);
-    const uint32_t c = blockIdx.y, k0 = c * S.chunk;
-    if (!R.any || k0 >= R.s.keys) return;
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, l = lane & 15;
-    constexpr int D = KS * 64;
-    __shared__ int32_t s_hi[512], s_lo[512];
+    constexpr int D = KS * 64, VS = value_steps(KS);
+    __shared__ int32_t s_hi[512], s_lo[512], s_m[16];
+    __shared__ uint32_t s_sum[16];
     __shared__ unsigned long long s_o[TILE_ROWS * D];
     __shared__ uint32_t s_mag;
     for (uint32_t i = tid; i < 512; i += 256) { s_hi[i] = g_exp.hi[i]; s_lo[i] = g_exp.lo[i]; }
-    for (uint32_t i = tid; i < TILE_ROWS * D; i += 256) s_o[i] = 0;
-    if (tid == 0) s_mag = 0;
-    const uint32_t r = R.row0 + l;
-    const bool mine = r < R.n_rows;
-    const uint32_t id = row_id(A, R, mine ? r : R.row0);
-    int32_t m = 0;
-    uint32_t inv = 0;
-    if (mine) {
-        m = S.rmax[id];
-        uint32_t sum = 0;
-        for (uint32_t x = 0; x * SEGMENT < R.s.keys; x++) sum = __builtin_elementwise_add_sat(sum, S.csum[(int64_t)x * S.n_rows + id]);
-        inv = sum ? (1u << (2 * SCALE)) / sum : 0;
-    }
-    __syncthreads();
-    constexpr int VS = value_steps(KS);
-    Range rv;
-    const uint32_t k1 = min(k0 + S.chunk, R.s.keys);
+    const Line line(A, S);
+    const uint32_t end = line.begin(blockIdx.x + 1);
 #pragma unroll 1
-    for (int f0 = 0; f0 < KS; f0 += VS) {
-        Product<VS> P;
-        each_product<CT, VS, FAST>(A, R, f0, k0 + wave * 64, 256, k1, g, l, P, rv, [&](uint32_t j, v4i& w0, v4i& w1) {
+    for (uint32_t u = line.begin(blockIdx.x); u < end;) {
+        const Stretch X = stretch_at(A, S, blockIdx.x, u, end);
+        const RowTile& R = X.R;
+        u += X.units;
+        for (uint32_t i = tid; i < X.n * D; i += 256) s_o[i] = 0;
+        if (tid == 0) s_mag = 0;
+        // the rows' maxima and sums over all shares: 16 lanes of a row each
+        {
+            int32_t m = GONE;
+            uint32_t sum = 0;
+            const uint32_t r = tid >> 4;
+            if (r < X.n)
+                each_share(A, S, X.tile, R.kvh, tid & 15, 16, [&](uint32_t part, uint32_t) {
+                    m = max(m, S.cmax[part + r]);
+                    sum = __builtin_elementwise_add_sat(sum, S.csum[part + r]);
+                });
+            for (int o = 8; o; o >>= 1) { m = max(m, __shfl_xor(m, o)); sum = __builtin_elementwise_add_sat(sum, (uint32_t)__shfl_xor((int)sum, o)); }
+            if ((tid & 15) == 0) { s_m[r] = m; s_sum[r] = sum; }
+        }
+        __syncthreads();
+        const bool mine = l < X.n;
+        const int32_t m = s_m[l];
+        const uint32_t inv = mine && s_sum[l] ? (1u << (2 * SCALE)) / s_sum[l] : 0;
+        const int32_t* from = S.scores + (int64_t)(X.row + (mine ? l : 0)) * S.pitch + 4 * g;      // lanes without a row: another's, inv is 0
+        Range rv;
+#pragma unroll 1
+        for (int f0 = 0; f0 < KS; f0 += VS) {
+            Product<VS> P;
+            each_product<CT, VS, FAST>(A, R, f0, X.k0 + wave * 64, UNIT, X.k1, g, l, P, rv, [&](uint32_t j, v4i& w0, v4i& w1) {
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const v4i x = *(const v4i*)(S.scores + (int64_t)id * S.pitch + j + 16 * t + 4 * g);      // lanes without a row: another's, inv is 0
-                uint32_t p[4];
+                for (int t = 0; t < 4; t++) {
+                    const v4i x = *(const v4i*)(from + j + 16 * t);
+                    uint32_t p[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) p[i] = __umul24((uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
-                int a, b;
-                weight_bytes(p, a, b);
-                w0[t] = a; w1[t] = b;
-            }
-        });
-        if (mine) add_product<VS>(P, f0, D, g, l, s_o);
+                    for (int i = 0; i < 4; i++) p[i] = __umul24((uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
+                    int a, b;
+                    weight_bytes(p, a, b);
+                    w0[t] = a; w1[t] = b;
+                }
+            });
+            if (mine) add_product<VS>(P, f0, D, g, l, s_o);
+        }
+        atomicOr(&s_mag, rv.word());
+        __syncthreads();
+        for (uint32_t i = tid; i < X.n * D; i += 256) {
+            const uint32_t x = i / D, y = i % D;
+            if (y < A.d) S.part[(int64_t)(X.part + x) * A.d + y] = (int64_t)s_o[i];
+        }
+        if (tid == 0) S.v_mag[X.mag] = s_mag;
+        __syncthreads();
     }
-    atomicOr(&s_mag, rv.word());
-    __syncthreads();
-    const uint32_t rows = min(TILE_ROWS, R.n_rows - R.row0);
-    for (uint32_t i = tid; i < rows * D; i += 256) {
-        const uint32_t x = i / D, y = i % D;
-        if (y < A.d) S.part[((int64_t)c * S.n_rows + row_id(A, R, R.row0 + x)) * A.d + y] = (int64_t)s_o[i];
-    }
-    if (tid == 0) S.v_mag[(int64_t)c * gridDim.x + blockIdx.x] = s_mag;
 }
 
-// One workgroup per row: the chunks' products added up, every dim by 256 / DP threads; where the operands did not fit the digits, the row again in 64 bits
+// One workgroup per row: the shares' products added up, every dim by 256 / DP threads; where the operands did not fit the digits, the row again in 64 bits
 template <class CT>
 __global__ __launch_bounds__(256) void k_split_join(Args A, Split S, uint32_t dp) {
-    const uint32_t id = blockIdx.x, t = id / A.H, h = id % A.H, tid = threadIdx.x, kvh = h / A.G;
+    const uint32_t t = blockIdx.x / A.H, h = blockIdx.x % A.H, tid = threadIdx.x, kvh = h / A.G;
     const uint32_t si = find_seq(A.cu, A.n_seqs, t);
     if (si >= A.n_seqs) return;
     const Seq s = seq_at(A, si);
     if (t < s.begin || t - s.begin >= s.n_new) return;
-    const uint32_t chunks = (s.keys + S.chunk - 1) / S.chunk;
-    const uint32_t tile = (uint32_t)((uint64_t)s.begin * A.G / TILE_ROWS) + si + ((t - s.begin) * A.G + h % A.G) / TILE_ROWS, at = tile * A.KV + kvh, tiles = S.n_tiles * A.KV;
+    const uint32_t row = (t - s.begin) * A.G + h % A.G, tile = (uint32_t)((uint64_t)s.begin * A.G / TILE_ROWS) + si + row / TILE_ROWS, r = row % TILE_ROWS;
     __shared__ uint32_t s_mag[3];
     __shared__ int32_t s_q[256], s_p[256];
     __shared__ uint64_t s_red[256];
     if (tid < 3) s_mag[tid] = 0;
     __syncthreads();
-    for (uint32_t c = tid; c < chunks; c += 256) {
-        atomicOr(&s_mag[1], S.k_mag[(int64_t)c * tiles + at]);
-        atomicOr(&s_mag[2], S.v_mag[(int64_t)c * tiles + at]);
-        if (c == 0) atomicOr(&s_mag[0], S.q_mag[at]);
-    }
+    each_share(A, S, tile, kvh, tid, 256, [&](uint32_t, uint32_t mag) { atomicOr(&s_mag[0], S.q_mag[mag]); atomicOr(&s_mag[1], S.k_mag[mag]); atomicOr(&s_mag[2], S.v_mag[mag]); });
     const uint32_t y = tid & (dp - 1), parts = 256 / dp;
     int64_t sum = 0;
-    if (y < A.d) for (uint32_t c = tid / dp; c < chunks; c += parts) sum += S.part[((int64_t)c * S.n_rows + id) * A.d + y];
+    if (y < A.d) each_share(A, S, tile, kvh, tid / dp, parts, [&](uint32_t part, uint32_t) { sum += S.part[(int64_t)(part + r) * A.d + y]; });
     s_red[tid] = (uint64_t)sum;
     __syncthreads();
     const uint32_t mq = s_mag[0], mk = s_mag[1], mv = s_mag[2];

@@ -65,14 +65,6 @@ struct Planes {
 // Offsets cu[s] / 32 + s are far enough apart for ceil(len / 32) tiles each: no prefix sum is needed
 __device__ inline uint32_t tile_base(const Args& A, const Planes& P, uint32_t s) { return P.per_seq ? s * P.per_seq : min((uint32_t)max(A.cu[s], 0), A.n_tokens) / 32 + s; }
 
-// largest s with base(s) <= x, base increasing
-template <class F>
-__device__ inline uint32_t last_at_most(uint32_t n, uint64_t x, F base) {
-    uint32_t lo = 0, hi = n;
-    while (hi - lo > 1) { const uint32_t mid = (lo + hi) / 2; if (base(mid) <= x) lo = mid; else hi = mid; }
-    return lo;
-}
-
 template <class CT, int DP>
 __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
     constexpr int F = DP / 32;
