@@ -34,39 +34,45 @@ int with_dim(int dp, F f) {
     }
 }
 
-// the digit planes of the tile kernel in a workspace; per_seq = 0: the tiles of packed prompts
+// the digit planes and the held e of the tile kernel in a workspace; cached_keys = 0: packed prompts
 struct PlanesLayout {
-    size_t tiles, per_seq, bytes, v_at, mag_at, there_at;
-    PlanesLayout(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys) {
+    size_t max_keys, tiles, per_seq, held, work, wgs, v_at, mag_at, there_at, next_at, e_at, bytes;
+    PlanesLayout(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t cached_keys) {
         const size_t slack = 4;                                        // a step reads up to 4 tiles: its last ones may lie behind a sequence's end
-        per_seq = max_keys ? (max_keys + 31) / 32 : 0;
-        tiles = (max_keys ? n_seqs * per_seq : n_tokens / 32 + n_seqs) + slack;
-        const size_t one = tiles * s->n_kv_heads * (size_t)(padded_dim(s->head_dim) / 32 * 3072);
+        const int dp = padded_dim(s->head_dim), rows = with_dim(dp, [](auto d) { return (int)TileShape<decltype(d)::value>::ROWS; });
+        per_seq = (cached_keys + 31) / 32;
+        max_keys = cached_keys ? cached_keys : n_tokens;
+        tiles = (cached_keys ? n_seqs * per_seq : n_tokens / 32 + n_seqs) + slack;
+        held = std::min<size_t>((max_keys + 127) / 128 * 128, HELD);
+        work = (n_tokens * (s->n_heads / s->n_kv_heads) / rows + n_seqs) * s->n_kv_heads;
+        wgs = std::min<size_t>(work, TILE_WGS);
+        const size_t one = tiles * s->n_kv_heads * (size_t)(dp / 32 * 3072);
         v_at = one;
         mag_at = 2 * one;
         there_at = mag_at + 8 * tiles * s->n_kv_heads;
-        bytes = there_at + 4 * tiles;
+        next_at = there_at + 4 * tiles;
+        e_at = (next_at + 4 + 15) / 16 * 16;
+        bytes = e_at + wgs * rows * held * 2;
     }
     Planes at(void* ws, const atlas_attn_shape_t* s) const {
         uint8_t* w = (uint8_t*)ws;
-        return Planes{w, w + v_at, (uint32_t*)(w + mag_at), (uint32_t*)(w + mag_at) + tiles * s->n_kv_heads, (uint32_t*)(w + there_at), (uint32_t)tiles, (uint32_t)per_seq};
+        return Planes{w, w + v_at, (uint32_t*)(w + mag_at), (uint32_t*)(w + mag_at) + tiles * s->n_kv_heads, (uint32_t*)(w + there_at), w + e_at, (uint32_t*)(w + next_at), (uint32_t)tiles, (uint32_t)per_seq};
     }
 };
-bool many_rows(size_t n_seqs, size_t n_tokens) { return n_tokens > 4 * n_seqs; }
 template <class CT>
-int launch_tiles(const Args& A, const Planes& P, size_t dp, hipStream_t stream) {
-    return with_dim((int)dp, [&](auto dim) -> int {
+int launch_tiles(const Args& A, const PlanesLayout& L, const Planes& P, hipStream_t stream) {
+    return with_dim(padded_dim(A.d), [&](auto dim) -> int {
         constexpr int DP = decltype(dim)::value;
         using T = TileShape<DP>;
-        k_attn_planes<CT, DP><<<dim3(P.tiles, A.KV), 256, 0, stream>>>(A, P);
-        const uint64_t wgs = ((uint64_t)A.n_tokens * A.G / T::ROWS + A.n_seqs) * A.KV;
-        if (wgs > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows for one call");
-        if (T::LDS > 65536) HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_tile<CT, DP>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS));
-        k_attn_tile<CT, DP><<<(unsigned)wgs, 256, T::LDS, stream>>>(A, P);
+        if (L.work > 0x7fffffff || L.tiles > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows for one call");
+        k_attn_planes<CT, DP><<<dim3((unsigned)L.tiles, A.KV), 256, 0, stream>>>(A, P);
+        auto* k = L.max_keys > HELD ? &k_attn_tile<CT, DP, true> : &k_attn_tile<CT, DP, false>;
+        if (T::LDS > 65536) HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS));
+        k<<<(unsigned)L.wgs, 256, T::LDS, stream>>>(A, P, (uint32_t)L.work, (uint32_t)L.held);
         return ATLAS_OK;
     });
 }
-
+bool many_rows(size_t n_seqs, size_t n_tokens) { return n_tokens > 4 * n_seqs; }
 // Few rows: the workspace of the split path
 struct SplitLayout {
     Split S{};
@@ -170,7 +176,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
         return L.end();
     }
     const PlanesLayout P(shape, n_seqs, n_tokens, 0);
-    if (int rc = launch_tiles<int32_t>(A, P.at(d_workspace, shape), padded_dim(shape->head_dim), L.stream)) return rc;
+    if (int rc = launch_tiles<int32_t>(A, P, P.at(d_workspace, shape), L.stream)) return rc;
     return L.end();
 }
 
@@ -207,8 +213,7 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     }
     if (many_rows(n_seqs, n_tokens)) {
         const PlanesLayout P(shape, n_seqs, n_tokens, std::max<size_t>(A.max_keys, 1));
-        const int dp = padded_dim(shape->head_dim);
-        if (int rc = cache->bits == 16 ? launch_tiles<int16_t>(A, P.at(d_workspace, shape), dp, L.stream) : launch_tiles<int32_t>(A, P.at(d_workspace, shape), dp, L.stream)) return rc;
+        if (int rc = cache->bits == 16 ? launch_tiles<int16_t>(A, P, P.at(d_workspace, shape), L.stream) : launch_tiles<int32_t>(A, P, P.at(d_workspace, shape), L.stream)) return rc;
         return L.end();
     }
     const SplitLayout P(shape, n_seqs, n_tokens, A.max_keys, d_workspace);

@@ -60,6 +60,8 @@ struct Planes {
     uint8_t *k, *v;
     uint32_t *k_mag, *v_mag;       // [kv head][tile]
     uint32_t* there;               // [tile]: which of its keys exist
+    uint8_t* e;                    // [workgroup][rows][held] e, 2 bytes each
+    uint32_t* next;                // the counter of the tile kernel's work
     uint32_t tiles, per_seq;       // per_seq: tiles of a sequence (cached); 0: by its offset (prompt)
 };
 // Offsets cu[s] / 32 + s are far enough apart for ceil(len / 32) tiles each: no prefix sum is needed
@@ -68,6 +70,7 @@ __device__ inline uint32_t tile_base(const Args& A, const Planes& P, uint32_t s)
 template <class CT, int DP>
 __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
     constexpr int F = DP / 32;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *P.next = 0;
     const uint32_t tile = blockIdx.x, kvh = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     const uint32_t si = P.per_seq ? tile / P.per_seq : last_at_most(A.n_seqs, tile, [&](uint32_t s) { return (uint64_t)tile_base(A, P, s); });
     if (si >= A.n_seqs) return;
@@ -158,235 +161,261 @@ struct TileShape {
     static constexpr int OF = F / SPLIT;                      // output fragments of a wave
     static constexpr uint32_t TILE = F * 3072, STEP = TILE * SUBS;
     static constexpr int BUFS = DP == 256 ? 1 : 2;            // 160 KB of LDS hold one step of 256 dims
-    static constexpr uint32_t LUT = 4096, P_BYTES = SPLIT > 1 ? GROUPS * SUBS * 2048 : 0;
-    static constexpr uint32_t LDS = LUT + P_BYTES + STEP * BUFS + 1024;
+    static constexpr uint32_t LUT = 4096, LDS = LUT + STEP * BUFS + 1024;
 };
+// The workgroups that fit the chip at once take tiles from a counter.  Each has room for the e of HELD keys of its rows; where a tile has more keys, the scores of the
+// others are taken a third time.
+constexpr uint32_t TILE_WGS = 768, HELD = 16384;
 
-template <class CT, int DP>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Planes P) {
+template <class CT, int DP, bool LONG>      // LONG: tiles may have more than HELD keys; the product's sums then live through another pass over scores
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Planes P, uint32_t n_work, uint32_t held) {
     using T = TileShape<DP>;
     constexpr int F = T::F, SPLIT = T::SPLIT, SUBS = T::SUBS;
     extern __shared__ __align__(16) uint8_t lds[];
     int32_t* s_hi = (int32_t*)lds;
     int32_t* s_lo = s_hi + 512;
-    uint8_t* s_p = lds + T::LUT;
-    uint8_t* s_a = s_p + T::P_BYTES;
+    uint8_t* s_a = lds + T::LUT;
     uint8_t* s_b = s_a + (T::BUFS == 2 ? T::STEP : 0);
     uint32_t* s_red = (uint32_t*)(s_a + T::STEP * T::BUFS);        // 256 words
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
     const uint32_t group = wave / SPLIT, part = wave % SPLIT;
-    // the kv head runs fastest: with 8 of them each XCD's L2 sees one head's planes; late tiles (many keys under the causal mask) start first
-    const uint32_t kvh = blockIdx.x % A.KV, qt = gridDim.x / A.KV - 1 - blockIdx.x / A.KV;
-    auto q_base = [&](uint32_t s) { return (uint64_t)min((uint32_t)max(A.cu[s], 0), A.n_tokens) * A.G / T::ROWS + s; };
-    const uint32_t si = last_at_most(A.n_seqs, qt, q_base);
-    const Seq s = seq_at(A, si);
-    const uint64_t first = (uint64_t)(qt - q_base(si)) * T::ROWS;
-    const uint32_t n_rows = s.n_new * A.G;
-    if (qt < q_base(si) || first >= n_rows) return;
-    const uint32_t row0 = (uint32_t)first, rows = min((uint32_t)T::ROWS, n_rows - row0);
-    const uint32_t base = tile_base(A, P, si);
-    // my row
-    const uint32_t r = row0 + group * 32 + l32;
-    const bool mine = r < n_rows;
-    const uint32_t rr = mine ? r : n_rows - 1, tok = rr / A.G, head = kvh * A.G + rr % A.G;
-    const uint32_t limit = min(key_limit(A, s, tok), s.keys);
-    const uint32_t most = min(key_limit(A, s, (row0 + rows - 1) / A.G), s.keys), n_steps = (most + T::KEYS - 1) / T::KEYS;
-
     for (uint32_t i = tid; i < 512; i += 256) { s_hi[i] = g_exp.hi[i]; s_lo[i] = g_exp.lo[i]; }
-    if (tid < 3) s_red[tid] = 0;
-    __syncthreads();
-    v4i q0[F], q1[F], q2[F];
-    uint32_t mq = 0, mk = 0, mv = 0;
-    {
-        Range rq;
-        const int32_t* q = A.q.d + (int64_t)(s.begin + tok) * A.q.ts + (int64_t)head * A.q.hs;
-#pragma unroll
-        for (int f = 0; f < F; f++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                int32_t e[4];
-                load4(q, f * 32 + half * 16 + c * 4, A.d, e);
-                int a, b, g;
-                digits4(e[0], e[1], e[2], e[3], a, b, g, rq);
-                q0[f][c] = a; q1[f][c] = b; q2[f][c] = g;
-            }
-        const uint32_t tiles = (most + 31) / 32;
-        for (uint32_t i = tid; i < tiles; i += 256) { mk |= P.k_mag[(size_t)kvh * P.tiles + base + i]; mv |= P.v_mag[(size_t)kvh * P.tiles + base + i]; }
-        atomicOr(&s_red[0], rq.word());
-        if (mk) atomicOr(&s_red[1], mk);
-        if (mv) atomicOr(&s_red[2], mv);
+    // e of this wave's rows: [tile of 32 keys][lane][16], 2 bytes each, in the order in which a lane has its scores
+    const uint32_t held_steps = held / T::KEYS;
+    v4i* const e_rows = (v4i*)(P.e + ((size_t)blockIdx.x * T::GROUPS + group) * held * 64) + lane * 2;
+#pragma unroll 1
+    for (;;) {
         __syncthreads();
-        mq = s_red[0]; mk = s_red[1]; mv = s_red[2];
+        if (tid == 0) s_red[3] = atomicAdd(P.next, 1u);
+        if (tid < 3) s_red[tid] = 0;
         __syncthreads();
-    }
-    if (((mq | mk | mv) & WIDE) || bits_of(mq) + bits_of(mk) + bits_of(A.d - 1) > 45) {
-        int32_t* x_q = (int32_t*)s_a;                                  // 1 KB, 1 KB, 2 KB of the tile buffer
-        for (uint32_t x = 0; x < rows; x++) row_exact<CT>(A, s, (row0 + x) / A.G, kvh * A.G + (row0 + x) % A.G, x_q, x_q + 256, (uint64_t*)(x_q + 512));
-        return;
-    }
+        const uint32_t work = __builtin_amdgcn_readfirstlane(s_red[3]);
+        if (work >= n_work) return;
+        // the kv head runs fastest: with 8 of them each XCD's L2 sees one head's planes; late tiles (many keys under the causal mask) start first
+        const uint32_t kvh = work % A.KV, qt = n_work / A.KV - 1 - work / A.KV;
+        auto q_base = [&](uint32_t s) { return (uint64_t)min((uint32_t)max(A.cu[s], 0), A.n_tokens) * A.G / T::ROWS + s; };
+        const uint32_t si = last_at_most(A.n_seqs, qt, q_base);
+        const Seq s = seq_at(A, si);
+        const uint64_t first = (uint64_t)(qt - q_base(si)) * T::ROWS;
+        const uint32_t n_rows = s.n_new * A.G;
+        if (qt < q_base(si) || first >= n_rows) continue;
+        const uint32_t row0 = (uint32_t)first, rows = min((uint32_t)T::ROWS, n_rows - row0);
+        const uint32_t base = tile_base(A, P, si);
+        // my row; lanes behind the last one repeat it
+        const bool mine = row0 + group * 32 + l32 < n_rows;
+        const uint32_t rr = min(row0 + group * 32 + l32, n_rows - 1), tok = rr / A.G, head = kvh * A.G + rr % A.G;
+        const uint32_t limit = min(key_limit(A, s, tok), s.keys);
+        const uint32_t most = min(key_limit(A, s, (row0 + rows - 1) / A.G), s.keys), n_steps = (most + T::KEYS - 1) / T::KEYS;
 
-    const uint8_t* gk = P.k + ((int64_t)kvh * P.tiles + base) * T::TILE;
-    const uint8_t* gv = P.v + ((int64_t)kvh * P.tiles + base) * T::TILE;
-    // the scores of sub-tile `sub` of the step in `buf`, in one sweep over the fragments with five accumulators
-    auto scores = [&](const uint8_t* buf, int sub, v16i& x) {
-        v16i a0 = {}, a1 = {}, a2 = {}, a3 = {}, a4 = {};
-        const v4i* kf = (const v4i*)(buf + sub * T::TILE) + lane;
+        v4i q0[F], q1[F], q2[F];
+        {
+            uint32_t mq = 0, mk = 0, mv = 0;
+            Range rq;
+            const int32_t* q = A.q.d + (int64_t)(s.begin + tok) * A.q.ts + (int64_t)head * A.q.hs;
 #pragma unroll
-        for (int f = 0; f < F; f++) {
-            const v4i k0 = kf[f * 192], k1 = kf[f * 192 + 64], k2 = kf[f * 192 + 128];
-            a4 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q2[f], a4, 0, 0, 0);
-            a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q1[f], a3, 0, 0, 0);
-            a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q0[f], a2, 0, 0, 0);
-            a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q0[f], a1, 0, 0, 0);
-            a0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q0[f], a0, 0, 0, 0);
-            a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q2[f], a3, 0, 0, 0);
-            a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q1[f], a2, 0, 0, 0);
-            a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q1[f], a1, 0, 0, 0);
-            a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q2[f], a2, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = combine<DP == 256>(a0[i], a1[i], a2[i], a3[i], a4[i]);
-        if (A.mul != ONE)
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = rescale(x[i], A.mul);
-    };
-    // which of a lane's 16 keys of a sub-tile count: bit i; `all`: every one of the wave's does
-    auto seen = [&](uint32_t step, int sub, bool& all) -> uint32_t {
-        const uint32_t j0 = step * T::KEYS + sub * 32, t = j0 / 32;
-        const uint32_t there = j0 < s.keys ? P.there[base + t] : 0;
-        uint32_t in = limit >= j0 + 32 ? ~0u : limit > j0 ? (1u << (limit - j0)) - 1 : 0;
-        in &= there;
-        all = __all(in == ~0u);
-        const uint32_t w = in >> (4 * half);                           // byte c: keys 8 c + 4 half ..
-        return (w & 0xf) | ((w >> 4) & 0xf0) | ((w >> 8) & 0xf00) | ((w >> 12) & 0xf000);
-    };
-
-    // ---- pass 1: the maximum, pass 2: the sum
-    int32_t m = INT32_MIN;
-    uint32_t sum = 0;
-#pragma unroll 1
-    for (int pass = 0; pass < 2; pass++) {
-        if (T::BUFS == 2 && n_steps) copy_to_lds(gk, s_a, T::STEP, wave, lane);
-#pragma unroll 1
-        for (uint32_t step = 0; step < n_steps; step++) {
-            uint8_t* buf = T::BUFS == 2 && (step & 1) ? s_b : s_a;
-            if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gk + (int64_t)step * T::STEP, buf, T::STEP, wave, lane); }
-            wait_loads();
-            __syncthreads();
-            if (T::BUFS == 2 && step + 1 < n_steps) copy_to_lds(gk + (int64_t)(step + 1) * T::STEP, (step & 1) ? s_a : s_b, T::STEP, wave, lane);
-#pragma unroll 1
-            for (int y = 0; y < T::MY_SUBS; y++) {
-                const int sub = part * T::MY_SUBS + y;
-                bool all;
-                const uint32_t in = seen(step, sub, all);
-                if (!__any(in != 0)) continue;
-                v16i x;
-                scores(buf, sub, x);
-                if (pass == 0) {
-#pragma unroll
-                    for (int i = 0; i < 16; i++) { const int32_t v = all || ((in >> i) & 1) ? x[i] : INT32_MIN; m = max(m, v); }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int32_t e = exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo);
-                        sum = __builtin_elementwise_add_sat(sum, all || ((in >> i) & 1) ? (uint32_t)e : 0u);
-                    }
-                }
-            }
-        }
-        // the other half-wave has the rest of the row's keys, and so have the waves that share the rows
-        if (pass == 0) m = max(m, __shfl_xor(m, 32)); else sum = __builtin_elementwise_add_sat(sum, (uint32_t)__shfl_xor((int)sum, 32));
-        __syncthreads();
-        if (SPLIT > 1) {
-            if (half == 0) s_red[wave * 32 + l32] = pass == 0 ? (uint32_t)m : sum;
-            __syncthreads();
-            for (int p = 0; p < SPLIT; p++) {
-                const uint32_t o = s_red[(group * SPLIT + p) * 32 + l32];
-                if (p != (int)part) { if (pass == 0) m = max(m, (int32_t)o); else sum = __builtin_elementwise_add_sat(sum, o); }
-            }
-            __syncthreads();
-        }
-    }
-    const uint32_t inv = sum ? (1u << (2 * SCALE)) / sum : 0;
-
-    // ---- pass 3: the weights again, and their product with the values.  o[.][f]: the sums with the values' digit 0, 1, 2
-    v16i o0[T::OF] = {}, o1[T::OF] = {}, o2[T::OF] = {};
-    if (T::BUFS == 2 && n_steps) copy_to_lds(gk, s_a, T::STEP, wave, lane);
-#pragma unroll 1
-    for (uint32_t step = 0; step < n_steps; step++) {
-        if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gk + (int64_t)step * T::STEP, s_a, T::STEP, wave, lane); }
-        wait_loads();
-        __syncthreads();
-        if (T::BUFS == 2) copy_to_lds(gv + (int64_t)step * T::STEP, s_b, T::STEP, wave, lane);
-        v4i w0[T::MY_SUBS], w1[T::MY_SUBS];
-#pragma unroll
-        for (int y = 0; y < T::MY_SUBS; y++) {
-            const int sub = part * T::MY_SUBS + y;
-            bool all;
-            const uint32_t in = seen(step, sub, all);
-            w0[y] = v4i{}; w1[y] = v4i{};
-            if (__any(in != 0)) {
-                v16i x;
-                scores(s_a, sub, x);
+            for (int f = 0; f < F; f++)
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    uint32_t p[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t e = (uint32_t)exp_q((uint32_t)m - (uint32_t)x[4 * c + i], s_hi, s_lo);
-                        p[i] = all || ((in >> (4 * c + i)) & 1) ? __umul24(e, inv) >> SCALE : 0;
-                    }
-                    // p = (signed byte) p + 2^8 ((p + 128) >> 8)
-                    const uint32_t a = p[0] | (p[1] << 16), b = p[2] | (p[3] << 16);
-                    w0[y][c] = (int)__builtin_amdgcn_perm(b, a, 0x06040200u);
-                    w1[y][c] = (int)__builtin_amdgcn_perm(b + 0x00800080u, a + 0x00800080u, 0x07050301u);
+                    int32_t e[4];
+                    load4(q, f * 32 + half * 16 + c * 4, A.d, e);
+                    int a, b, g;
+                    digits4(e[0], e[1], e[2], e[3], a, b, g, rq);
+                    q0[f][c] = a; q1[f][c] = b; q2[f][c] = g;
                 }
-            }
-            if (SPLIT > 1) {
-                v4i* to = (v4i*)(s_p + (group * SUBS + sub) * 2048) + lane;
-                to[0] = w0[y]; to[64] = w1[y];
+            const uint32_t tiles = (most + 31) / 32;
+            for (uint32_t i = tid; i < tiles; i += 256) { mk |= P.k_mag[(size_t)kvh * P.tiles + base + i]; mv |= P.v_mag[(size_t)kvh * P.tiles + base + i]; }
+            atomicOr(&s_red[0], rq.word());
+            if (mk) atomicOr(&s_red[1], mk);
+            if (mv) atomicOr(&s_red[2], mv);
+            __syncthreads();
+            mq = s_red[0]; mk = s_red[1]; mv = s_red[2];
+            __syncthreads();
+            if (((mq | mk | mv) & WIDE) || bits_of(mq) + bits_of(mk) + bits_of(A.d - 1) > 45) {
+                int32_t* x_q = (int32_t*)s_a;                          // 1 KB, 1 KB, 2 KB of the tile buffer
+                for (uint32_t x = 0; x < rows; x++) row_exact<CT>(A, s, (row0 + x) / A.G, kvh * A.G + (row0 + x) % A.G, x_q, x_q + 256, (uint64_t*)(x_q + 512));
+                continue;
             }
         }
-        if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gv + (int64_t)step * T::STEP, s_b, T::STEP, wave, lane); }
-        wait_loads();
-        __syncthreads();
-        if (T::BUFS == 2 && step + 1 < n_steps) copy_to_lds(gk + (int64_t)(step + 1) * T::STEP, s_a, T::STEP, wave, lane);
+        const uint8_t* gk = P.k + ((int64_t)kvh * P.tiles + base) * T::TILE;
+        const uint8_t* gv = P.v + ((int64_t)kvh * P.tiles + base) * T::TILE;
+        // the scores of sub-tile `sub` of the step in `buf`, in one sweep over the fragments with five accumulators
+        auto scores = [&](const uint8_t* buf, int sub, v16i& x) {
+            v16i a0 = {}, a1 = {}, a2 = {}, a3 = {}, a4 = {};
+            const v4i* kf = (const v4i*)(buf + sub * T::TILE) + lane;
 #pragma unroll
-        for (int sub = 0; sub < SUBS; sub++) {
-            v4i b0, b1;
-            if (SPLIT > 1) { const v4i* from = (const v4i*)(s_p + (group * SUBS + sub) * 2048) + lane; b0 = from[0]; b1 = from[64]; }
-            else { b0 = w0[sub]; b1 = w1[sub]; }
-            const bool second = __any((b1[0] | b1[1] | b1[2] | b1[3]) != 0);
-            if (!second && !__any((b0[0] | b0[1] | b0[2] | b0[3]) != 0)) continue;
-            const v4i* vf = (const v4i*)(s_b + sub * T::TILE + part * T::OF * 3072) + lane;
+            for (int f = 0; f < F; f++) {
+                const v4i k0 = kf[f * 192], k1 = kf[f * 192 + 64], k2 = kf[f * 192 + 128];
+                a4 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q2[f], a4, 0, 0, 0);
+                a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q1[f], a3, 0, 0, 0);
+                a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q0[f], a2, 0, 0, 0);
+                a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q0[f], a1, 0, 0, 0);
+                a0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q0[f], a0, 0, 0, 0);
+                a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q2[f], a3, 0, 0, 0);
+                a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q1[f], a2, 0, 0, 0);
+                a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q1[f], a1, 0, 0, 0);
+                a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q2[f], a2, 0, 0, 0);
+            }
 #pragma unroll
-            for (int f = 0; f < T::OF; f++) {
-                const v4i x0 = vf[f * 192], x1 = vf[f * 192 + 64], x2 = vf[f * 192 + 128];
-                o0[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x0, b0, o0[f], 0, 0, 0);
-                o1[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x1, b0, o1[f], 0, 0, 0);
-                o2[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x2, b0, o2[f], 0, 0, 0);
-                if (second) {
-                    const v16i y0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x0, b1, v16i{}, 0, 0, 0), y1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x1, b1, v16i{}, 0, 0, 0),
-                               y2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x2, b1, v16i{}, 0, 0, 0);
-                    o0[f] += y0 * 256; o1[f] += y1 * 256; o2[f] += y2 * 256;
+            for (int i = 0; i < 16; i++) x[i] = combine<DP == 256>(a0[i], a1[i], a2[i], a3[i], a4[i]);
+            if (A.mul != ONE)
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[i] = rescale(x[i], A.mul);
+        };
+        // which of a lane's 16 keys of a sub-tile count, as bits 8 c + i of 4 half + ..; ~0 where all of the wave's do
+        auto seen = [&](uint32_t step, int sub) -> uint32_t {
+            const uint32_t j0 = step * T::KEYS + sub * 32;
+            uint32_t in = limit >= j0 + 32 ? ~0u : limit > j0 ? (1u << (limit - j0)) - 1 : 0;
+            in &= j0 < s.keys ? P.there[base + j0 / 32] : 0;
+            return __all(in == ~0u) ? ~0u : in >> (4 * half);
+        };
+        int32_t m = INT32_MIN;
+        uint32_t sum = 0;
+        // steps [from, to): their maximum (MAX), or their e, summed and held
+        enum { MAX, SUM, HOLD };
+        auto pass = [&](uint32_t from, uint32_t to, int what) {
+            if (T::BUFS == 2 && from < to) copy_to_lds(gk + (int64_t)from * T::STEP, s_a, T::STEP, wave, lane);
+#pragma unroll 1
+            for (uint32_t step = from; step < to; step++) {
+                uint8_t* buf = T::BUFS == 2 && ((step - from) & 1) ? s_b : s_a;
+                if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gk + (int64_t)step * T::STEP, buf, T::STEP, wave, lane); }
+                wait_loads();
+                __syncthreads();
+                if (T::BUFS == 2 && step + 1 < to) copy_to_lds(gk + (int64_t)(step + 1) * T::STEP, ((step - from) & 1) ? s_a : s_b, T::STEP, wave, lane);
+#pragma unroll 1
+                for (int y = 0; y < T::MY_SUBS; y++) {
+                    const int sub = part * T::MY_SUBS + y;
+                    const uint32_t in = seen(step, sub);
+                    const bool any = __any(in != 0);
+                    v16i x;
+                    if (any) scores(buf, sub, x);
+                    if (what == MAX) {
+                        if (!any) continue;
+                        if (in != ~0u)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) { const int32_t keep = (int32_t)(in << (31 - (8 * (i / 4) + i % 4))) >> 31; x[i] = (x[i] & keep) | (INT32_MIN & ~keep); }
+#pragma unroll
+                        for (int i = 0; i < 16; i++) m = max(m, x[i]);
+                    } else {
+                        uint32_t e[16] = {};
+                        if (any) {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) e[i] = (uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo);
+                            if (in != ~0u)
+#pragma unroll
+                                for (int i = 0; i < 16; i++) e[i] &= (uint32_t)((int32_t)(in << (31 - (8 * (i / 4) + i % 4))) >> 31);
+                        }
+                        if (what == SUM) {
+                            uint32_t t = 0;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) t += e[i];                       // <= 2^18
+                            sum = __builtin_elementwise_add_sat(sum, t);
+                        }
+                        if (!LONG || step - from < held_steps) {
+                            v4i w[2];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) w[i / 4][i % 4] = (int)(e[2 * i] | (e[2 * i + 1] << 16));
+                            v4i* to_e = e_rows + (size_t)((step - from) * SUBS + sub) * 128;
+                            to_e[0] = w[0]; to_e[1] = w[1];
+                        }
+                    }
                 }
             }
+            __threadfence_block();
+            __syncthreads();
+        };
+#pragma unroll 1
+        for (int what = MAX; what <= SUM; what++) {
+            pass(0, n_steps, what);
+            // the other half-wave has the rest of the row's keys, and so have the waves that share the rows
+            if (what == MAX) m = max(m, __shfl_xor(m, 32)); else sum = __builtin_elementwise_add_sat(sum, (uint32_t)__shfl_xor((int)sum, 32));
+            if (SPLIT > 1) {
+                if (half == 0) s_red[wave * 32 + l32] = what == MAX ? (uint32_t)m : sum;
+                __syncthreads();
+                for (int p = 0; p < SPLIT; p++) {
+                    const uint32_t o = s_red[(group * SPLIT + p) * 32 + l32];
+                    if (p != (int)part) { if (what == MAX) m = max(m, (int32_t)o); else sum = __builtin_elementwise_add_sat(sum, o); }
+                }
+                __syncthreads();
+            }
+        }
+        const uint32_t inv = sum ? (1u << (2 * SCALE)) / sum : 0;
+
+        // ---- the weights from the e that are held, and their product with the values.  o[.][f]: the sums with the values' digit 0, 1, 2
+        v16i o0[T::OF] = {}, o1[T::OF] = {}, o2[T::OF] = {};
+        auto product = [&](uint32_t from, uint32_t to) {
+            if (from >= to) return;
+            v4i w[SUBS][2];
+            auto load_e = [&](uint32_t step) {
+#pragma unroll
+                for (int sub = 0; sub < SUBS; sub++) { const v4i* x = e_rows + (size_t)((step - from) * SUBS + sub) * 128; w[sub][0] = x[0]; w[sub][1] = x[1]; }
+            };
+            if (T::BUFS == 2) copy_to_lds(gv + (int64_t)from * T::STEP, s_a, T::STEP, wave, lane);
+            load_e(from);
+#pragma unroll 1
+            for (uint32_t step = from; step < to; step++) {
+                uint8_t* buf = T::BUFS == 2 && ((step - from) & 1) ? s_b : s_a;
+                if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gv + (int64_t)step * T::STEP, buf, T::STEP, wave, lane); }
+                // p = (signed byte) p + 2^8 ((p + 128) >> 8)
+                v4i b0[SUBS], b1[SUBS];
+#pragma unroll
+                for (int sub = 0; sub < SUBS; sub++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t a = (uint32_t)w[sub][c / 2][2 * (c % 2)], b = (uint32_t)w[sub][c / 2][2 * (c % 2) + 1];
+                        a = (__umul24(a & 0xffff, inv) >> SCALE) | ((__umul24(a >> 16, inv) >> SCALE) << 16);
+                        b = (__umul24(b & 0xffff, inv) >> SCALE) | ((__umul24(b >> 16, inv) >> SCALE) << 16);
+                        b0[sub][c] = (int)__builtin_amdgcn_perm(b, a, 0x06040200u);
+                        b1[sub][c] = (int)__builtin_amdgcn_perm(b + 0x00800080u, a + 0x00800080u, 0x07050301u);
+                    }
+                wait_loads();
+                __syncthreads();
+                if (step + 1 < to) {
+                    if (T::BUFS == 2) copy_to_lds(gv + (int64_t)(step + 1) * T::STEP, ((step - from) & 1) ? s_a : s_b, T::STEP, wave, lane);
+                    load_e(step + 1);
+                }
+#pragma unroll
+                for (int sub = 0; sub < SUBS; sub++) {
+                    const bool second = __any((b1[sub][0] | b1[sub][1] | b1[sub][2] | b1[sub][3]) != 0);
+                    const v4i* vf = (const v4i*)(buf + sub * T::TILE + part * T::OF * 3072) + lane;
+#pragma unroll
+                    for (int f = 0; f < T::OF; f++) {
+                        const v4i x0 = vf[f * 192], x1 = vf[f * 192 + 64], x2 = vf[f * 192 + 128];
+                        o0[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x0, b0[sub], o0[f], 0, 0, 0);
+                        o1[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x1, b0[sub], o1[f], 0, 0, 0);
+                        o2[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x2, b0[sub], o2[f], 0, 0, 0);
+                        if (second) {
+                            const v16i y0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x0, b1[sub], v16i{}, 0, 0, 0), y1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x1, b1[sub], v16i{}, 0, 0, 0),
+                                       y2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x2, b1[sub], v16i{}, 0, 0, 0);
+                            o0[f] += y0 * 256; o1[f] += y1 * 256; o2[f] += y2 * 256;
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+        };
+        product(0, LONG ? min(n_steps, held_steps) : n_steps);
+        if constexpr (LONG)
+#pragma unroll 1
+            for (uint32_t from = held_steps; from < n_steps; from += held_steps) {
+                pass(from, min(n_steps, from + held_steps), HOLD);
+                product(from, min(n_steps, from + held_steps));
+            }
+        // floor((o0 + 2^8 o1 + 2^16 o2) / 2^14): a lane holds dims 8 c + 4 half .. + 3 of its row
+        if (mine) {
+            int32_t* out = A.out.d + (int64_t)(s.begin + tok) * A.out.ts + (int64_t)head * A.out.hs;
+#pragma unroll
+            for (int f = 0; f < T::OF; f++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const uint32_t i = (part * T::OF + f) * 32 + 8 * c + 4 * half;
+                    i32x4 y;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] = (int32_t)(((int64_t)o0[f][4 * c + e] + ((int64_t)o1[f][4 * c + e] << 8) + ((int64_t)o2[f][4 * c + e] << 16)) >> SCALE);
+                    if (i + 4 <= A.d) *(i32x4*)(out + i) = y;
+                    else for (uint32_t e = 0; e < 4; e++) if (i + e < A.d) out[i + e] = y[e];
+                }
         }
     }
-    // floor((o0 + 2^8 o1 + 2^16 o2) / 2^14): a lane holds dims 8 c + 4 half .. + 3 of its row
-    if (!mine) return;
-    int32_t* out = A.out.d + (int64_t)(s.begin + tok) * A.out.ts + (int64_t)head * A.out.hs;
-#pragma unroll
-    for (int f = 0; f < T::OF; f++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const uint32_t i = (part * T::OF + f) * 32 + 8 * c + 4 * half;
-            i32x4 y;
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = (int32_t)(((int64_t)o0[f][4 * c + e] + ((int64_t)o1[f][4 * c + e] << 8) + ((int64_t)o2[f][4 * c + e] << 16)) >> SCALE);
-            if (i + 4 <= A.d) *(i32x4*)(out + i) = y;
-            else for (uint32_t e = 0; e < 4; e++) if (i + e < A.d) out[i + e] = y[e];
-        }
 }
 
 }  // namespace atlas_attn
