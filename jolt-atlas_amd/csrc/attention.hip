@@ -51,7 +51,7 @@ struct PlanesLayout {
         mag_at = 2 * one;
         there_at = mag_at + 8 * tiles * s->n_kv_heads;
         next_at = there_at + 4 * tiles;
-        e_at = (next_at + 4 + 15) / 16 * 16;
+        e_at = (next_at + 32 + 15) / 16 * 16;
         bytes = e_at + wgs * rows * held * 2;
     }
     Planes at(void* ws, const atlas_attn_shape_t* s) const {

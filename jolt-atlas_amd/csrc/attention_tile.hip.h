@@ -61,7 +61,7 @@ struct Planes {
     uint32_t *k_mag, *v_mag;       // [kv head][tile]
     uint32_t* there;               // [tile]: which of its keys exist
     uint8_t* e;                    // [workgroup][rows][held] e, 2 bytes each
-    uint32_t* next;                // the counter of the tile kernel's work
+    uint32_t* next;                // the counters of the tile kernel's work lists
     uint32_t tiles, per_seq;       // per_seq: tiles of a sequence (cached); 0: by its offset (prompt)
 };
 // Offsets cu[s] / 32 + s are far enough apart for ceil(len / 32) tiles each: no prefix sum is needed
@@ -70,7 +70,7 @@ __device__ inline uint32_t tile_base(const Args& A, const Planes& P, uint32_t s)
 template <class CT, int DP>
 __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
     constexpr int F = DP / 32;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *P.next = 0;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 8) P.next[threadIdx.x] = 0;
     const uint32_t tile = blockIdx.x, kvh = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
     const uint32_t si = P.per_seq ? tile / P.per_seq : last_at_most(A.n_seqs, tile, [&](uint32_t s) { return (uint64_t)tile_base(A, P, s); });
     if (si >= A.n_seqs) return;
@@ -134,7 +134,9 @@ __device__ inline void copy_to_lds(const uint8_t* src, uint8_t* lds, uint32_t by
     for (uint32_t o = wave * 1024; o < bytes; o += 4096)
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o + lane * 16), (__attribute__((address_space(3))) void*)(lds + o), 16, 0, 0);
 }
-__device__ inline void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0), the others untouched
+// until at most N of the wave's loads and stores are outstanding; the other counters untouched
+template <int N>
+__device__ inline void wait_loads() { static_assert(N < 16); __builtin_amdgcn_s_waitcnt(0x0f70 | N); }
 
 // the Mul node's rescale: floor(s c / 2^14) with 1 <= c <= 2^14, s = 2^14 a + b:  a c + floor(b c / 2^14), in 24-bit multiplications
 __device__ inline int32_t rescale(int32_t s, int32_t c) {
@@ -160,12 +162,13 @@ struct TileShape {
     static constexpr int KEYS = 32 * SUBS, MY_SUBS = SUBS / SPLIT;
     static constexpr int OF = F / SPLIT;                      // output fragments of a wave
     static constexpr uint32_t TILE = F * 3072, STEP = TILE * SUBS;
-    static constexpr int BUFS = DP == 256 ? 1 : 2;            // 160 KB of LDS hold one step of 256 dims
+    static constexpr int BUFS = DP == 256 ? 1 : 3;            // two steps are on their way while one is worked on; of 256 dims 160 KB of LDS hold one step
+    static constexpr int COPIES = STEP / 4096;                // that a wave has issued for a step, at least
     static constexpr uint32_t LUT = 4096, LDS = LUT + STEP * BUFS + 1024;
 };
 // The workgroups that fit the chip at once take tiles from a counter.  Each has room for the e of HELD keys of its rows; where a tile has more keys, the scores of the
 // others are taken a third time.
-constexpr uint32_t TILE_WGS = 768, HELD = 16384;
+constexpr uint32_t TILE_WGS = 512, HELD = 16384;
 
 template <class CT, int DP, bool LONG>      // LONG: tiles may have more than HELD keys; the product's sums then live through another pass over scores
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Planes P, uint32_t n_work, uint32_t held) {
@@ -175,24 +178,31 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
     int32_t* s_hi = (int32_t*)lds;
     int32_t* s_lo = s_hi + 512;
     uint8_t* s_a = lds + T::LUT;
-    uint8_t* s_b = s_a + (T::BUFS == 2 ? T::STEP : 0);
     uint32_t* s_red = (uint32_t*)(s_a + T::STEP * T::BUFS);        // 256 words
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
     const uint32_t group = wave / SPLIT, part = wave % SPLIT;
     for (uint32_t i = tid; i < 512; i += 256) { s_hi[i] = g_exp.hi[i]; s_lo[i] = g_exp.lo[i]; }
     // e of this wave's rows: [tile of 32 keys][lane][16], 2 bytes each, in the order in which a lane has its scores
     const uint32_t held_steps = held / T::KEYS;
+    // Work lists by kv head: workgroups go to the 8 XCDs in turn, and those of one XCD begin with the same heads, so that its L2 holds their planes.  A list that
+    // has run out is followed by the next one.
+    const uint32_t lists = A.KV % 8 == 0 ? 8 : A.KV % 4 == 0 ? 4 : A.KV % 2 == 0 ? 2 : 1;
+    uint32_t list = blockIdx.x % lists, tried = 0;
     v4i* const e_rows = (v4i*)(P.e + ((size_t)blockIdx.x * T::GROUPS + group) * held * 64) + lane * 2;
 #pragma unroll 1
     for (;;) {
         __syncthreads();
-        if (tid == 0) s_red[3] = atomicAdd(P.next, 1u);
+        if (tid == 0) s_red[3] = atomicAdd(P.next + list, 1u);
         if (tid < 3) s_red[tid] = 0;
+        if (tid == 4) s_red[4] = 0;
         __syncthreads();
         const uint32_t work = __builtin_amdgcn_readfirstlane(s_red[3]);
-        if (work >= n_work) return;
-        // the kv head runs fastest: with 8 of them each XCD's L2 sees one head's planes; late tiles (many keys under the causal mask) start first
-        const uint32_t kvh = work % A.KV, qt = n_work / A.KV - 1 - work / A.KV;
+        if (work >= n_work / lists) {
+            if (++tried == lists) return;
+            list = (list + 1) % lists;
+            continue;
+        }
+        const uint32_t heads = A.KV / lists, kvh = list + lists * (work % heads), qt = n_work / A.KV - 1 - work / heads;      // late tiles (many keys under the causal mask) first
         auto q_base = [&](uint32_t s) { return (uint64_t)min((uint32_t)max(A.cu[s], 0), A.n_tokens) * A.G / T::ROWS + s; };
         const uint32_t si = last_at_most(A.n_seqs, qt, q_base);
         const Seq s = seq_at(A, si);
@@ -208,6 +218,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
         const uint32_t most = min(key_limit(A, s, (row0 + rows - 1) / A.G), s.keys), n_steps = (most + T::KEYS - 1) / T::KEYS;
 
         v4i q0[F], q1[F], q2[F];
+        bool holes;                                   // some of the sequence's keys lie in blocks that do not exist
         {
             uint32_t mq = 0, mk = 0, mv = 0;
             Range rq;
@@ -223,12 +234,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
                     q0[f][c] = a; q1[f][c] = b; q2[f][c] = g;
                 }
             const uint32_t tiles = (most + 31) / 32;
-            for (uint32_t i = tid; i < tiles; i += 256) { mk |= P.k_mag[(size_t)kvh * P.tiles + base + i]; mv |= P.v_mag[(size_t)kvh * P.tiles + base + i]; }
+            uint32_t hole = 0;
+            for (uint32_t i = tid; i < tiles; i += 256) {
+                mk |= P.k_mag[(size_t)kvh * P.tiles + base + i]; mv |= P.v_mag[(size_t)kvh * P.tiles + base + i];
+                const uint32_t n = s.keys - i * 32;
+                hole |= ~P.there[base + i] & (n < 32 ? (1u << n) - 1 : ~0u);
+            }
+            if (hole) s_red[4] = 1;
             atomicOr(&s_red[0], rq.word());
             if (mk) atomicOr(&s_red[1], mk);
             if (mv) atomicOr(&s_red[2], mv);
             __syncthreads();
             mq = s_red[0]; mk = s_red[1]; mv = s_red[2];
+            holes = s_red[4];
             __syncthreads();
             if (((mq | mk | mv) & WIDE) || bits_of(mq) + bits_of(mk) + bits_of(A.d - 1) > 45) {
                 int32_t* x_q = (int32_t*)s_a;                          // 1 KB, 1 KB, 2 KB of the tile buffer
@@ -238,6 +256,27 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
         }
         const uint8_t* gk = P.k + ((int64_t)kvh * P.tiles + base) * T::TILE;
         const uint8_t* gv = P.v + ((int64_t)kvh * P.tiles + base) * T::TILE;
+        // Steps [from, to) of a plane array through the LDS buffers: begin() sends the first on their way, arrive() waits for one, lets all waves be done with the
+        // one before it, and sends the next into that one's place
+        auto begin = [&](const uint8_t* src, uint32_t from, uint32_t to) {
+            if (T::BUFS == 3 && from < to) copy_to_lds(src + (int64_t)from * T::STEP, s_a, T::STEP, wave, lane);
+            if (T::BUFS == 3 && from + 1 < to) copy_to_lds(src + (int64_t)(from + 1) * T::STEP, s_a + T::STEP, T::STEP, wave, lane);
+        };
+        auto arrive = [&](const uint8_t* src, uint32_t from, uint32_t step, uint32_t to) -> const uint8_t* {
+            if constexpr (T::BUFS == 1) {
+                __syncthreads();
+                copy_to_lds(src + (int64_t)step * T::STEP, s_a, T::STEP, wave, lane);
+                wait_loads<0>();
+                __syncthreads();
+                return s_a;
+            } else {
+                const uint32_t at = (step - from) % 3;
+                if (step + 1 < to) wait_loads<T::COPIES>(); else wait_loads<0>();       // the next step's copies may still be out
+                __syncthreads();
+                if (step + 2 < to) copy_to_lds(src + (int64_t)(step + 2) * T::STEP, s_a + (at == 0 ? 2 : at - 1) * T::STEP, T::STEP, wave, lane);
+                return s_a + at * T::STEP;
+            }
+        };
         // the scores of sub-tile `sub` of the step in `buf`, in one sweep over the fragments with five accumulators
         auto scores = [&](const uint8_t* buf, int sub, v16i& x) {
             v16i a0 = {}, a1 = {}, a2 = {}, a3 = {}, a4 = {};
@@ -265,7 +304,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
         auto seen = [&](uint32_t step, int sub) -> uint32_t {
             const uint32_t j0 = step * T::KEYS + sub * 32;
             uint32_t in = limit >= j0 + 32 ? ~0u : limit > j0 ? (1u << (limit - j0)) - 1 : 0;
-            in &= j0 < s.keys ? P.there[base + j0 / 32] : 0;
+            if (holes) in &= j0 < s.keys ? P.there[base + j0 / 32] : 0;
             return __all(in == ~0u) ? ~0u : in >> (4 * half);
         };
         int32_t m = INT32_MIN;
@@ -273,14 +312,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
         // steps [from, to): their maximum (MAX), or their e, summed and held
         enum { MAX, SUM, HOLD };
         auto pass = [&](uint32_t from, uint32_t to, int what) {
-            if (T::BUFS == 2 && from < to) copy_to_lds(gk + (int64_t)from * T::STEP, s_a, T::STEP, wave, lane);
+            begin(gk, from, to);
 #pragma unroll 1
             for (uint32_t step = from; step < to; step++) {
-                uint8_t* buf = T::BUFS == 2 && ((step - from) & 1) ? s_b : s_a;
-                if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gk + (int64_t)step * T::STEP, buf, T::STEP, wave, lane); }
-                wait_loads();
-                __syncthreads();
-                if (T::BUFS == 2 && step + 1 < to) copy_to_lds(gk + (int64_t)(step + 1) * T::STEP, ((step - from) & 1) ? s_a : s_b, T::STEP, wave, lane);
+                const uint8_t* buf = arrive(gk, from, step, to);
 #pragma unroll 1
                 for (int y = 0; y < T::MY_SUBS; y++) {
                     const int sub = part * T::MY_SUBS + y;
@@ -349,12 +384,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
 #pragma unroll
                 for (int sub = 0; sub < SUBS; sub++) { const v4i* x = e_rows + (size_t)((step - from) * SUBS + sub) * 128; w[sub][0] = x[0]; w[sub][1] = x[1]; }
             };
-            if (T::BUFS == 2) copy_to_lds(gv + (int64_t)from * T::STEP, s_a, T::STEP, wave, lane);
+            begin(gv, from, to);
             load_e(from);
 #pragma unroll 1
             for (uint32_t step = from; step < to; step++) {
-                uint8_t* buf = T::BUFS == 2 && ((step - from) & 1) ? s_b : s_a;
-                if (T::BUFS == 1) { __syncthreads(); copy_to_lds(gv + (int64_t)step * T::STEP, buf, T::STEP, wave, lane); }
                 // p = (signed byte) p + 2^8 ((p + 128) >> 8)
                 v4i b0[SUBS], b1[SUBS];
 #pragma unroll
@@ -367,12 +400,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
                         b0[sub][c] = (int)__builtin_amdgcn_perm(b, a, 0x06040200u);
                         b1[sub][c] = (int)__builtin_amdgcn_perm(b + 0x00800080u, a + 0x00800080u, 0x07050301u);
                     }
-                wait_loads();
-                __syncthreads();
-                if (step + 1 < to) {
-                    if (T::BUFS == 2) copy_to_lds(gv + (int64_t)(step + 1) * T::STEP, ((step - from) & 1) ? s_a : s_b, T::STEP, wave, lane);
-                    load_e(step + 1);
-                }
+                const uint8_t* buf = arrive(gv, from, step, to);
+                if (step + 1 < to) load_e(step + 1);
 #pragma unroll
                 for (int sub = 0; sub < SUBS; sub++) {
                     const bool second = __any((b1[sub][0] | b1[sub][1] | b1[sub][2] | b1[sub][3]) != 0);
