@@ -51,6 +51,15 @@ __device__ inline int32_t exp_q(uint32_t z, const int32_t* hi, const int32_t* lo
     z = min(z, (uint32_t)atlas::ExpTable::Z_MAX);
     return (int32_t)(__umul24((uint32_t)hi[z >> atlas::ExpTable::LOG_BASE], (uint32_t)lo[z & (atlas::ExpTable::BASE - 1)]) >> SCALE);      // <= 2^28
 }
+// The same from tables in LDS that are shifted up by 9: the upper half of one 24-bit product is (hi lo) >> 14
+template <uint32_t NT>
+__device__ inline void load_exp(uint32_t* s_hi, uint32_t* s_lo) {
+    for (uint32_t i = threadIdx.x; i < 512; i += NT) { s_hi[i] = (uint32_t)g_exp.hi[i] << 9; s_lo[i] = (uint32_t)g_exp.lo[i] << 9; }
+}
+__device__ inline uint32_t exp_lds(uint32_t z, const uint32_t* s_hi, const uint32_t* s_lo) {
+    z = min(z, (uint32_t)atlas::ExpTable::Z_MAX);
+    return (uint32_t)(((uint64_t)(s_hi[z >> atlas::ExpTable::LOG_BASE] & 0xffffff) * (s_lo[z & (atlas::ExpTable::BASE - 1)] & 0xffffff)) >> 32);
+}
 // sums of e saturate: from 2^28 + 1 on the reciprocal floor(2^28 / sum) is 0 whatever the sum
 __device__ inline uint32_t add_sat(uint32_t a, uint32_t b) { const uint32_t s = a + b; return s < a ? 0xffffffffu : s; }
 

@@ -282,7 +282,8 @@ template <class CT, int KS, bool FAST>
 __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint32_t pitch) {
     constexpr int D = KS * 64;
     extern __shared__ __align__(16) int32_t s_x[];                 // [16][pitch] scores; the sums of the products afterwards
-    __shared__ int32_t s_hi[512], s_lo[512], s_m[FUSED_WAVES][16];
+    __shared__ uint32_t s_hi[512], s_lo[512];
+    __shared__ int32_t s_m[FUSED_WAVES][16];
     __shared__ uint32_t s_s[FUSED_WAVES][16], s_mag[3];
     const RowTile R = row_tile(A, blockIdx.x / A.KV, blockIdx.x % A.KV);
     if (!R.any) return;
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
     const bool mine = r < R.n_rows;
     const uint32_t limit = mine ? min(key_limit(A, R.s, r / A.G), R.s.keys) : 0;
     const uint32_t k1 = min(key_limit(A, R.s, (R.row0 + rows - 1) / A.G), R.s.keys);      // the most that a row of the tile sees
-    s_hi[tid] = g_exp.hi[tid]; s_lo[tid] = g_exp.lo[tid];
+    load_exp<FUSED_WAVES * 64>(s_hi, s_lo);
     if (tid < 3) s_mag[tid] = 0;
     __syncthreads();
     Range rk;
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
             v4i* at = (v4i*)(s_x + l * pitch + j0 + 16 * t + 4 * g);
             v4i x = *at;
 #pragma unroll
-            for (int i = 0; i < 4; i++) { x[i] = exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo); sum += (uint32_t)x[i]; }      // GONE lies 2^30 below: 0
+            for (int i = 0; i < 4; i++) { x[i] = (int)exp_lds((uint32_t)m - (uint32_t)x[i], s_hi, s_lo); sum += (uint32_t)x[i]; }      // GONE lies 2^30 below: 0
             *at = x;
         }
     sum += (uint32_t)__shfl_xor((int)sum, 16);
@@ -487,8 +488,8 @@ __device__ inline void each_share(const Args& A, const Split& S, uint32_t t, uin
 // a wave takes a row of the share at a time, 256 keys by 4 per lane
 __global__ __launch_bounds__(256) void k_split_sums(Args A, Split S) {
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    __shared__ int32_t s_hi[512], s_lo[512];
-    for (uint32_t i = tid; i < 512; i += 256) { s_hi[i] = g_exp.hi[i]; s_lo[i] = g_exp.lo[i]; }
+    __shared__ uint32_t s_hi[512], s_lo[512];
+    load_exp<256>(s_hi, s_lo);
     __syncthreads();
     const Line line(A, S);
     const uint32_t end = line.begin(blockIdx.x + 1);
@@ -505,7 +506,7 @@ __global__ __launch_bounds__(256) void k_split_sums(Args A, Split S) {
             for (uint32_t j = X.k0 + lane * 4; j < X.k1; j += 256) {
                 const v4i x = *(const v4i*)(S.scores + (int64_t)(X.row + r) * S.pitch + j);      // behind the last key: GONE up to the next multiple of 64
 #pragma unroll
-                for (int i = 0; i < 4; i++) sum = __builtin_elementwise_add_sat(sum, (uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo));
+                for (int i = 0; i < 4; i++) sum = __builtin_elementwise_add_sat(sum, exp_lds((uint32_t)m - (uint32_t)x[i], s_hi, s_lo));
             }
             for (int o = 32; o; o >>= 1) sum = __builtin_elementwise_add_sat(sum, (uint32_t)__shfl_xor((int)sum, o));
             if (lane == 0) S.csum[X.part + r] = m == GONE ? 0 : sum;
@@ -517,11 +518,12 @@ template <class CT, int KS, bool FAST>
 __global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, l = lane & 15;
     constexpr int D = KS * 64, VS = value_steps(KS);
-    __shared__ int32_t s_hi[512], s_lo[512], s_m[16];
+    __shared__ uint32_t s_hi[512], s_lo[512];
+    __shared__ int32_t s_m[16];
     __shared__ uint32_t s_sum[16];
     __shared__ unsigned long long s_o[TILE_ROWS * D];
     __shared__ uint32_t s_mag;
-    for (uint32_t i = tid; i < 512; i += 256) { s_hi[i] = g_exp.hi[i]; s_lo[i] = g_exp.lo[i]; }
+    load_exp<256>(s_hi, s_lo);
     const Line line(A, S);
     const uint32_t end = line.begin(blockIdx.x + 1);
 #pragma unroll 1
@@ -559,7 +561,7 @@ __global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
                     const v4i x = *(const v4i*)(from + j + 16 * t);
                     uint32_t p[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) p[i] = __umul24((uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
+                    for (int i = 0; i < 4; i++) p[i] = __umul24(exp_lds((uint32_t)m - (uint32_t)x[i], s_hi, s_lo), inv) >> SCALE;
                     int a, b;
                     weight_bytes(p, a, b);
                     w0[t] = a; w1[t] = b;

@@ -148,9 +148,15 @@ __device__ inline int32_t rescale(int32_t s, int32_t c) {
 // shifted down first (the floors nest)
 template <bool LONG>
 __device__ inline int32_t combine(int32_t a0, int32_t a1, int32_t a2, int32_t a3, int32_t a4) {
-    const uint32_t hi = (uint32_t)a2 + ((uint32_t)a3 << 8) + ((uint32_t)a4 << 16);
+    uint32_t hi = (uint32_t)a2 + ((uint32_t)a3 << 8) + ((uint32_t)a4 << 16);
+    asm("" : "+v"(hi));                       // or the shift by 2 is distributed over the three: an instruction more
     const int32_t lo = LONG ? ((a0 >> 8) + a1) >> 6 : (a0 + (int32_t)((uint32_t)a1 << 8)) >> SCALE;
     return (int32_t)((hi << 2) + (uint32_t)lo);
+}
+
+// m - rescale(s), the subtraction inside the multiply-add
+__device__ inline uint32_t below(int32_t m, int32_t s, int32_t c) {
+    return (uint32_t)(__mul24(s >> SCALE, -c) + m) - (__umul24((uint32_t)s & (ONE - 1), (uint32_t)c) >> SCALE);
 }
 
 template <int DP>
@@ -175,13 +181,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
     using T = TileShape<DP>;
     constexpr int F = T::F, SPLIT = T::SPLIT, SUBS = T::SUBS;
     extern __shared__ __align__(16) uint8_t lds[];
-    int32_t* s_hi = (int32_t*)lds;
-    int32_t* s_lo = s_hi + 512;
+    uint32_t* s_hi = (uint32_t*)lds;
+    uint32_t* s_lo = s_hi + 512;
     uint8_t* s_a = lds + T::LUT;
     uint32_t* s_red = (uint32_t*)(s_a + T::STEP * T::BUFS);        // 256 words
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, l32 = lane & 31;
     const uint32_t group = wave / SPLIT, part = wave % SPLIT;
-    for (uint32_t i = tid; i < 512; i += 256) { s_hi[i] = g_exp.hi[i]; s_lo[i] = g_exp.lo[i]; }
+    load_exp<256>(s_hi, s_lo);
     // e of this wave's rows: [tile of 32 keys][lane][16], 2 bytes each, in the order in which a lane has its scores
     const uint32_t held_steps = held / T::KEYS;
     // Work lists by kv head: workgroups go to the 8 XCDs in turn, and those of one XCD begin with the same heads, so that its L2 holds their planes.  A list that
@@ -277,28 +283,32 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
                 return s_a + at * T::STEP;
             }
         };
-        // the scores of sub-tile `sub` of the step in `buf`, in one sweep over the fragments with five accumulators
+        // the scores of sub-tile `sub` of the step in `buf` before the Mul node, in one sweep over the fragments with five accumulators
         auto scores = [&](const uint8_t* buf, int sub, v16i& x) {
-            v16i a0 = {}, a1 = {}, a2 = {}, a3 = {}, a4 = {};
+            // All fragments are read first: left to itself the compiler reads each into the same registers right before its products, and LDS' latency
+            // stands between every four of them
+            v4i k[F][3];
             const v4i* kf = (const v4i*)(buf + sub * T::TILE) + lane;
 #pragma unroll
+            for (int f = 0; f < F; f++)
+#pragma unroll
+                for (int p = 0; p < 3; p++) k[f][p] = kf[f * 192 + p * 64];
+            __builtin_amdgcn_sched_barrier(0);
+            v16i a0 = {}, a1 = {}, a2 = {}, a3 = {}, a4 = {};
+#pragma unroll
             for (int f = 0; f < F; f++) {
-                const v4i k0 = kf[f * 192], k1 = kf[f * 192 + 64], k2 = kf[f * 192 + 128];
-                a4 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q2[f], a4, 0, 0, 0);
-                a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q1[f], a3, 0, 0, 0);
-                a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k2, q0[f], a2, 0, 0, 0);
-                a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q0[f], a1, 0, 0, 0);
-                a0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q0[f], a0, 0, 0, 0);
-                a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q2[f], a3, 0, 0, 0);
-                a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k1, q1[f], a2, 0, 0, 0);
-                a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q1[f], a1, 0, 0, 0);
-                a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k0, q2[f], a2, 0, 0, 0);
+                a4 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[f][2], q2[f], a4, 0, 0, 0);
+                a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[f][2], q1[f], a3, 0, 0, 0);
+                a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[f][2], q0[f], a2, 0, 0, 0);
+                a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[f][1], q0[f], a1, 0, 0, 0);
+                a0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[f][0], q0[f], a0, 0, 0, 0);
+                a3 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[f][1], q2[f], a3, 0, 0, 0);
+                a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[f][1], q1[f], a2, 0, 0, 0);
+                a1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[f][0], q1[f], a1, 0, 0, 0);
+                a2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[f][0], q2[f], a2, 0, 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < 16; i++) x[i] = combine<DP == 256>(a0[i], a1[i], a2[i], a3[i], a4[i]);
-            if (A.mul != ONE)
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = rescale(x[i], A.mul);
         };
         // which of a lane's 16 keys of a sub-tile count, as bits 8 c + i of 4 half + ..; ~0 where all of the wave's do
         auto seen = [&](uint32_t step, int sub) -> uint32_t {
@@ -334,7 +344,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
                         uint32_t e[16] = {};
                         if (any) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) e[i] = (uint32_t)exp_q((uint32_t)m - (uint32_t)x[i], s_hi, s_lo);
+                            for (int i = 0; i < 16; i++) e[i] = exp_lds(below(m, x[i], A.mul), s_hi, s_lo);
                             if (in != ~0u)
 #pragma unroll
                                 for (int i = 0; i < 16; i++) e[i] &= (uint32_t)((int32_t)(in << (31 - (8 * (i / 4) + i % 4))) >> 31);
@@ -362,6 +372,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
         for (int what = MAX; what <= SUM; what++) {
             pass(0, n_steps, what);
             // the other half-wave has the rest of the row's keys, and so have the waves that share the rows
+            // (the Mul node's rescale does not change the order: it is left to the maximum)
             if (what == MAX) m = max(m, __shfl_xor(m, 32)); else sum = __builtin_elementwise_add_sat(sum, (uint32_t)__shfl_xor((int)sum, 32));
             if (SPLIT > 1) {
                 if (half == 0) s_red[wave * 32 + l32] = what == MAX ? (uint32_t)m : sum;
@@ -372,6 +383,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
                 }
                 __syncthreads();
             }
+            if (what == MAX) m = rescale(m, A.mul);
         }
         const uint32_t inv = sum ? (1u << (2 * SCALE)) / sum : 0;
 
@@ -401,21 +413,30 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Pl
                         b1[sub][c] = (int)__builtin_amdgcn_perm(b + 0x00800080u, a + 0x00800080u, 0x07050301u);
                     }
                 const uint8_t* buf = arrive(gv, from, step, to);
+                v4i v[SUBS][T::OF][3];
+#pragma unroll
+                for (int sub = 0; sub < SUBS; sub++)
+#pragma unroll
+                    for (int f = 0; f < T::OF; f++)
+#pragma unroll
+                        for (int p = 0; p < 3; p++) v[sub][f][p] = ((const v4i*)(buf + sub * T::TILE + (part * T::OF + f) * 3072) + lane)[p * 64];
                 if (step + 1 < to) load_e(step + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int sub = 0; sub < SUBS; sub++) {
                     const bool second = __any((b1[sub][0] | b1[sub][1] | b1[sub][2] | b1[sub][3]) != 0);
-                    const v4i* vf = (const v4i*)(buf + sub * T::TILE + part * T::OF * 3072) + lane;
 #pragma unroll
                     for (int f = 0; f < T::OF; f++) {
-                        const v4i x0 = vf[f * 192], x1 = vf[f * 192 + 64], x2 = vf[f * 192 + 128];
-                        o0[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x0, b0[sub], o0[f], 0, 0, 0);
-                        o1[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x1, b0[sub], o1[f], 0, 0, 0);
-                        o2[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x2, b0[sub], o2[f], 0, 0, 0);
-                        if (second) {
-                            const v16i y0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x0, b1[sub], v16i{}, 0, 0, 0), y1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x1, b1[sub], v16i{}, 0, 0, 0),
-                                       y2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(x2, b1[sub], v16i{}, 0, 0, 0);
-                            o0[f] += y0 * 256; o1[f] += y1 * 256; o2[f] += y2 * 256;
+                        o0[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(v[sub][f][0], b0[sub], o0[f], 0, 0, 0);
+                        o1[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(v[sub][f][1], b0[sub], o1[f], 0, 0, 0);
+                        o2[f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(v[sub][f][2], b0[sub], o2[f], 0, 0, 0);
+                    }
+                    if (second) {
+#pragma unroll
+                        for (int f = 0; f < T::OF; f++) {
+                            o0[f] += __builtin_amdgcn_mfma_i32_32x32x32_i8(v[sub][f][0], b1[sub], v16i{}, 0, 0, 0) * 256;
+                            o1[f] += __builtin_amdgcn_mfma_i32_32x32x32_i8(v[sub][f][1], b1[sub], v16i{}, 0, 0, 0) * 256;
+                            o2[f] += __builtin_amdgcn_mfma_i32_32x32x32_i8(v[sub][f][2], b1[sub], v16i{}, 0, 0, 0) * 256;
                         }
                     }
                 }
