@@ -24,27 +24,37 @@ Args args_of(const atlas_attn_shape_t* s, const atlas_attn_rows_t* q, const int3
 
 // head sizes are padded to the fragments of the tile kernel
 int padded_dim(size_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+// f(padded dims, waves to a row)
 template <class F>
-int with_dim(int dp, F f) {
+auto with_shape(int dp, bool few, F f) {
+    auto go = [&](auto d) {
+        constexpr int DP = decltype(d)::value;
+        if (few) return f(d, std::integral_constant<int, tile_split(DP, true)>{});
+        return f(d, std::integral_constant<int, tile_split(DP, false)>{});
+    };
     switch (dp) {
-        case 32: return f(std::integral_constant<int, 32>{});
-        case 64: return f(std::integral_constant<int, 64>{});
-        case 128: return f(std::integral_constant<int, 128>{});
-        default: return f(std::integral_constant<int, 256>{});
+        case 32: return go(std::integral_constant<int, 32>{});
+        case 64: return go(std::integral_constant<int, 64>{});
+        case 128: return go(std::integral_constant<int, 128>{});
+        default: return go(std::integral_constant<int, 256>{});
     }
 }
 
 // the digit planes and the held e of the tile kernel in a workspace; cached_keys = 0: packed prompts
 struct PlanesLayout {
+    bool few;
     size_t max_keys, tiles, per_seq, held, work, wgs, v_at, mag_at, there_at, next_at, e_at, bytes;
     PlanesLayout(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t cached_keys) {
         const size_t slack = 4;                                        // a step reads up to 4 tiles: its last ones may lie behind a sequence's end
-        const int dp = padded_dim(s->head_dim), rows = with_dim(dp, [](auto d) { return (int)TileShape<decltype(d)::value>::ROWS; });
+        const int dp = padded_dim(s->head_dim);
+        const size_t G = s->n_heads / s->n_kv_heads, usual = with_shape(dp, false, [](auto d, auto w) { return TileShape<decltype(d)::value, decltype(w)::value>::ROWS; });
+        few = (n_tokens * G / usual + n_seqs) * s->n_kv_heads < (dp <= 64 ? 512 : 192);
+        const size_t rows = with_shape(dp, few, [](auto d, auto w) { return TileShape<decltype(d)::value, decltype(w)::value>::ROWS; });
         per_seq = (cached_keys + 31) / 32;
         max_keys = cached_keys ? cached_keys : n_tokens;
         tiles = (cached_keys ? n_seqs * per_seq : n_tokens / 32 + n_seqs) + slack;
         held = std::min<size_t>((max_keys + 127) / 128 * 128, HELD);
-        work = (n_tokens * (s->n_heads / s->n_kv_heads) / rows + n_seqs) * s->n_kv_heads;
+        work = (n_tokens * G / rows + n_seqs) * s->n_kv_heads;
         wgs = std::min<size_t>(work, TILE_WGS);
         const size_t one = tiles * s->n_kv_heads * (size_t)(dp / 32 * 3072);
         v_at = one;
@@ -61,18 +71,21 @@ struct PlanesLayout {
 };
 template <class CT>
 int launch_tiles(const Args& A, const PlanesLayout& L, const Planes& P, hipStream_t stream) {
-    return with_dim(padded_dim(A.d), [&](auto dim) -> int {
-        constexpr int DP = decltype(dim)::value;
-        using T = TileShape<DP>;
-        if (L.work > 0x7fffffff || L.tiles > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows for one call");
+    if (L.work > 0x7fffffff || L.tiles > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows for one call");
+    return with_shape(padded_dim(A.d), L.few, [&](auto dim, auto split) -> int {
+        constexpr int DP = decltype(dim)::value, SPLIT = decltype(split)::value;
+        using T = TileShape<DP, SPLIT>;
         k_attn_planes<CT, DP><<<dim3((unsigned)L.tiles, A.KV), 256, 0, stream>>>(A, P);
-        auto* k = L.max_keys > HELD ? &k_attn_tile<CT, DP, true> : &k_attn_tile<CT, DP, false>;
+        auto* k = L.max_keys > HELD ? &k_attn_tile<CT, DP, SPLIT, true> : &k_attn_tile<CT, DP, SPLIT, false>;
         if (T::LDS > 65536) HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS));
         k<<<(unsigned)L.wgs, 256, T::LDS, stream>>>(A, P, (uint32_t)L.work, (uint32_t)L.held);
         return ATLAS_OK;
     });
 }
-bool many_rows(size_t n_seqs, size_t n_tokens) { return n_tokens > 4 * n_seqs; }
+// On average more than 96 query rows to a sequence and kv head: tiles; below, 16 rows at a time that read the cache themselves.  One MI355X, int32, 64 sequences of 2000
+// keys: 32 heads of 128 over 8, 16 new tokens (64 rows) 820 us in tiles and 833 us in 16 rows, 32 new tokens 961 and 1599 us; 16 heads of 64, 32 new
+// tokens (32 rows) 1346 and 581 us.
+bool many_rows(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens) { return n_tokens * (s->n_heads / s->n_kv_heads) > 96 * n_seqs; }
 // Few rows: the workspace of the split path
 struct SplitLayout {
     Split S{};
@@ -122,11 +135,13 @@ int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
     return ATLAS_OK;
 }
 
-// One launch while LDS holds the scores — up to 1024 keys, beyond that only where there are workgroups enough for the chip: 16 heads of 64 over 1000 / 2000 keys
-// take 27 / 42 us in one launch of 16 workgroups and 30 / 31 us in the split path's five launches
-bool fused(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys) {
+// One launch while LDS holds the scores.  Few rows: up to 1024 keys, beyond that where there are workgroups enough for the chip (16 heads of 64, one token over
+// 1000 / 2000 keys: 27 / 42 us in one launch of 16 workgroups, 30 / 31 us in the split path's five; 16 such tokens over 2000 keys: 56 and 84 us).  Many rows: while
+// the 16-row workgroups fit the chip about once (16 heads of 64, a prompt of 512: 40 us and 55 us in tiles, of 1024: 92 and 85 us).
+bool fused(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys, bool many) {
     const size_t wgs = (n_tokens * (s->n_heads / s->n_kv_heads) / TILE_ROWS + n_seqs) * s->n_kv_heads;
-    return max_keys <= 1024 || (max_keys <= fused_keys(s->head_dim) && wgs >= 256);
+    if (max_keys > fused_keys(s->head_dim)) return false;
+    return many ? wgs <= 640 : max_keys <= 1024 || wgs >= 256;
 }
 template <class CT>
 int launch_fused(const Args& A, size_t max_keys, hipStream_t stream) {
@@ -149,7 +164,7 @@ extern "C" {
 
 size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens)) return 0;
-    return fused(shape, n_seqs, n_tokens, n_tokens) ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
+    return fused(shape, n_seqs, n_tokens, n_tokens, true) ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
 }
 
 int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
@@ -171,7 +186,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (int rc = L.on_device({q->d, k->d, v->d, d_cu_seqlens, out->d, d_workspace})) return rc;
     Args A = args_of(shape, q, d_cu_seqlens, n_seqs, n_tokens, out);
     A.k = rows_of(k); A.v = rows_of(v);
-    if (fused(shape, n_seqs, n_tokens, n_tokens)) {
+    if (fused(shape, n_seqs, n_tokens, n_tokens, true)) {
         if (int rc = launch_fused<int32_t>(A, n_tokens, L.stream)) return rc;
         return L.end();
     }
@@ -182,8 +197,8 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
 
 size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
-    if (fused(shape, n_seqs, n_tokens, max_blocks * cache->block_size)) return 16;
-    return many_rows(n_seqs, n_tokens) ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_blocks * cache->block_size, 1)).bytes
+    if (fused(shape, n_seqs, n_tokens, max_blocks * cache->block_size, many_rows(shape, n_seqs, n_tokens))) return 16;
+    return many_rows(shape, n_seqs, n_tokens) ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_blocks * cache->block_size, 1)).bytes
                                        : SplitLayout(shape, n_seqs, n_tokens, max_blocks * cache->block_size, nullptr).bytes;
 }
 
@@ -207,11 +222,11 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     Args A = args_of(shape, q, d_cu_new, n_seqs, n_tokens, out);
     A.ck = cache->d_k; A.cv = cache->d_v; A.lens = d_kv_lens; A.table = d_block_table; A.table_stride = (int64_t)table_stride;
     A.n_blocks = (uint32_t)cache->n_blocks; A.log_block = log2_of(cache->block_size); A.max_keys = (uint32_t)(max_blocks * cache->block_size);
-    if (fused(shape, n_seqs, n_tokens, A.max_keys)) {
+    if (fused(shape, n_seqs, n_tokens, A.max_keys, many_rows(shape, n_seqs, n_tokens))) {
         if (int rc = cache->bits == 16 ? launch_fused<int16_t>(A, A.max_keys, L.stream) : launch_fused<int32_t>(A, A.max_keys, L.stream)) return rc;
         return L.end();
     }
-    if (many_rows(n_seqs, n_tokens)) {
+    if (many_rows(shape, n_seqs, n_tokens)) {
         const PlanesLayout P(shape, n_seqs, n_tokens, std::max<size_t>(A.max_keys, 1));
         if (int rc = cache->bits == 16 ? launch_tiles<int16_t>(A, P, P.at(d_workspace, shape), L.stream) : launch_tiles<int32_t>(A, P, P.at(d_workspace, shape), L.stream)) return rc;
         return L.end();

@@ -159,10 +159,10 @@ __device__ inline uint32_t below(int32_t m, int32_t s, int32_t c) {
     return (uint32_t)(__mul24(s >> SCALE, -c) + m) - (__umul24((uint32_t)s & (ONE - 1), (uint32_t)c) >> SCALE);
 }
 
-template <int DP>
+// SPLIT waves share 32 query rows: each scores its own keys and carries 1 / SPLIT of the output's dims
+template <int DP, int SPLIT>
 struct TileShape {
     static constexpr int F = DP / 32;                         // fragments of 32 dims
-    static constexpr int SPLIT = DP <= 64 ? 1 : DP / 64;      // waves that share 32 query rows: each scores its own keys and carries 64 of the output's dims
     static constexpr int GROUPS = 4 / SPLIT, ROWS = 32 * GROUPS;
     static constexpr int SUBS = SPLIT < 2 ? 2 : SPLIT;        // key sub-tiles of 32 per step
     static constexpr int KEYS = 32 * SUBS, MY_SUBS = SUBS / SPLIT;
@@ -171,15 +171,20 @@ struct TileShape {
     static constexpr int BUFS = DP == 256 ? 1 : 3;            // two steps are on their way while one is worked on; of 256 dims 160 KB of LDS hold one step
     static constexpr int COPIES = STEP / 4096;                // that a wave has issued for a step, at least
     static constexpr uint32_t LUT = 4096, LDS = LUT + STEP * BUFS + 1024;
+    static constexpr int WAVES = LDS > 80 * 1024 ? 1 : 2;     // per SIMD
 };
+// Many tiles: two workgroups per CU, as many rows to a fragment of keys as the registers carry.  FEW tiles: half the rows and twice the waves to a row, so that a tile is
+// done in half the time.  A prompt of 2000 with 16 heads of 64 (266 tiles): 206 -> 149 us; with 15 heads of 80 (125 tiles for 512 tokens, 474 for 2000, one workgroup per CU
+// then): 64 -> 54 us, but 183 -> 233 us.
+constexpr int tile_split(int dp, bool few) { return dp == 32 ? 1 : dp == 64 ? (few ? 2 : 1) : dp == 128 ? (few ? 4 : 2) : 4; }
 // The workgroups that fit the chip at once take tiles from a counter.  Each has room for the e of HELD keys of its rows; where a tile has more keys, the scores of the
 // others are taken a third time.
 constexpr uint32_t TILE_WGS = 512, HELD = 16384;
 
-template <class CT, int DP, bool LONG>      // LONG: tiles may have more than HELD keys; the product's sums then live through another pass over scores
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void k_attn_tile(Args A, Planes P, uint32_t n_work, uint32_t held) {
-    using T = TileShape<DP>;
-    constexpr int F = T::F, SPLIT = T::SPLIT, SUBS = T::SUBS;
+template <class CT, int DP, int SPLIT, bool LONG>      // LONG: tiles may have more than HELD keys; the product's sums then live through another pass over scores
+__global__ __launch_bounds__(256, (TileShape<DP, SPLIT>::WAVES)) void k_attn_tile(Args A, Planes P, uint32_t n_work, uint32_t held) {
+    using T = TileShape<DP, SPLIT>;
+    constexpr int F = T::F, SUBS = T::SUBS;
     extern __shared__ __align__(16) uint8_t lds[];
     uint32_t* s_hi = (uint32_t*)lds;
     uint32_t* s_lo = s_hi + 512;
