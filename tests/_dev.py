@@ -64,4 +64,10 @@ class Dev:
 
 
 def workspace(n):
-    return Dev(np.full(max(n, 16), 0xA5, np.uint8))       # what an allocation holds is nobody's business
+    """n bytes of device memory that hold anything but zeros"""
+    b = Buffer(n)
+    ok(hip().hipMemset(b.p, C.c_int(0xA5), C.c_size_t(max(n, 16))))
+    ok(hip().hipDeviceSynchronize())
+    v = Dev(np.empty(0, np.uint8), b, 0, (max(n, 16),), (1,))
+    v.total = max(n, 16)
+    return v

@@ -24,17 +24,30 @@ def any_int32(rng, shape):
     return np.where(rng.random(shape) < 0.1, rng.choice([-(1 << 31), (1 << 31) - 1, 0, -1, 1 << 23, -(1 << 23)], size=shape), x).astype(np.int32)
 
 
-def run_prompt(A, q, k, v, lens, mul=ONE, causal=True, rows=None, views=None):
-    """rows: the rows of the arrays (more than the sequences use); views: strided device views of q, k, v"""
+# Which kernels take a call goes by what the host knows of it: the rows of the arrays (prompts) and the columns of the table (cached).  Rows behind the last
+# sequence, and columns that no sequence uses, send the same sequences through each: all scores in LDS; tiles; tiles with more keys than their e is held for;
+# keys split over workgroups.
+PROMPT_ROWS = (0, 2100, 16500)
+CACHED_KEYS = (0, 1100, 4200, 16600)
+
+
+def run_prompt(A, q, k, v, lens, mul=ONE, causal=True, pads=PROMPT_ROWS):
     import jolt_atlas_amd.attention as T
     n, H, d = q.shape
     at = T.Attention(H, k.shape[1], d, mul, causal)
     cu = Dev(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
-    out = Dev(np.full((n, H, d), MARK, np.int32))
-    ws = workspace(at.prompt_workspace_bytes(len(lens), n))
-    dq, dk, dv = views or (Dev(q), Dev(k), Dev(v))
-    assert at.prompt(dq, dk, dv, cu, out, ws) is out
-    return out.numpy()
+    got = None
+    for rows in pads:
+        rows = max(rows, n)
+        more = lambda x, fill: np.concatenate([x, np.full((rows - n,) + x.shape[1:], fill, np.int32)])  # noqa: E731
+        out = Dev(np.full((rows, H, d), MARK, np.int32))
+        ws = workspace(at.prompt_workspace_bytes(len(lens), rows))
+        assert at.prompt(Dev(more(q, -(1 << 31))), Dev(more(k, -(1 << 31))), Dev(more(v, -(1 << 31))), cu, out, ws) is out
+        x = out.numpy()
+        assert (x[n:] == MARK).all(), rows
+        assert got is None or np.array_equal(got, x[:n]), rows
+        got = x[:n]
+    return got
 
 
 SHAPES = [(1, 1, 1), (4, 4, 4), (4, 4, 16), (4, 2, 20), (6, 2, 32), (5, 5, 33), (16, 16, 64), (8, 2, 64), (3, 1, 80), (8, 1, 96), (12, 4, 128), (7, 7, 100), (2, 1, 192), (3, 3, 256), (5, 1, 255)]
@@ -158,16 +171,24 @@ def paged(rng, keys, KV, d, block, bits, spare=3, cols=None, sigma=None):
     return ck, cv, table, flat
 
 
-def run_cached(q, ck, cv, table, keys, new, mul=ONE, causal=True, table_view=None):
+def run_cached(q, ck, cv, table, keys, new, mul=ONE, causal=True, table_view=None, caps=CACHED_KEYS):
     import jolt_atlas_amd.attention as T
     n, H, d = q.shape
     at = T.Attention(H, ck.shape[1], d, mul, causal)
     cache = T.KVCache(Dev(ck), Dev(cv))
-    out = Dev(np.full(q.shape, MARK, np.int32))
-    tab = table_view or Dev(table)
-    ws = workspace(at.cached_workspace_bytes(len(new), n, cache, tab.shape[1]))
-    at.cached(Dev(q), Dev(np.cumsum([0] + list(new)).astype(np.int32)), Dev(np.array(keys, np.int32)), cache, tab, out, ws)
-    return out.numpy()
+    cu, lens, dq = Dev(np.cumsum([0] + list(new)).astype(np.int32)), Dev(np.array(keys, np.int32)), Dev(q)
+    got = None
+    for cap in ((0,) if table_view else caps):
+        tab = table_view
+        if tab is None:
+            cols = max(-(-cap // ck.shape[2]), table.shape[1])
+            tab = Dev(np.concatenate([table, np.full((len(table), cols - table.shape[1]), 2 ** 31 - 1, np.int32)], axis=1))
+        out = Dev(np.full(q.shape, MARK, np.int32))
+        at.cached(dq, cu, lens, cache, tab, out, workspace(at.cached_workspace_bytes(len(new), n, cache, tab.shape[1])))
+        x = out.numpy()
+        assert got is None or np.array_equal(got, x), cap
+        got = x
+    return got
 
 
 def want_cached(q, ck, cv, table, flat, keys, new, mul=ONE, causal=True):
@@ -192,12 +213,13 @@ def test_cached_single_tokens(atlas, H, KV, d, bits, block):
     assert np.array_equal(run_cached(q, ck, cv, table, keys, new, mul), want_cached(q, ck, cv, table, flat, keys, new, mul))
 
 
-@pytest.mark.parametrize("H,KV,d,bits,block", [(4, 4, 16, 32, 16), (8, 2, 128, 32, 32), (8, 2, 64, 16, 8), (6, 2, 100, 32, 64), (2, 1, 256, 16, 128), (16, 2, 33, 32, 4)])
+@pytest.mark.parametrize("H,KV,d,bits,block", [(4, 4, 16, 32, 16), (8, 2, 128, 32, 32), (8, 2, 64, 16, 8), (6, 2, 100, 32, 64), (2, 1, 256, 16, 128), (16, 2, 33, 32, 4), (8, 1, 128, 16, 16)])
 @pytest.mark.parametrize("causal", [True, False])
-def test_cached_chunks(atlas, H, KV, d, bits, block, causal):
+@pytest.mark.parametrize("many", [False, True])
+def test_cached_chunks(atlas, H, KV, d, bits, block, causal, many):
     """several new tokens beside single ones, a request that pauses, a prompt without a past, more new tokens than keys (rows that see nothing)"""
     rng = np.random.default_rng(d)
-    keys, new = [90, 200, 33, 70, 300, 4, 0, 1], [17, 1, 33, 0, 70, 9, 2, 1]
+    keys, new = ([90, 200, 33, 70, 300, 4, 0, 1], [17, 1, 33, 0, 70, 9, 2, 1]) if not many else ([300, 260, 7], [201, 120, 9])
     ck, cv, table, flat = paged(rng, keys, KV, d, block, bits)
     q = values(rng, (sum(new), H, d))
     mul = int(round(ONE / np.sqrt(d)))
@@ -309,6 +331,31 @@ def test_cached_offsets_past_32_bits(atlas):
         want = was.copy()
         want[:, 255], want[:, 0] = x[0].clip(-32768, 32767), x[1].clip(-32768, 32767)
         assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("H,KV,d,n,bits", [(2, 1, 64, 3000, 0), (2, 2, 128, 2500, 0), (1, 1, 32, 5000, 0), (3, 1, 200, 1500, 0), (1, 1, 16, 17000, 0), (2, 1, 128, 17000, 0), (4, 1, 64, 17001, 32),
+                                           (2, 1, 256, 17001, 16), (16, 16, 64, 700, 0), (16, 8, 128, 500, 0)])
+def test_long_sequences_on_some_of_their_rows(atlas, H, KV, d, n, bits):
+    """many tiles, keys past what a tile holds e for; prompts (bits = 0) and chunks over a cache"""
+    rng = np.random.default_rng(n)
+    mul = int(round(ONE / np.sqrt(d)))
+    new = n if bits == 0 else 150
+    q, k, v = values(rng, (new, H, d)), values(rng, (n, KV, d)), values(rng, (n, KV, d))
+    if bits == 0:
+        got = run_prompt(atlas, q, k, v, [n], mul, pads=(0,))
+    else:
+        if bits == 16:
+            k, v = (k // 8).clip(-32768, 32767), (v // 8).clip(-32768, 32767)
+        B = 32
+        up = -(-n // B)
+        ids = rng.permutation(up).astype(np.int32)
+        pages = np.zeros((2, up, KV, B, d), np.int16 if bits == 16 else np.int32)
+        for c, x in zip(pages, (k, v)):
+            c[ids] = np.concatenate([x, np.zeros((up * B - n, KV, d), np.int32)]).reshape(up, B, KV, d).transpose(0, 2, 1, 3)
+        got = run_cached(q, pages[0], pages[1], ids[None], [n], [new], mul, caps=(0,))
+    rows = sorted({0, 1, 31, 32, 63, new // 2, new - 1, *rng.integers(0, new, 6).tolist()})
+    want = attend(q[rows], k, v, [n - new + r + 1 for r in rows], mul)
+    assert np.array_equal(got[rows], want)
 
 
 # ------------------------------------------------------------------------------------------------------------------- write
