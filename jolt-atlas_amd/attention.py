@@ -42,32 +42,46 @@ def _stream(stream):
     return None if stream is None else (stream or 1)          # ATLAS_STREAM_DEFAULT
 
 
+_names = {}                         # dtype -> "int32", ...: a call looks its arrays' types up six times
+
+
+def _name(dtype):
+    n = _names.get(dtype)
+    if n is None:
+        n = _names[dtype] = str(dtype).rpartition(".")[2]
+    return n
+
+
 def _is(t, name, dtype, ndim):
-    if len(t.shape) != ndim or str(t.dtype).rpartition(".")[2] != dtype:
-        raise ValueError(f"{name}: a {ndim}-dimensional {dtype} array expected, got {str(t.dtype)} {tuple(t.shape)}")
-    return t
+    if len(t.shape) != ndim or _name(t.dtype) != dtype:
+        raise ValueError(f"{name}: a {ndim}-dimensional {dtype} array expected, got {t.dtype} {tuple(t.shape)}")
 
 
 def _vector(t, name, dtype, n=None):
     """a contiguous array of `n` elements (None: any number), as a pointer"""
-    _is(t, name, dtype, 1)
-    if n is not None and t.shape[0] < n:
-        raise ValueError(f"{name}: {n} elements expected, got {t.shape[0]}")
-    if t.shape[0] > 1 and t.stride()[0] != 1:
+    shape = t.shape
+    if len(shape) != 1 or _name(t.dtype) != dtype:
+        _is(t, name, dtype, 1)
+    if n is not None and shape[0] < n:
+        raise ValueError(f"{name}: {n} elements expected, got {shape[0]}")
+    if shape[0] > 1 and t.stride()[0] != 1:
         raise ValueError(f"{name}: a contiguous array expected")
     return t.data_ptr()
 
 
 def _rows(t, name, heads, dim):
-    _is(t, name, "int32", 3)
-    if tuple(t.shape[1:]) != (heads, dim):
-        raise ValueError(f"{name}: [tokens][{heads}][{dim}] expected, got {tuple(t.shape)}")
-    if t.shape[0] == 0:
+    shape = t.shape
+    if len(shape) != 3 or _name(t.dtype) != "int32":
+        _is(t, name, "int32", 3)
+    n, h, d = shape
+    if h != heads or d != dim:
+        raise ValueError(f"{name}: [tokens][{heads}][{dim}] expected, got {tuple(shape)}")
+    if n == 0:
         return _Rows(t.data_ptr(), heads * dim, dim)
-    s = t.stride()
-    if dim > 1 and s[2] != 1 or min(s) < 0:
+    a, b, c = t.stride()
+    if c != 1 and dim > 1 or a < 0 or b < 0:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
-    return _Rows(t.data_ptr(), s[0] if t.shape[0] > 1 else max(s[0], dim), s[1] if heads > 1 else max(s[1], dim))
+    return _Rows(t.data_ptr(), a if n > 1 else max(a, dim), b if heads > 1 else max(b, dim))
 
 
 def _table(t):
@@ -87,7 +101,7 @@ class KVCache:
     def __init__(self, k, v):
         if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or str(k.dtype) != str(v.dtype):
             raise ValueError("KVCache: two arrays [n_blocks][n_kv_heads][block_size][head_dim] of one type expected")
-        bits = {"int32": 32, "int16": 16}.get(str(k.dtype).rpartition(".")[2])
+        bits = {"int32": 32, "int16": 16}.get(_name(k.dtype))
         if bits is None:
             raise ValueError(f"KVCache: int32 or int16 expected, got {k.dtype}")
         for t in (k, v):
