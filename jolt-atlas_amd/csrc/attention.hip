@@ -131,7 +131,8 @@ int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
         k_split_sums<<<WGS, 256, 0, stream>>>(A, L.S);
         k_split_values<CT, decltype(ks)::value, decltype(fast)::value><<<WGS, 256, 0, stream>>>(A, L.S);
     });
-    k_split_join<CT><<<L.S.n_rows, 256, 0, stream>>>(A, L.S, (uint32_t)padded_dim(A.d));
+    if (L.S.n_rows < 512) k_split_join<CT, 1024><<<L.S.n_rows, 1024, 0, stream>>>(A, L.S, (uint32_t)padded_dim(A.d));
+    else k_split_join<CT, 256><<<L.S.n_rows, 256, 0, stream>>>(A, L.S, (uint32_t)padded_dim(A.d));
     return ATLAS_OK;
 }
 
@@ -177,6 +178,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (!why) why = bad_rows(v, n_tokens, shape->n_kv_heads, shape->head_dim);
     if (!why) why = bad_rows(out, n_tokens, shape->n_heads, shape->head_dim);
     if (!why) why = bad_out(out, n_tokens, shape->n_heads, shape->head_dim);
+    if (!why && n_tokens && (out->d == q->d || out->d == k->d || out->d == v->d)) why = "attn_prompt: out may not be q, k or v";
     if (!why && !d_cu_seqlens) why = "attn_prompt: cu_seqlens is null";
     if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_attn_prompt_workspace(shape, n_seqs, n_tokens))) why = "attn_prompt: workspace is null, unaligned or too small";
     if (why) return fail(ATLAS_EINVAL, why);
@@ -211,6 +213,7 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (!why) why = bad_rows(out, n_tokens, shape->n_heads, shape->head_dim);
     if (!why) why = bad_out(out, n_tokens, shape->n_heads, shape->head_dim);
     if (!why) why = bad_cache(cache);
+    if (!why && n_tokens && out->d == q->d) why = "attn_cached: out may not be q";
     if (!why && (!d_cu_new || !d_kv_lens || !d_block_table)) why = "attn_cached: cu_new, kv_lens or block_table is null";
     if (!why && (max_blocks > 0x7fffffff / cache->block_size || table_stride < max_blocks || table_stride > 0x7fffffff)) why = "attn_cached: table_stride must be at least max_blocks, the keys of a row below 2^31";
     if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_attn_cached_workspace(shape, n_seqs, n_tokens, cache, max_blocks))) why = "attn_cached: workspace is null, unaligned or too small";

@@ -378,10 +378,16 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
 }
 
 // ---- longer contexts
-// One workgroup: the prefix sums of the tiles' units and rows
+// One workgroup: the prefix sums of the tiles' units and rows.  Offsets that do not ascend would count rows twice, more than the workspace has room for: then
+// there are none.
 __global__ __launch_bounds__(1024) void k_split_plan(Args A, Split S) {
-    __shared__ uint32_t s_u[16], s_r[16];
+    __shared__ uint32_t s_u[16], s_r[16], s_bad;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < A.n_seqs; i += 1024) if (A.cu[i] < 0 || A.cu[i + 1] < A.cu[i] || A.cu[i + 1] > (int64_t)A.n_tokens) s_bad = 1;
+    __syncthreads();
+    const bool bad = s_bad;
     uint32_t u0 = 0, r0 = 0;
     for (uint32_t i0 = 0; i0 < S.n_tiles; i0 += 1024) {
         const uint32_t i = i0 + tid;
@@ -392,7 +398,7 @@ __global__ __launch_bounds__(1024) void k_split_plan(Args A, Split S) {
             while (hi - lo > 1) { const uint32_t mid = (lo + hi) / 2; if (base(mid) <= i) lo = mid; else hi = mid; }
             const Seq s = seq_at(A, lo);
             const uint64_t b = base(lo), first = i >= b ? (i - b) * TILE_ROWS : ~0ull;
-            if (first < (uint64_t)s.n_new * A.G) { r = min(TILE_ROWS, s.n_new * A.G - (uint32_t)first); u = (s.keys + UNIT - 1) / UNIT; }
+            if (!bad && first < (uint64_t)s.n_new * A.G) { r = min(TILE_ROWS, s.n_new * A.G - (uint32_t)first); u = (s.keys + UNIT - 1) / UNIT; }
         }
         const uint32_t u_mine = u, r_mine = r;
 #pragma unroll
@@ -407,10 +413,12 @@ __global__ __launch_bounds__(1024) void k_split_plan(Args A, Split S) {
     }
     if (tid == 0) { S.units[S.n_tiles] = u0; S.rows[S.n_tiles] = r0; }
 }
-// The line's units over the workgroups: n of them have a share, the first `more` of them per + 1 units and the others per
+// The line's units over the workgroups: n of them have a share, the first `more` of them per + 1 units and the others per.  Half as many where a share would be
+// less than 4 units: two workgroups fit a CU (4 tokens over 65000 16-bit keys: the scores 49 -> 45, the values 46 -> 40 us; 64 over up to 8191 int32 ones, which
+// have more: the scores 162 -> 172, the sums 17 -> 26 us)
 struct Line {
     uint32_t n, per, more;
-    __device__ Line(const Args& A, const Split& S) { const uint32_t U = S.units[S.n_tiles] * A.KV; n = max(min(U, WGS), 1u); per = U / n; more = U % n; }
+    __device__ Line(const Args& A, const Split& S) { const uint32_t U = S.units[S.n_tiles] * A.KV; n = max(min(U, U >= 4 * WGS ? WGS : WGS / 2), 1u); per = U / n; more = U % n; }
     __device__ uint32_t begin(uint32_t w) const { return min(w, n) * per + min(w, more); }
     __device__ uint32_t owner(uint32_t u) const { const uint32_t x = more * (per + 1); return u < x ? u / (per + 1) : more + (u - x) / per; }
 };
@@ -580,9 +588,10 @@ __global__ __launch_bounds__(256, 2) void k_split_values(Args A, Split S) {
     }
 }
 
-// One workgroup per row: the shares' products added up, every dim by 256 / DP threads; where the operands did not fit the digits, the row again in 64 bits
-template <class CT>
-__global__ __launch_bounds__(256) void k_split_join(Args A, Split S, uint32_t dp) {
+// One workgroup per row: the shares' products added up, every dim by JOIN / DP threads; where the operands did not fit the digits, the row again in 64 bits.
+// JOIN: 1024 where the rows are few (128 rows: 40 -> 14 us), 256 where they fill the chip (2048 rows: 12 us, 25 with 1024)
+template <class CT, uint32_t JOIN>
+__global__ __launch_bounds__(JOIN) void k_split_join(Args A, Split S, uint32_t dp) {
     const uint32_t t = blockIdx.x / A.H, h = blockIdx.x % A.H, tid = threadIdx.x, kvh = h / A.G;
     const uint32_t si = find_seq(A.cu, A.n_seqs, t);
     if (si >= A.n_seqs) return;
@@ -590,19 +599,29 @@ __global__ __launch_bounds__(256) void k_split_join(Args A, Split S, uint32_t dp
     if (t < s.begin || t - s.begin >= s.n_new) return;
     const uint32_t row = (t - s.begin) * A.G + h % A.G, tile = (uint32_t)((uint64_t)s.begin * A.G / TILE_ROWS) + si + row / TILE_ROWS, r = row % TILE_ROWS;
     __shared__ uint32_t s_mag[3];
-    __shared__ int32_t s_q[256], s_p[256];
-    __shared__ uint64_t s_red[256];
+    __shared__ int32_t s_q[JOIN], s_p[JOIN];
+    __shared__ uint64_t s_red[JOIN];
     if (tid < 3) s_mag[tid] = 0;
     __syncthreads();
-    each_share(A, S, tile, kvh, tid, 256, [&](uint32_t, uint32_t mag) { atomicOr(&s_mag[0], S.q_mag[mag]); atomicOr(&s_mag[1], S.k_mag[mag]); atomicOr(&s_mag[2], S.v_mag[mag]); });
-    const uint32_t y = tid & (dp - 1), parts = 256 / dp;
+    const uint32_t per = S.units[tile + 1] - S.units[tile], n = S.rows[tile + 1] - S.rows[tile];
+    const uint32_t y = tid & (dp - 1), parts = JOIN / dp;
     int64_t sum = 0;
-    if (y < A.d) each_share(A, S, tile, kvh, tid / dp, parts, [&](uint32_t part, uint32_t) { sum += S.part[(int64_t)(part + r) * A.d + y]; });
+    if (per) {
+        const Line line(A, S);
+        const uint32_t p = S.units[tile] * A.KV + kvh * per, w0 = line.owner(p), w1 = line.owner(p + per - 1), mag = tile * A.KV + kvh;
+        uint32_t mq = 0, mk = 0, mv = 0;
+        for (uint32_t w = w0 + tid; w <= w1; w += JOIN) { mq |= S.q_mag[w + mag]; mk |= S.k_mag[w + mag]; mv |= S.v_mag[w + mag]; }
+        if (mq | mk | mv) { atomicOr(&s_mag[0], mq); atomicOr(&s_mag[1], mk); atomicOr(&s_mag[2], mv); }
+        const int64_t* from = S.part + (int64_t)(S.rows[tile] * A.KV + kvh * n + r) * A.d + y;
+        if (y < A.d)
+#pragma unroll 4
+            for (uint32_t w = w0 + tid / dp; w <= w1; w += parts) sum += from[(int64_t)w * TILE_ROWS * A.d];
+    }
     s_red[tid] = (uint64_t)sum;
     __syncthreads();
     const uint32_t mq = s_mag[0], mk = s_mag[1], mv = s_mag[2];
     if (((mq | mk | mv) & WIDE) || bits_of(mq) + bits_of(mk) + bits_of(A.d - 1) > SPLIT_BITS) {
-        row_exact<CT>(A, s, t - s.begin, h, s_q, s_p, s_red);
+        row_exact<CT, JOIN>(A, s, t - s.begin, h, s_q, s_p, s_red);
         return;
     }
     if (tid < A.d) {

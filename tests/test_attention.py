@@ -67,7 +67,7 @@ class Fake:
 
 def _prompt(**kw):
     import jolt_atlas_amd.attention as T
-    a = dict(heads=4, kv=2, dim=8, mul=1 << 14, q=Fake((5, 4, 8)), k=Fake((5, 2, 8)), v=Fake((5, 2, 8)), cu=Fake((3,)), out=Fake((5, 4, 8)), ws=Fake((1 << 22,), "uint8"))
+    a = dict(heads=4, kv=2, dim=8, mul=1 << 14, q=Fake((5, 4, 8)), k=Fake((5, 2, 8)), v=Fake((5, 2, 8)), cu=Fake((3,)), out=Fake((5, 4, 8), ptr=1 << 41), ws=Fake((1 << 22,), "uint8"))
     a.update(kw)
     at = T.Attention(a["heads"], a["kv"], a["dim"], a["mul"])
     at.prompt(a["q"], a["k"], a["v"], a["cu"], a["out"], a["ws"])
@@ -79,7 +79,7 @@ def _prompt(**kw):
     (dict(dim=257, q=Fake((5, 4, 257)), k=Fake((5, 2, 257)), v=Fake((5, 2, 257)), out=Fake((5, 4, 257))), "head_dim"),
     (dict(mul=0), "score_mul"), (dict(mul=(1 << 14) + 1), "score_mul"), (dict(mul=-5), "score_mul"),
     (dict(q=Fake((5, 4, 8), strides=(32, 4, 1))), "strides"),
-    (dict(out=Fake((5, 4, 8), strides=(8, 8, 1))), "overlap"),
+    (dict(out=Fake((5, 4, 8), strides=(8, 8, 1))), "overlap"), (dict(out=Fake((5, 4, 8))), "may not be"),
     (dict(out=Fake((5, 4, 8), strides=(0, 8, 1))), "strides"),
     (dict(q=Fake((5, 4, 8), ptr=(1 << 40) + 2)), "aligned"),
     (dict(ws=Fake((8,), "uint8")), "workspace"),
@@ -102,7 +102,7 @@ def test_prompt_refusals_of_the_wrapper(kw):
 
 def _cached(**kw):
     import jolt_atlas_amd.attention as T
-    a = dict(q=Fake((3, 4, 8)), cu=Fake((3,)), lens=Fake((2,)), ck=Fake((7, 2, 16, 8)), cv=Fake((7, 2, 16, 8)), table=Fake((2, 5)), out=Fake((3, 4, 8)), ws=Fake((1 << 22,), "uint8"))
+    a = dict(q=Fake((3, 4, 8)), cu=Fake((3,)), lens=Fake((2,)), ck=Fake((7, 2, 16, 8)), cv=Fake((7, 2, 16, 8)), table=Fake((2, 5)), out=Fake((3, 4, 8), ptr=1 << 41), ws=Fake((1 << 22,), "uint8"))
     a.update(kw)
     T.Attention(4, 2, 8).cached(a["q"], a["cu"], a["lens"], T.KVCache(a["ck"], a["cv"]), a["table"], a["out"], a["ws"])
 
@@ -114,6 +114,7 @@ def _cached(**kw):
     (dict(ck=Fake((7, 2, 16, 8), ptr=(1 << 40) + 2)), "alignment"),
     (dict(cv=Fake((7, 2, 16, 8), ptr=0)), "null"),
     (dict(lens=Fake((2,), ptr=0)), "null"),
+    (dict(out=Fake((3, 4, 8))), "may not be"),
     (dict(table=Fake((2, 1 << 28))), "table_stride"),
     (dict(ws=Fake((8,), "uint8")), "workspace"),
 ])

@@ -92,7 +92,7 @@ def test_prompt_without_rows_or_sequences(atlas):
     at.prompt(e(2), e(1), e(1), Dev(np.zeros(4, np.int32)), e(2), workspace(at.prompt_workspace_bytes(3, 0)))
     x = np.full((5, 2, 8), MARK, np.int32)
     out = Dev(x)
-    at.prompt(Dev(x), Dev(x[:, :1]), Dev(x[:, :1]), Dev(np.zeros(1, np.int32)), out, workspace(at.prompt_workspace_bytes(0, 5)))
+    at.prompt(Dev(x.copy()), Dev(x[:, :1]), Dev(x[:, :1]), Dev(np.zeros(1, np.int32)), out, workspace(at.prompt_workspace_bytes(0, 5)))
     assert (out.numpy() == MARK).all()
 
 
@@ -550,6 +550,90 @@ def test_a_serving_run(atlas):
     assert n_free.numpy()[0] == n_blocks - sum(-(-h // B) for h in have)
 
 
+@pytest.mark.parametrize("cu", [[0, 40, 10, 60], [50, 20, 60, 0], [-5, 30, 60, 60], [0, 70, 80, 90], [2 ** 31 - 1, -(2 ** 31), 2 ** 31 - 1, 0], [0, 60, 0, 60]])
+def test_offsets_that_make_no_sense_stay_inside(atlas, cu):
+    """offsets that do not ascend, or pass the arrays: whatever is computed, nothing is written outside of out's rows and the workspace"""
+    import jolt_atlas_amd.attention as T
+    rng = np.random.default_rng(2)
+    n, H, KV, d = 60, 4, 2, 64
+    at = T.Attention(H, KV, d, 2048)
+    big = Dev(np.full((n + 200, H, d), MARK, np.int32))
+    out = big.view(100 * H * d, (n, H, d), (H * d, d, 1))
+    q, k = Dev(values(rng, (n, H, d))), Dev(values(rng, (n, KV, d)))
+    c = Dev(np.array(cu, np.int32))
+
+    def guarded(size):
+        w = workspace(size + 8192)
+        return w, w.view(4096, (size,), (1,))
+
+    def intact(w, size):
+        x = w.numpy()
+        assert (x[:4096] == 0xA5).all() and (x[4096 + size:] == 0xA5).all()
+        y = big.numpy()
+        assert (y[:100] == MARK).all() and (y[100 + n:] == MARK).all()
+
+    size = at.prompt_workspace_bytes(3, n)
+    w, v = guarded(size)
+    at.prompt(q, k, k, c, out, v)
+    intact(w, size)
+    for rows, cols in ((n, 4), (n, 80), (n, 300)):
+        ck = values(rng, (6, KV, 16, d))
+        cache = T.KVCache(Dev(ck), Dev(ck))
+        table = Dev(rng.integers(-2, 8, size=(3, cols)).astype(np.int32))
+        size = at.cached_workspace_bytes(3, n, cache, cols)
+        w, v = guarded(size)
+        for lens in ([60, 60, 60], [cols * 16, -1, 2 ** 31 - 1]):
+            at.cached(q, c, Dev(np.array(lens, np.int32)), cache, table, out, v)
+            intact(w, size)
+
+
+@pytest.mark.parametrize("d", [32, 128])
+def test_every_kernel_captured(atlas, d):
+    """tiles, tiles of long sequences and the split path inside one graph, replayed over changed inputs"""
+    import jolt_atlas_amd.attention as T
+    h = hip()
+    rng = np.random.default_rng(d)
+    H, KV, n, B = 4, 2, 40, 16
+    at = T.Attention(H, KV, d, 2048)
+    st, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    ok(h.hipStreamCreateWithFlags(C.byref(st), C.c_uint(1)))
+    rows = 16500
+    q, k, v = (Dev(np.zeros((rows, x, d), np.int32)) for x in (H, KV, KV))
+    outs = [Dev(np.zeros((rows, H, d), np.int32)) for _ in range(4)]
+    cu = Dev(np.array([0, 25, n], np.int32))
+    ck, cv, table, flat = paged(rng, [70, 30], KV, d, B, 32)
+    cache, cq, one = T.KVCache(Dev(ck), Dev(cv)), Dev(np.zeros((2, H, d), np.int32)), Dev(np.array([0, 1, 2], np.int32))
+    lens, wide = Dev(np.array([70, 30], np.int32)), Dev(np.concatenate([table, np.full((2, 300), -1, np.int32)], axis=1))
+    calls = []
+    for x, m in zip(outs, (n, 2100, rows)):
+        cut = lambda y: y.view(0, (m,) + y.shape[1:], y.stride())  # noqa: E731
+        calls.append(lambda s, a=(cut(q), cut(k), cut(v), cu, cut(x), workspace(at.prompt_workspace_bytes(2, m))): at.prompt(*a, stream=s))
+    cout = outs[3].view(0, (2, H, d), (H * d, d, 1))
+    cws = workspace(at.cached_workspace_bytes(2, 2, cache, wide.shape[1]))
+    calls.append(lambda s: at.cached(cq, one, lens, cache, wide, cout, cws, stream=s))
+    ok(h.hipDeviceSynchronize())
+    ok(h.hipStreamBeginCapture(st, C.c_int(0)))
+    for f in calls:
+        f(st.value)
+    ok(h.hipStreamEndCapture(st, C.byref(graph)))
+    ok(h.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)))
+    for rep in range(3):
+        hq, hk, hv, hc = values(rng, (n, H, d)), values(rng, (n, KV, d)), values(rng, (n, KV, d)), values(rng, (2, H, d))
+        for dev, x in ((q, hq), (k, hk), (v, hv), (cq, hc)):
+            ok(h.hipMemcpy(dev.buf.p, np.ascontiguousarray(x).ctypes.data_as(C.c_void_p), C.c_size_t(x.nbytes), C.c_int(1)))
+        ok(h.hipDeviceSynchronize())
+        ok(h.hipGraphLaunch(exe, st))
+        ok(h.hipDeviceSynchronize())
+        want = prompt(hq, hk, hv, [25, 15], 2048)
+        for x in outs[:3]:
+            assert np.array_equal(x.numpy()[:n], want), rep
+        assert np.array_equal(cout.numpy(), want_cached(hc, ck, cv, table, flat, [70, 30], [1, 1], 2048)), rep
+        run_prompt(atlas, hq, hk, hv, [25, 15], 2048, pads=(2100,))          # eager work between the replays
+    ok(h.hipGraphExecDestroy(exe))
+    ok(h.hipGraphDestroy(graph))
+    ok(h.hipStreamDestroy(st))
+
+
 def test_pointers_that_are_no_device_memory(atlas):
     import jolt_atlas_amd.attention as T
     at = T.Attention(1, 1, 4)
@@ -557,7 +641,8 @@ def test_pointers_that_are_no_device_memory(atlas):
     host = np.zeros((2, 1, 4), np.int32)
     fake = Dev(np.empty(0, np.int32), x.buf, 0, (2, 1, 4), (4, 4, 1))
     fake.data_ptr = lambda: host.ctypes.data
-    for a in ((fake, x, x, x), (x, fake, x, x), (x, x, fake, x), (x, x, x, fake)):
+    y = Dev(host)
+    for a in ((fake, x, x, y), (x, fake, x, y), (x, x, fake, y), (x, x, x, fake)):
         with pytest.raises(atlas.AtlasError, match="device"):
             at.prompt(a[0], a[1], a[2], Dev(np.array([0, 2], np.int32)), a[3], workspace(at.prompt_workspace_bytes(1, 2)))
 
