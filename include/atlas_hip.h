@@ -861,12 +861,14 @@ int atlas_verify_graph(atlas_graph_t g, const atlas_hyperkzg_vk_t *vk, const int
  *     e = (HI[z >> 9] LO[z & 511]) >> 14;  w = 2^28 / sum_j e;  p = (e w) >> 14;  out = clamp((sum_j p v) >> 14)
  * with the digit tables of SoftmaxLastAxis (atlas-onnx-tracer/src/ops/softmax.rs:74-269), floor shifts and clamps to 32 bits
  * (ops/einsum.rs:34-213).  Masked keys carry no weight (a graph whose mask fill lies 2^18 or more below every row's maximum); a row that
- * sees no key is 0.  Any int32 value is computed exactly (sums wrap modulo 2^64, as the graph's do); operands below 2^19 in magnitude take the fast path.
+ * sees no key is 0.  Any int32 value is computed exactly (sums wrap modulo 2^64, as the graph's do); operands in [-8421504, 8355711]
+ * with |q| |k| head_dim < 2^44 take the matrix cores (trained models stay far below: 2^18 is 16.0), rows beyond that a 64-bit path that is ~100 times slower.
  *
  * These entry points enqueue and return: no allocation, no wait, no state between calls, so they can be captured into HIP graphs.  `stream` is the
  * caller's hipStream_t; NULL = the library stream, ATLAS_STREAM_DEFAULT = HIP's default stream.  Lengths, tables and slots are read on the
  * device when the launches run.  All pointers are device memory of the calling thread's device (atlas_init / atlas_init_thread).  A workspace
- * (16-byte aligned) belongs to one call in flight: two streams, or two captured graphs that may run at once, need one each. */
+ * (16-byte aligned) belongs to one call in flight: two streams, or two captured graphs that may run at once, need one each.  Its size goes by the
+ * arguments, not by the lengths on the device: a table of many columns costs atlas_attn_cached the room for max_blocks * block_size keys a sequence. */
 #define ATLAS_STREAM_DEFAULT ((void *)1)
 typedef struct {
     size_t n_heads, n_kv_heads;   /* head h reads the keys and values of head h / (n_heads / n_kv_heads); at most 1024 heads */
