@@ -21,7 +21,6 @@ Args args_of(const atlas_attn_shape_t* s, const atlas_attn_rows_t* q, const int3
     return A;
 }
 
-
 // head sizes are padded to the fragments of the tile kernel
 int padded_dim(size_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 // f(padded dims, waves to a row)

@@ -2,8 +2,8 @@
 // query rows (k_attn_tile).
 //
 // An int32 operand in [-8421504, 8355711] is d0 + 2^8 d1 + 2^16 d2 with signed bytes d: the bytes of v + 0x808080, each less 128.  A product of two
-// such operands is nine i8 products in five weights, exact in the 32-bit accumulators of v_mfma_i32_32x32x32_i8: 9 x 2 d / 5 POP/s per score against a 64-bit
-// multiply-add per element on the vector unit.  The five sums recombine without 64-bit arithmetic: with hi = a2 + 2^8 a3 + 2^16 a4 and lo = a0 + 2^8 a1,
+// such operands is nine i8 products in five weights, exact in the 32-bit accumulators of v_mfma_i32_32x32x32_i8; on the vector
+// unit it is a 64-bit multiply-add per element (the first kernel: 206 ms where this one takes 1.87).  The five sums recombine without 64-bit arithmetic: with hi = a2 + 2^8 a3 + 2^16 a4 and lo = a0 + 2^8 a1,
 //     floor((2^16 hi + lo) / 2^14) = 4 hi + (lo >> 14),
 // and hi may wrap, as long as the score itself fits 32 bits: |q| |k| d < 2^45, decided per tile from the operands' magnitudes.  Tiles that do not
 // qualify (and operands beyond three bytes) are computed row by row in 64 bits (row_exact).
@@ -12,6 +12,15 @@
 // follow each other there are four bytes of the operand of O^T = V^T P^T (the keys of V's fragments are laid out in that order).  The weights
 // 0 .. 2^14 are two signed bytes; of the second, most tiles have none (p < 128) and skip it.  sum_j p <= 2^14, so an output accumulator stays below
 // 2^21 however many keys there are.
+//
+// Three passes over the scores, since the floors are taken under the final maximum and sum: maximum; e and its sum (e is held in 16 bits while the keys are few enough, HELD, or
+// taken again); product.  Bound by the vector unit, that is by recombining five sums into each score and by the two table look-ups: per step of 64 keys and 64 rows of 128 dims two
+// workgroups on a CU take 4.1, 5.9 and 3.4 thousand cycles in the passes, the vector unit busy for 51-57 % of them and the matrix cores for 38 %.  Six prompts of up to 6000 tokens,
+// 32 heads of 128 over 8 (295 GFLOP of exact products, 24 i8 products for two of them): 1.87 ms, 158 TFLOP/s, 1.7-1.9 POP/s in int8, where a library's int8 product of
+// 8192^3 reaches 2.2.  130 new tokens for each of some of 12 sequences over up to 5001 keys (186 MB, 24 GFLOP): 562 us, 70 of them the digit planes (k_attn_planes, 4.6 TB/s read and
+// written); the rest is the longest sequence's tile, three passes one after the other.
+// Measured and dropped: 3 waves per SIMD (168 registers: spills, 2.6 ms), a raised wave priority around the products (none), the look-ups of 16 scores read together before
+// the first product (spills, 2 % slower).
 #pragma once
 #include "attention_kernels.hip.h"
 
