@@ -260,6 +260,28 @@ def test_cached_pages_that_do_not_exist(atlas):
         assert (run_cached(q, ck, cv, table, [-5, 0, -(2 ** 31), 0], new, 2896) == 0).all()
 
 
+@pytest.mark.parametrize("d", [32, 36, 64, 128, 256])
+@pytest.mark.parametrize("new", [[1, 1, 1], [60, 90, 33]])
+def test_cached_pages_that_do_not_exist_and_a_first_block_of_extremes(atlas, d, new):
+    """whatever is read in the place of a page that is missing does not count: the cache's first block holds the largest operands, and no sequence has it"""
+    rng = np.random.default_rng(d)
+    keys = [150, 97, 33]
+    ck, cv, table, flat = paged(rng, keys, 2, d, 16, 32)
+    table = np.where(table >= 0, table + 1, -1).astype(np.int32)
+    ends = np.array([-(1 << 31), (1 << 31) - 1], np.int32)
+    first = lambda c: np.concatenate([rng.choice(ends, size=c[:1].shape).astype(np.int32), c])  # noqa: E731
+    small = [ck, cv]
+    ck, cv = first(ck), first(cv)
+    table[0, 3], table[1, 0], table[2, 1] = -1, len(ck), -(1 << 31)
+    q, want, at = values(rng, (sum(new), 8, d)), np.zeros((sum(new), 8, d), np.int32), 0
+    for i, (m, n) in enumerate(zip(keys, new)):
+        there = np.repeat((table[i] >= 0) & (table[i] < len(ck)), 16)[:m]
+        lim = [there & (np.arange(m) < m - n + j + 1) for j in range(n)]
+        want[at:at + n] = attend(q[at:at + n], flat(small[0], i), flat(small[1], i), lim, 1448)
+        at += n
+    assert np.array_equal(run_cached(q, ck, cv, table, keys, new, 1448), want)
+
+
 def test_cached_of_any_int32(atlas):
     rng = np.random.default_rng(5)
     for new in ([1, 1], [40, 3]):
