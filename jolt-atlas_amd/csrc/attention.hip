@@ -55,7 +55,7 @@ struct PlanesLayout {
         held = std::min<size_t>((max_keys + 127) / 128 * 128, HELD);
         work = (n_tokens * G / rows + n_seqs) * s->n_kv_heads;
         wgs = std::min<size_t>(work, TILE_WGS);
-        const size_t one = tiles * s->n_kv_heads * (size_t)(dp / 32 * 3072);
+        const size_t one = tiles * s->n_kv_heads * (size_t)(dp / 32) * FRAGMENT;
         v_at = one;
         mag_at = 2 * one;
         there_at = mag_at + 8 * tiles * s->n_kv_heads;

@@ -31,6 +31,7 @@ typedef int v16i __attribute__((ext_vector_type(16)));
 typedef int32_t i32x4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef int16_t i16x4 __attribute__((ext_vector_type(4), aligned(2)));
 
+constexpr uint32_t FRAGMENT = 3 * 1024;            // bytes of 32 x 32 operands: three planes
 constexpr uint32_t WIDE = 0x80000000u;             // in a magnitude word: an operand beyond three signed bytes
 
 // the extremes of the operands seen
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
         const Rows& r = value ? A.v : A.k;
         return (const CT*)r.d + (int64_t)(s.begin + j) * r.ts + (int64_t)kvh * r.hs;
     };
-    const int64_t at = ((int64_t)kvh * P.tiles + tile) * (F * 3 * 1024);
+    const int64_t at = ((int64_t)kvh * P.tiles + tile) * (F * FRAGMENT);
     Range rk, rv;
     const uint32_t jk = min(j0 + l32, s.keys - 1);
     const int64_t mine = A.table ? block_of(A, s, jk) : 0;
@@ -156,13 +157,13 @@ __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
             zero_behind(f * 32 + half * 16, A.d, e);
 #pragma unroll
             for (int c = 0; c < 4; c++) { int a, b, g; digits4(e[c][0], e[c][1], e[c][2], e[c][3], a, b, g, rk); p0[c] = a; p1[c] = b; p2[c] = g; }
-            v4i* to = (v4i*)(P.k + at + f * 3072) + lane;
+            v4i* to = (v4i*)(P.k + at + f * (int)FRAGMENT) + lane;
             to[0] = p0; to[64] = p1; to[128] = p2;
         }
         if (vs) {
 #pragma unroll
             for (int c = 0; c < 4; c++) { int a, b, g; digits4(v[c][0], v[c][1], v[c][2], v[c][3], a, b, g, rv); p0[c] = a; p1[c] = b; p2[c] = g; }
-            v4i* to = (v4i*)(P.v + at + f * 3072) + lane;
+            v4i* to = (v4i*)(P.v + at + f * (int)FRAGMENT) + lane;
             to[0] = p0; to[64] = p1; to[128] = p2;
         }
     }
@@ -212,7 +213,7 @@ struct TileShape {
     static constexpr int SUBS = SPLIT < 2 ? 2 : SPLIT;        // key sub-tiles of 32 per step
     static constexpr int KEYS = 32 * SUBS, MY_SUBS = SUBS / SPLIT;
     static constexpr int OF = F / SPLIT;                      // output fragments of a wave
-    static constexpr uint32_t TILE = F * 3072, STEP = TILE * SUBS;
+    static constexpr uint32_t TILE = F * FRAGMENT, STEP = TILE * SUBS;
     static constexpr int BUFS = DP == 256 ? 1 : 3;            // two steps are on their way while one is worked on; of 256 dims 160 KB of LDS hold one step
     static constexpr int COPIES = STEP / 4096;                // that a wave has issued for a step, at least
     static constexpr uint32_t LUT = 4096, LDS = LUT + STEP * BUFS + 1024;
@@ -469,7 +470,7 @@ __global__ __launch_bounds__(256, (TileShape<DP, SPLIT>::WAVES)) void k_attn_til
 #pragma unroll
                     for (int f = 0; f < T::OF; f++)
 #pragma unroll
-                        for (int p = 0; p < 3; p++) v[sub][f][p] = ((const v4i*)(buf + sub * T::TILE + (part * T::OF + f) * 3072) + lane)[p * 64];
+                        for (int p = 0; p < 3; p++) v[sub][f][p] = ((const v4i*)(buf + sub * T::TILE + (part * T::OF + f) * (int)FRAGMENT) + lane)[p * 64];
                 if (step + 1 < to) load_e(step + 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
