@@ -5,8 +5,8 @@
 // such operands is nine i8 products in five weights, exact in the 32-bit accumulators of v_mfma_i32_32x32x32_i8; on the vector
 // unit it is a 64-bit multiply-add per element (the first kernel: 206 ms where this one takes 1.87).  The five sums recombine without 64-bit arithmetic: with hi = a2 + 2^8 a3 + 2^16 a4 and lo = a0 + 2^8 a1,
 //     floor((2^16 hi + lo) / 2^14) = 4 hi + (lo >> 14),
-// and hi may wrap, as long as the score itself fits 32 bits: |q| |k| d < 2^45, decided per tile from the operands' magnitudes.  Tiles that do not
-// qualify (and operands beyond three bytes) are computed row by row in 64 bits (row_exact).
+// and hi may wrap, as long as the score itself fits 32 bits: |q| |k| d < 2^45, decided per tile from the operands' magnitudes (at 2^45, which only two
+// negative powers of two reach, the score is 2^31 and clamps).  Tiles that do not qualify (and operands beyond three bytes) are computed row by row in 64 bits (row_exact).
 //
 // The products are taken as S^T = K Q^T, so a lane holds 16 scores of ONE query row: maximum, sum and weights stay in registers, and four weights that
 // follow each other there are four bytes of the operand of O^T = V^T P^T (the keys of V's fragments are laid out in that order).  The weights
@@ -33,12 +33,15 @@ typedef int16_t i16x4 __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr uint32_t FRAGMENT = 3 * 1024;            // bytes of 32 x 32 operands: three planes
 constexpr uint32_t WIDE = 0x80000000u;             // in a magnitude word: an operand beyond three signed bytes
+constexpr uint32_t LOWEST = 0x40000000u;           // an operand may be -2^n, n the word's bits; all others are below 2^n
 
 // the extremes of the operands seen
 struct Range {
     int32_t hi = 0, lo = 0;
-    // bits of the largest magnitude as a mask, WIDE where three signed bytes do not hold an operand
+    // bits of the largest magnitude as a mask (-2^n counts n bits), WIDE where three signed bytes do not hold an operand
     __device__ uint32_t word() const { return (uint32_t)hi | (uint32_t)(lo ^ (lo >> 31)) | (hi > 8355711 || lo < -8421504 ? WIDE : 0); }
+    // LOWEST where the least operand is -2^m: of the words that are joined, the one with the joint n among them says so
+    __device__ uint32_t lowest() const { return lo < 0 && (lo & (0u - (uint32_t)lo)) == 0u - (uint32_t)lo ? LOWEST : 0; }
 };
 // four operands that follow each other along the product's inner dimension -> a dword of each digit plane.  The extremes are taken at once (the empty asm):
 // left to itself the compiler keeps every operand to do it later, and spills.
@@ -167,13 +170,13 @@ __global__ __launch_bounds__(256) void k_attn_planes(Args A, Planes P) {
             to[0] = p0; to[64] = p1; to[128] = p2;
         }
     }
-    atomicOr(&s_mag[0], rk.word());
+    atomicOr(&s_mag[0], rk.word() | rk.lowest());
     atomicOr(&s_mag[1], rv.word());
     __syncthreads();
     if (threadIdx.x == 0) { P.k_mag[(size_t)kvh * P.tiles + tile] = s_mag[0]; P.v_mag[(size_t)kvh * P.tiles + tile] = s_mag[1]; }
 }
 
-__device__ inline uint32_t bits_of(uint32_t mag) { return mag ? 32 - __builtin_clz(mag) : 0; }
+__device__ inline uint32_t bits_of(uint32_t mag) { mag &= ~LOWEST; return mag ? 32 - __builtin_clz(mag) : 0; }
 
 // 16 bytes per lane from global memory to LDS without a register on the way; lds: the wave's first byte
 __device__ inline void copy_to_lds(const uint8_t* src, uint8_t* lds, uint32_t bytes, uint32_t wave, uint32_t lane) {
@@ -298,14 +301,15 @@ __global__ __launch_bounds__(256, (TileShape<DP, SPLIT>::WAVES)) void k_attn_til
                 hole |= ~P.there[base + i] & (n < 32 ? (1u << n) - 1 : ~0u);
             }
             if (hole) s_red[4] = 1;
-            atomicOr(&s_red[0], rq.word());
+            atomicOr(&s_red[0], rq.word() | rq.lowest());
             if (mk) atomicOr(&s_red[1], mk);
             if (mv) atomicOr(&s_red[2], mv);
             __syncthreads();
             mq = s_red[0]; mk = s_red[1]; mv = s_red[2];
             holes = s_red[4];
             __syncthreads();
-            if (((mq | mk | mv) & WIDE) || bits_of(mq) + bits_of(mk) + bits_of(A.d - 1) > 45) {
+            const uint32_t most_bits = mq & mk & LOWEST ? 44 : 45;         // |q| |k| d may BE 2^45 where both have their lowest
+            if (((mq | mk | mv) & WIDE) || bits_of(mq) + bits_of(mk) + bits_of(A.d - 1) > most_bits) {
                 int32_t* x_q = (int32_t*)s_a;                          // 1 KB, 1 KB, 2 KB of the tile buffer
                 for (uint32_t x = 0; x < rows; x++) row_exact<CT>(A, s, (row0 + x) / A.G, kvh * A.G + (row0 + x) % A.G, x_q, x_q + 256, (uint64_t*)(x_q + 512));
                 continue;

@@ -119,6 +119,32 @@ def test_prompt_of_any_int32(atlas, H, KV, d, n, kind):
         assert np.array_equal(run_prompt(atlas, q, k, v, [n], mul), prompt(q, k, v, [n], mul))
 
 
+# |q| |k| d = 2^45: the score is 2^31, one more than 32 bits hold, and the definition clamps it
+BORDER = [(1, 23, 22), (16, 21, 20), (32, 20, 20), (64, 22, 17), (64, 23, 16), (64, 19, 20), (128, 23, 15), (256, 20, 17)]
+
+
+@pytest.mark.parametrize("d,a,b", BORDER)
+def test_prompt_scores_of_2_to_31(atlas, d, a, b):
+    rng = np.random.default_rng(d)
+    n = 70
+    q, k, v = np.full((n, 2, d), -(1 << a), np.int32), np.zeros((n, 1, d), np.int32), values(rng, (n, 1, d))
+    k[5], k[40] = -(1 << b), (1 << b) - 1                # one key at the border, one as far below
+    assert int(q[0, 0].astype(np.int64) @ k[5, 0]) == 1 << 45
+    for mul in (ONE, 1448):
+        assert np.array_equal(run_prompt(atlas, q, k, v, [n], mul), prompt(q, k, v, [n], mul))
+
+
+@pytest.mark.parametrize("d,a,b", BORDER)
+@pytest.mark.parametrize("new", [1, 70])
+def test_cached_scores_of_2_to_31(atlas, d, a, b, new):
+    rng = np.random.default_rng(d)
+    ck, cv, table, flat = paged(rng, [100], 1, d, 16, 32)
+    ck[:] = 0
+    ck[table[0, 0], 0, 3], ck[table[0, 1], 0, 2] = -(1 << b), (1 << b) - 1
+    q = np.full((new, 2, d), -(1 << a), np.int32)
+    assert np.array_equal(run_cached(q, ck, cv, table, [100], [new], 2048), want_cached(q, ck, cv, table, flat, [100], [new], 2048))
+
+
 def test_prompt_scores_that_are_equal_or_far_apart(atlas):
     rng = np.random.default_rng(9)
     n, d = 257, 64
