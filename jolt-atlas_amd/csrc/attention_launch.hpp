@@ -56,6 +56,7 @@ struct Launch {
         if (dev != rt().device) { HIP_TRY(hipSetDevice(rt().device)); back = dev; }
         if (!user) { lk = std::unique_lock<atlas_rt::Mutex>(rt().mu); stream = rt().stream; }
         else stream = user == ATLAS_STREAM_DEFAULT ? nullptr : (hipStream_t)user;
+        (void)hipGetLastError();          // of an earlier call of the caller's: end() is to tell of these launches
         return ATLAS_OK;
     }
     // every pointer must be memory of the runtime's device (managed and pinned host memory that the device maps is refused too: the kernels are

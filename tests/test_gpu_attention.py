@@ -781,3 +781,23 @@ def test_calls_of_two_threads(atlas):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not wrong
+
+
+def test_an_error_that_the_caller_left(atlas):
+    """an earlier HIP call of the caller's failed: that is not the attention's error"""
+    import jolt_atlas_amd.attention as T
+    h, rng = hip(), np.random.default_rng(3)
+    at, pager = T.Attention(1, 1, 8), T.Pager(4, 8)
+    q, k, v = (values(rng, (5, 1, 8)) for _ in range(3))
+    dev, out, cu, ws = [Dev(x) for x in (q, k, v)], Dev(np.zeros((5, 1, 8), np.int32)), Dev(np.array([0, 5], np.int32)), workspace(at.prompt_workspace_bytes(1, 5))
+    i32 = lambda *x: Dev(np.array(x, np.int32))  # noqa: E731
+    cache, ck, slots = T.KVCache(Dev(np.zeros((8, 1, 4, 8), np.int32)), Dev(np.zeros((8, 1, 4, 8), np.int32))), Dev(np.zeros((5, 1, 8), np.int32)), Dev(np.zeros(5, np.int64))
+    have, new, table, free, n_free, lens, status = i32(0), i32(5), i32(0, 0).view(0, (1, 2), (2, 1)), i32(*range(8)), i32(8), i32(0), i32(7)
+    wp, wc, pcu = workspace(pager.workspace_bytes(1, 5)), workspace(at.cached_workspace_bytes(1, 5, cache, 2)), i32(0, 0)
+    calls = [lambda: at.prompt(*dev, cu, out, ws), lambda: pager.plan(have, new, table, free, n_free, n_free, pcu, lens, slots, None, status, wp),
+             lambda: cache.write(dev[1], dev[2], slots), lambda: at.cached(dev[0], pcu, lens, cache, table, ck, wc)]
+    for f in calls:
+        assert h.hipSetDevice(C.c_int(4096)) != 0
+        f()
+    want = prompt(q, k, v, [5])
+    assert status.numpy()[0] == 0 and np.array_equal(out.numpy(), want) and np.array_equal(ck.numpy(), want)
