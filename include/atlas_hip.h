@@ -871,7 +871,7 @@ int atlas_verify_graph(atlas_graph_t g, const atlas_hyperkzg_vk_t *vk, const int
  * arguments, not by the lengths on the device: a table of many columns costs atlas_attn_cached the room for max_blocks * block_size keys a sequence. */
 #define ATLAS_STREAM_DEFAULT ((void *)1)
 typedef struct {
-    size_t n_heads, n_kv_heads;   /* head h reads the keys and values of head h / (n_heads / n_kv_heads); at most 1024 heads */
+    size_t n_heads, n_kv_heads;   /* head h reads the keys and values of head h / (n_heads / n_kv_heads); at most 1024 heads, n_tokens * n_heads / n_kv_heads at most 2^32 - 256 */
     size_t head_dim;              /* 1 .. 256 */
     int32_t score_mul;            /* the Mul node's constant at scale 2^14, 1 .. 2^14 (2^14: no scaling; 2^14 / sqrt(head_dim) rounded: the usual) */
     int32_t causal;               /* 1: a token sees the keys up to its own; 0: all keys of its sequence */

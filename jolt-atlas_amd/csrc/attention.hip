@@ -163,7 +163,7 @@ int launch_fused(const Args& A, size_t max_keys, hipStream_t stream) {
 extern "C" {
 
 size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens) {
-    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens)) return 0;
+    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_count(shape, n_tokens)) return 0;
     return fused(shape, n_seqs, n_tokens, n_tokens, true) ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
 }
 
@@ -172,6 +172,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
                       void* stream) {
     const char* why = bad_shape(shape);
     if (!why) why = bad_sizes(n_seqs, n_tokens);
+    if (!why) why = bad_count(shape, n_tokens);
     if (!why) why = bad_rows(q, n_tokens, shape->n_heads, shape->head_dim);
     if (!why) why = bad_rows(k, n_tokens, shape->n_kv_heads, shape->head_dim);
     if (!why) why = bad_rows(v, n_tokens, shape->n_kv_heads, shape->head_dim);
@@ -197,7 +198,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
 }
 
 size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
-    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
+    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_count(shape, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
     if (fused(shape, n_seqs, n_tokens, max_blocks * cache->block_size, many_rows(shape, n_seqs, n_tokens))) return 16;
     return many_rows(shape, n_seqs, n_tokens) ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_blocks * cache->block_size, 1)).bytes
                                        : SplitLayout(shape, n_seqs, n_tokens, max_blocks * cache->block_size, nullptr).bytes;
@@ -208,6 +209,7 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
                       void* d_workspace, size_t workspace_bytes, void* stream) {
     const char* why = bad_shape(shape);
     if (!why) why = bad_sizes(n_seqs, n_tokens);
+    if (!why) why = bad_count(shape, n_tokens);
     if (!why) why = bad_rows(q, n_tokens, shape->n_heads, shape->head_dim);
     if (!why) why = bad_rows(out, n_tokens, shape->n_heads, shape->head_dim);
     if (!why) why = bad_out(out, n_tokens, shape->n_heads, shape->head_dim);

@@ -77,5 +77,9 @@ struct Launch {
 inline const char* bad_sizes(size_t n_seqs, size_t n_tokens) {
     return n_seqs > MAX_SEQS ? "attention: more than 2^24 sequences" : n_tokens > MAX_TOKENS ? "attention: more than 2^30 tokens" : nullptr;
 }
+// the query rows of a sequence under one kv head are counted in 32 bits, and so are the up to 255 places of a tile behind its last one
+inline const char* bad_count(const atlas_attn_shape_t* s, size_t n_tokens) {
+    return n_tokens * (s->n_heads / s->n_kv_heads) > 0xffffff00 ? "attention: more than 2^32 - 256 query rows to a kv head" : nullptr;
+}
 
 }  // namespace atlas_attn

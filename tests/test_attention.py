@@ -179,3 +179,20 @@ def test_workspace_sizes():
         with pytest.raises(A.AtlasError):
             bad()
     assert A.lib.atlas_attn_prompt_workspace(C.POINTER(T._Shape)(), 1, 1) == 0
+
+
+@pytest.mark.parametrize("n", [1 << 22, (1 << 22) + 5, 1 << 30])
+def test_query_rows_past_32_bits_are_refused(n):
+    """1024 heads over one kv head: the rows of a sequence are counted in 32 bits"""
+    import jolt_atlas_amd as A
+    import jolt_atlas_amd.attention as T
+    ws, out = Fake((1 << 50,), "uint8"), Fake((n, 1024, 1), ptr=1 << 41)
+    with pytest.raises(A.AtlasError, match="query rows"):
+        _prompt(heads=1024, kv=1, dim=1, q=Fake((n, 1024, 1)), k=Fake((n, 1, 1)), v=Fake((n, 1, 1)), out=out, ws=ws)
+    at, cache = T.Attention(1024, 1, 1, causal=False), T.KVCache(Fake((7, 1, 16, 1)), Fake((7, 1, 16, 1)))
+    with pytest.raises(A.AtlasError, match="query rows"):
+        at.cached(Fake((n, 1024, 1)), Fake((2,)), Fake((1,)), cache, Fake((1, 1)), out, ws)
+    for f in (lambda: at.prompt_workspace_bytes(1, n), lambda: at.cached_workspace_bytes(1, n, cache, 1)):
+        with pytest.raises(A.AtlasError):
+            f()
+    assert at.prompt_workspace_bytes(1, (1 << 22) - 1) > 0
