@@ -70,7 +70,6 @@ struct PlanesLayout {
 };
 template <class CT>
 int launch_tiles(const Args& A, const PlanesLayout& L, const Planes& P, hipStream_t stream) {
-    if (L.work > 0x7fffffff || L.tiles > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows for one call");
     return with_shape(padded_dim(A.d), L.few, [&](auto dim, auto split) -> int {
         constexpr int DP = decltype(dim)::value, SPLIT = decltype(split)::value;
         using T = TileShape<DP, SPLIT>;
@@ -121,9 +120,6 @@ void with_steps(const Args& A, F f) {
 }
 template <class CT>
 int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
-    // rows, parts, magnitudes and units are counted in 32 bits
-    const uint64_t tiles = (uint64_t)A.n_tokens * A.G / TILE_ROWS + A.n_seqs, units = ((uint64_t)A.max_keys + UNIT - 1) / UNIT;
-    if ((uint64_t)A.n_tokens * A.H > 0x40000000 || tiles * A.KV > 0x40000000 || tiles * A.KV * units > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows and keys for one call");
     k_split_plan<<<1, 1024, 0, stream>>>(A, L.S);
     with_steps<CT>(A, [&](auto ks, auto fast) {
         k_split_scores<CT, decltype(ks)::value, decltype(fast)::value><<<WGS, 256, 0, stream>>>(A, L.S);
@@ -143,10 +139,27 @@ bool fused(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t m
     if (max_keys > fused_keys(s->head_dim)) return false;
     return many ? wgs <= 640 : max_keys <= 1024 || wgs >= 256;
 }
+enum class Path { FUSED, TILES, SPLIT };
+Path path_of(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys, bool many) {
+    return fused(s, n_seqs, n_tokens, max_keys, many) ? Path::FUSED : many ? Path::TILES : Path::SPLIT;
+}
+// What a path's launches and 32-bit counters hold: a launch has fewer than 2^32 threads
+const char* too_many(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys, bool cached, Path path) {
+    const size_t row_tiles = n_tokens * (s->n_heads / s->n_kv_heads) / TILE_ROWS + n_seqs, launch = 0xffffffff;
+    bool over;
+    if (path == Path::FUSED) over = row_tiles * s->n_kv_heads > launch / (FUSED_WAVES * 64);
+    else if (path == Path::TILES) {
+        const PlanesLayout L(s, n_seqs, n_tokens, cached ? std::max<size_t>(max_keys, 1) : 0);
+        over = L.work > 0x7fffffff || L.tiles > launch / 256;
+    } else {
+        const size_t units = (max_keys + UNIT - 1) / UNIT;
+        over = n_tokens * s->n_heads > launch / 256 || row_tiles * s->n_kv_heads > 0x40000000 || row_tiles * s->n_kv_heads * units > 0x7fffffff;
+    }
+    return over ? "attention: too many sequences, rows or keys for one call" : nullptr;
+}
 template <class CT>
 int launch_fused(const Args& A, size_t max_keys, hipStream_t stream) {
     const uint64_t wgs = ((uint64_t)A.n_tokens * A.G / TILE_ROWS + A.n_seqs) * A.KV;
-    if (wgs > 0x7fffffff) return fail(ATLAS_EINVAL, "attention: too many rows for one call");
     int rc = ATLAS_OK;
     with_steps<CT>(A, [&](auto ks, auto fast) {
         constexpr int KS = decltype(ks)::value;
@@ -164,7 +177,9 @@ extern "C" {
 
 size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_count(shape, n_tokens)) return 0;
-    return fused(shape, n_seqs, n_tokens, n_tokens, true) ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
+    const Path path = path_of(shape, n_seqs, n_tokens, n_tokens, true);
+    if (too_many(shape, n_seqs, n_tokens, n_tokens, false, path)) return 0;
+    return path == Path::FUSED ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
 }
 
 int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
@@ -180,6 +195,8 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (!why) why = bad_out(out, n_tokens, shape->n_heads, shape->head_dim);
     if (!why && n_tokens && (out->d == q->d || out->d == k->d || out->d == v->d)) why = "attn_prompt: out may not be q, k or v";
     if (!why && !d_cu_seqlens) why = "attn_prompt: cu_seqlens is null";
+    const Path path = why ? Path::FUSED : path_of(shape, n_seqs, n_tokens, n_tokens, true);
+    if (!why) why = too_many(shape, n_seqs, n_tokens, n_tokens, false, path);
     if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_attn_prompt_workspace(shape, n_seqs, n_tokens))) why = "attn_prompt: workspace is null, unaligned or too small";
     if (why) return fail(ATLAS_EINVAL, why);
     if (!n_seqs || !n_tokens) return ATLAS_OK;
@@ -188,7 +205,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (int rc = L.on_device({q->d, k->d, v->d, d_cu_seqlens, out->d, d_workspace})) return rc;
     Args A = args_of(shape, q, d_cu_seqlens, n_seqs, n_tokens, out);
     A.k = rows_of(k); A.v = rows_of(v);
-    if (fused(shape, n_seqs, n_tokens, n_tokens, true)) {
+    if (path == Path::FUSED) {
         if (int rc = launch_fused<int32_t>(A, n_tokens, L.stream)) return rc;
         return L.end();
     }
@@ -199,9 +216,11 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
 
 size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
     if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_count(shape, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
-    if (fused(shape, n_seqs, n_tokens, max_blocks * cache->block_size, many_rows(shape, n_seqs, n_tokens))) return 16;
-    return many_rows(shape, n_seqs, n_tokens) ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_blocks * cache->block_size, 1)).bytes
-                                       : SplitLayout(shape, n_seqs, n_tokens, max_blocks * cache->block_size, nullptr).bytes;
+    const size_t max_keys = max_blocks * cache->block_size;
+    const Path path = path_of(shape, n_seqs, n_tokens, max_keys, many_rows(shape, n_seqs, n_tokens));
+    if (too_many(shape, n_seqs, n_tokens, max_keys, true, path)) return 0;
+    if (path == Path::FUSED) return 16;
+    return path == Path::TILES ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_keys, 1)).bytes : SplitLayout(shape, n_seqs, n_tokens, max_keys, nullptr).bytes;
 }
 
 int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const int32_t* d_cu_new, const int32_t* d_kv_lens, size_t n_seqs, size_t n_tokens,
@@ -217,6 +236,8 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (!why && n_tokens && out->d == q->d) why = "attn_cached: out may not be q";
     if (!why && (!d_cu_new || !d_kv_lens || !d_block_table)) why = "attn_cached: cu_new, kv_lens or block_table is null";
     if (!why && (max_blocks > 0x7fffffff / cache->block_size || table_stride < max_blocks || table_stride > 0x7fffffff)) why = "attn_cached: table_stride must be at least max_blocks, the keys of a row below 2^31";
+    const Path path = why ? Path::FUSED : path_of(shape, n_seqs, n_tokens, max_blocks * cache->block_size, many_rows(shape, n_seqs, n_tokens));
+    if (!why) why = too_many(shape, n_seqs, n_tokens, max_blocks * cache->block_size, true, path);
     if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_attn_cached_workspace(shape, n_seqs, n_tokens, cache, max_blocks))) why = "attn_cached: workspace is null, unaligned or too small";
     if (why) return fail(ATLAS_EINVAL, why);
     if (!n_seqs || !n_tokens) return ATLAS_OK;
@@ -226,11 +247,11 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     Args A = args_of(shape, q, d_cu_new, n_seqs, n_tokens, out);
     A.ck = cache->d_k; A.cv = cache->d_v; A.lens = d_kv_lens; A.table = d_block_table; A.table_stride = (int64_t)table_stride;
     A.n_blocks = (uint32_t)cache->n_blocks; A.log_block = log2_of(cache->block_size); A.max_keys = (uint32_t)(max_blocks * cache->block_size);
-    if (fused(shape, n_seqs, n_tokens, A.max_keys, many_rows(shape, n_seqs, n_tokens))) {
+    if (path == Path::FUSED) {
         if (int rc = cache->bits == 16 ? launch_fused<int16_t>(A, A.max_keys, L.stream) : launch_fused<int32_t>(A, A.max_keys, L.stream)) return rc;
         return L.end();
     }
-    if (many_rows(shape, n_seqs, n_tokens)) {
+    if (path == Path::TILES) {
         const PlanesLayout P(shape, n_seqs, n_tokens, std::max<size_t>(A.max_keys, 1));
         if (int rc = cache->bits == 16 ? launch_tiles<int16_t>(A, P, P.at(d_workspace, shape), L.stream) : launch_tiles<int32_t>(A, P, P.at(d_workspace, shape), L.stream)) return rc;
         return L.end();

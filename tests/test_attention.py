@@ -196,3 +196,29 @@ def test_query_rows_past_32_bits_are_refused(n):
         with pytest.raises(A.AtlasError):
             f()
     assert at.prompt_workspace_bytes(1, (1 << 22) - 1) > 0
+
+
+@pytest.mark.parametrize("heads,kv,n,seqs,cols", [(64, 64, 1 << 17, 1 << 17, 4), (32, 32, 1 << 19, 1 << 19, 300), (32, 8, 1 << 19, 1 << 19, 300),
+                                                  (32, 8, 100, 1 << 24, 300), (2, 1, 1 << 21, 1 << 14, 1 << 20)])
+def test_more_than_a_launch_holds_is_refused(heads, kv, n, seqs, cols):
+    """on the host, before the first of a path's launches"""
+    import jolt_atlas_amd as A
+    import jolt_atlas_amd.attention as T
+    at, cache = T.Attention(heads, kv, 8), T.KVCache(Fake((7, kv, 16, 8)), Fake((7, kv, 16, 8)))
+    with pytest.raises(A.AtlasError):
+        at.cached_workspace_bytes(seqs, n, cache, cols)
+    with pytest.raises(A.AtlasError, match="too many"):
+        at.cached(Fake((n, heads, 8)), Fake((seqs + 1,)), Fake((seqs,)), cache, Fake((seqs, cols)), Fake((n, heads, 8), ptr=1 << 41), Fake((1 << 60,), "uint8"))
+
+
+def test_more_tokens_than_a_launch_holds_are_refused():
+    import jolt_atlas_amd as A
+    import jolt_atlas_amd.attention as T
+    at, n = T.Attention(1, 1, 8), 1 << 29
+    with pytest.raises(A.AtlasError):
+        at.prompt_workspace_bytes(1, n)
+    with pytest.raises(A.AtlasError, match="too many"):
+        at.prompt(*(Fake((n, 1, 8)) for _ in range(3)), Fake((2,)), Fake((n, 1, 8), ptr=1 << 41), Fake((1 << 60,), "uint8"))
+    assert at.prompt_workspace_bytes(1, n - 1024) > 0
+    # 2^17 tokens of 64 heads over one: 655360 workgroups of 512 threads, below 2^32 of them
+    assert T.Attention(64, 1, 8).cached_workspace_bytes(1 << 17, 1 << 17, T.KVCache(Fake((7, 1, 16, 8)), Fake((7, 1, 16, 8))), 4) > 0
