@@ -91,6 +91,13 @@ def _table(t):
     return t.data_ptr(), t.shape[1], max(t.stride()[0], t.shape[1])
 
 
+def _status(t):
+    """one 32-bit word that the kernels write: any array of at least one element"""
+    if _name(t.dtype) not in ("int32", "uint32") or 0 in tuple(t.shape):
+        raise ValueError(f"status: one int32 or uint32 expected, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
 def _workspace(w):
     return w.data_ptr(), w.shape[0] * w.itemsize
 
@@ -122,7 +129,7 @@ class KVCache:
         if v.shape[0] != n:
             raise ValueError("KVCache.write: k and v have the same number of rows")
         _check(lib.atlas_kv_write(C.byref(self._shape), C.byref(_rows(k, "k", self.n_kv_heads, self.head_dim)), C.byref(_rows(v, "v", self.n_kv_heads, self.head_dim)),
-                                  _vector(slots, "slots", "int64", n), n, C.byref(self.desc), None if status is None else status.data_ptr(), _stream(stream)))
+                                  _vector(slots, "slots", "int64", n), n, C.byref(self.desc), None if status is None else _status(status), _stream(stream)))
 
 
 class Attention:
@@ -189,4 +196,4 @@ class Pager:
         _check(lib.atlas_kv_plan(self.block_size, self.n_blocks, _vector(cached_lens, "cached_lens", "int32"), _vector(new_lens, "new_lens", "int32", n), n, table, cols, stride,
                                  _vector(free_blocks, "free_blocks", "int32", self.n_blocks), _vector(n_free, "n_free", "int32", 1), _vector(n_free_out, "n_free_out", "int32", 1),
                                  _vector(cu_new, "cu_new", "int32", n + 1), _vector(kv_lens, "kv_lens", "int32", n), _vector(slots, "slots", "int64"),
-                                 None if positions is None else _vector(positions, "positions", "int32", cap), cap, status.data_ptr(), p, size, _stream(stream)))
+                                 None if positions is None else _vector(positions, "positions", "int32", cap), cap, _status(status), p, size, _stream(stream)))

@@ -222,3 +222,24 @@ def test_more_tokens_than_a_launch_holds_are_refused():
     assert at.prompt_workspace_bytes(1, n - 1024) > 0
     # 2^17 tokens of 64 heads over one: 655360 workgroups of 512 threads, below 2^32 of them
     assert T.Attention(64, 1, 8).cached_workspace_bytes(1 << 17, 1 << 17, T.KVCache(Fake((7, 1, 16, 8)), Fake((7, 1, 16, 8))), 4) > 0
+
+
+@pytest.mark.parametrize("status", [Fake((1,), "int8"), Fake((4,), "uint8"), Fake((1,), "bool"), Fake((1,), "int64"), Fake((0,)), Fake((3, 0))])
+def test_a_status_that_is_no_32_bit_word(status):
+    import jolt_atlas_amd.attention as T
+    cache = T.KVCache(Fake((7, 2, 16, 8)), Fake((7, 2, 16, 8)))
+    with pytest.raises(ValueError, match="status"):
+        cache.write(Fake((5, 2, 8)), Fake((5, 2, 8)), Fake((5,), "int64"), status)
+    with pytest.raises(ValueError, match="status"):
+        _plan(status=status)
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_a_status_that_is_not_aligned(off):
+    import jolt_atlas_amd as A
+    import jolt_atlas_amd.attention as T
+    cache, status = T.KVCache(Fake((7, 2, 16, 8)), Fake((7, 2, 16, 8))), Fake((1,), "uint32", ptr=(1 << 40) + off)
+    with pytest.raises(A.AtlasError, match="status must be 4-byte"):
+        cache.write(Fake((5, 2, 8)), Fake((5, 2, 8)), Fake((5,), "int64"), status)
+    with pytest.raises(A.AtlasError, match="status must be 4-byte"):
+        _plan(status=status)
