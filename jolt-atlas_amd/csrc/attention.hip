@@ -195,6 +195,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (!why) why = bad_out(out, n_tokens, shape->n_heads, shape->head_dim);
     if (!why && n_tokens && (out->d == q->d || out->d == k->d || out->d == v->d)) why = "attn_prompt: out may not be q, k or v";
     if (!why && !d_cu_seqlens) why = "attn_prompt: cu_seqlens is null";
+    if (!why && unaligned({d_cu_seqlens})) why = "attn_prompt: cu_seqlens must be 4-byte aligned";
     const Path path = why ? Path::FUSED : path_of(shape, n_seqs, n_tokens, n_tokens, true);
     if (!why) why = too_many(shape, n_seqs, n_tokens, n_tokens, false, path);
     if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_attn_prompt_workspace(shape, n_seqs, n_tokens))) why = "attn_prompt: workspace is null, unaligned or too small";
@@ -235,6 +236,7 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (!why) why = bad_cache(cache);
     if (!why && n_tokens && out->d == q->d) why = "attn_cached: out may not be q";
     if (!why && (!d_cu_new || !d_kv_lens || !d_block_table)) why = "attn_cached: cu_new, kv_lens or block_table is null";
+    if (!why && unaligned({d_cu_new, d_kv_lens, d_block_table})) why = "attn_cached: cu_new, kv_lens and block_table must be 4-byte aligned";
     if (!why && (max_blocks > 0x7fffffff / cache->block_size || table_stride < max_blocks || table_stride > 0x7fffffff)) why = "attn_cached: table_stride must be at least max_blocks, the keys of a row below 2^31";
     const Path path = why ? Path::FUSED : path_of(shape, n_seqs, n_tokens, max_blocks * cache->block_size, many_rows(shape, n_seqs, n_tokens));
     if (!why) why = too_many(shape, n_seqs, n_tokens, max_blocks * cache->block_size, true, path);

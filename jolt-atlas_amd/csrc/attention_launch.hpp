@@ -41,6 +41,10 @@ inline const char* bad_cache(const atlas_kv_cache_t* c) {
     if (c->n_blocks < 1 || c->n_blocks > 0x7fffffff) return "attention: n_blocks must be 1 .. 2^31 - 1";
     return nullptr;
 }
+inline bool unaligned(std::initializer_list<const void*> ps) {          // int32 arrays
+    for (const void* p : ps) if ((uintptr_t)p % 4) return true;
+    return false;
+}
 inline uint32_t log2_of(size_t v) { uint32_t l = 0; while (((size_t)1 << l) < v) l++; return l; }
 
 // Enqueues on the caller's stream, or on the library's: that one under its lock (another thread's pipeline may have it on a lane).  The calling thread's

@@ -224,6 +224,7 @@ int atlas_kv_plan(size_t block_size, size_t n_blocks, const int32_t* d_cached_le
     if (!why && n_seqs && (d_kv_lens == d_cached_lens || d_kv_lens == d_new_lens)) why = "kv_plan: kv_lens may not be cached_lens or new_lens";
     if (!why && (uintptr_t)d_slots % 8) why = "kv_plan: slots must be 8-byte aligned";
     if (!why && (uintptr_t)d_status % 4) why = "kv_plan: status must be 4-byte aligned";
+    if (!why && atlas_attn::unaligned({d_cached_lens, d_new_lens, d_block_table, d_free_blocks, d_n_free, d_n_free_out, d_cu_new, d_kv_lens, d_positions})) why = "kv_plan: int32 arrays must be 4-byte aligned";
     if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_kv_plan_workspace(n_seqs, max_tokens))) why = "kv_plan: workspace is null, unaligned or too small";
     if (why) return fail(ATLAS_EINVAL, why);
     atlas_attn::Launch L;

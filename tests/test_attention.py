@@ -243,3 +243,18 @@ def test_a_status_that_is_not_aligned(off):
         cache.write(Fake((5, 2, 8)), Fake((5, 2, 8)), Fake((5,), "int64"), status)
     with pytest.raises(A.AtlasError, match="status must be 4-byte"):
         _plan(status=status)
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_offsets_tables_and_lengths_that_are_not_aligned(off):
+    import jolt_atlas_amd as A
+    at = (1 << 40) + off
+    with pytest.raises(A.AtlasError, match="4-byte"):
+        _prompt(cu=Fake((3,), ptr=at))
+    for kw in (dict(cu=Fake((3,), ptr=at)), dict(lens=Fake((2,), ptr=at)), dict(table=Fake((2, 5), ptr=at))):
+        with pytest.raises(A.AtlasError, match="4-byte"):
+            _cached(**kw)
+    for kw in (dict(have=Fake((2,), ptr=at)), dict(new=Fake((2,), ptr=at)), dict(table=Fake((2, 5), ptr=at)), dict(free=Fake((9,), ptr=at)), dict(n_free=Fake((1,), ptr=at)),
+               dict(n_out=Fake((1,), ptr=at)), dict(cu=Fake((3,), ptr=at)), dict(lens=Fake((2,), ptr=(1 << 41) + off)), dict(pos=Fake((6,), ptr=at))):
+        with pytest.raises(A.AtlasError, match="4-byte"):
+            _plan(**kw)
