@@ -98,8 +98,17 @@ def _status(t):
     return t.data_ptr()
 
 
+def _contiguous(t, name):
+    want = 1
+    for n, s in zip(reversed(t.shape), reversed(t.stride())):
+        if n > 1 and s != want:
+            raise ValueError(f"{name}: a contiguous array expected")
+        want *= n
+    return want
+
+
 def _workspace(w):
-    return w.data_ptr(), w.shape[0] * w.itemsize
+    return w.data_ptr(), _contiguous(w, "workspace") * w.itemsize
 
 
 class KVCache:
@@ -111,12 +120,7 @@ class KVCache:
         bits = {"int32": 32, "int16": 16}.get(_name(k.dtype))
         if bits is None:
             raise ValueError(f"KVCache: int32 or int16 expected, got {k.dtype}")
-        for t in (k, v):
-            want = 1
-            for n, s in zip(reversed(t.shape), reversed(t.stride())):
-                if n > 1 and s != want:
-                    raise ValueError("KVCache: contiguous arrays expected")
-                want *= n
+        _contiguous(k, "KVCache: k"), _contiguous(v, "KVCache: v")
         self.k, self.v = k, v
         self.n_blocks, self.n_kv_heads, self.block_size, self.head_dim = k.shape
         self.desc = _Cache(k.data_ptr(), v.data_ptr(), self.n_blocks, self.block_size, bits)

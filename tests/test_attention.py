@@ -258,3 +258,11 @@ def test_offsets_tables_and_lengths_that_are_not_aligned(off):
                dict(n_out=Fake((1,), ptr=at)), dict(cu=Fake((3,), ptr=at)), dict(lens=Fake((2,), ptr=(1 << 41) + off)), dict(pos=Fake((6,), ptr=at))):
         with pytest.raises(A.AtlasError, match="4-byte"):
             _plan(**kw)
+
+
+@pytest.mark.parametrize("ws", [Fake((1 << 22,), "uint8", strides=(0,)), Fake((1 << 22,), "uint8", strides=(2,)), Fake((1 << 11, 1 << 11), "uint8", strides=(0, 1))])
+def test_a_workspace_that_is_not_all_there(ws):
+    """an expanded array is as long as its shape says and has the memory of one element"""
+    for call in (_prompt, _cached, _plan):
+        with pytest.raises(ValueError, match="workspace"):
+            call(ws=ws)
