@@ -140,6 +140,8 @@ class Attention:
     """score_mul: the Mul node's constant at scale 2^14 (round(2^14 / sqrt(head_dim)) is the usual; ONE: the graph has no such node)"""
 
     def __init__(self, n_heads, n_kv_heads, head_dim, score_mul=ONE, causal=True):
+        if not -(1 << 31) <= score_mul < 1 << 31:              # ctypes would cut it to 32 bits
+            raise ValueError(f"Attention: score_mul must be 1 .. 2^14, got {score_mul}")
         self.n_heads, self.n_kv_heads, self.head_dim = n_heads, n_kv_heads, head_dim
         self.shape = _Shape(n_heads, n_kv_heads, head_dim, score_mul, 1 if causal else 0)
 

@@ -266,3 +266,9 @@ def test_a_workspace_that_is_not_all_there(ws):
     for call in (_prompt, _cached, _plan):
         with pytest.raises(ValueError, match="workspace"):
             call(ws=ws)
+
+
+@pytest.mark.parametrize("mul", [(1 << 32) + 2048, -(1 << 32) + 1, 1 << 31])
+def test_a_score_mul_that_32_bits_do_not_hold(mul):
+    with pytest.raises(ValueError, match="score_mul"):
+        _prompt(mul=mul)
