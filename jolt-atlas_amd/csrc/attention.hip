@@ -194,7 +194,7 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (!why) why = bad_rows(out, n_tokens, shape->n_heads, shape->head_dim);
     if (!why) why = bad_out(out, n_tokens, shape->n_heads, shape->head_dim);
     if (!why && n_tokens && (out->d == q->d || out->d == k->d || out->d == v->d)) why = "attn_prompt: out may not be q, k or v";
-    if (!why && !d_cu_seqlens) why = "attn_prompt: cu_seqlens is null";
+    if (!why && n_seqs && n_tokens && !d_cu_seqlens) why = "attn_prompt: cu_seqlens is null";
     if (!why && unaligned({d_cu_seqlens})) why = "attn_prompt: cu_seqlens must be 4-byte aligned";
     const Path path = why ? Path::FUSED : path_of(shape, n_seqs, n_tokens, n_tokens, true);
     if (!why) why = too_many(shape, n_seqs, n_tokens, n_tokens, false, path);
@@ -235,7 +235,7 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (!why) why = bad_out(out, n_tokens, shape->n_heads, shape->head_dim);
     if (!why) why = bad_cache(cache);
     if (!why && n_tokens && out->d == q->d) why = "attn_cached: out may not be q";
-    if (!why && (!d_cu_new || !d_kv_lens || !d_block_table)) why = "attn_cached: cu_new, kv_lens or block_table is null";
+    if (!why && n_seqs && n_tokens && (!d_cu_new || !d_kv_lens || (max_blocks && !d_block_table))) why = "attn_cached: cu_new, kv_lens or block_table is null";
     if (!why && unaligned({d_cu_new, d_kv_lens, d_block_table})) why = "attn_cached: cu_new, kv_lens and block_table must be 4-byte aligned";
     if (!why && (max_blocks > 0x7fffffff / cache->block_size || table_stride < max_blocks || table_stride > 0x7fffffff)) why = "attn_cached: table_stride must be at least max_blocks, the keys of a row below 2^31";
     const Path path = why ? Path::FUSED : path_of(shape, n_seqs, n_tokens, max_blocks * cache->block_size, many_rows(shape, n_seqs, n_tokens));
@@ -247,7 +247,8 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (int rc = L.begin(stream)) return rc;
     if (int rc = L.on_device({q->d, d_cu_new, d_kv_lens, cache->d_k, cache->d_v, d_block_table, out->d, d_workspace})) return rc;
     Args A = args_of(shape, q, d_cu_new, n_seqs, n_tokens, out);
-    A.ck = cache->d_k; A.cv = cache->d_v; A.lens = d_kv_lens; A.table = d_block_table; A.table_stride = (int64_t)table_stride;
+    // a table without columns (nothing is cached, its array may be empty) is never looked at
+    A.ck = cache->d_k; A.cv = cache->d_v; A.lens = d_kv_lens; A.table = max_blocks ? d_block_table : d_kv_lens; A.table_stride = (int64_t)table_stride;
     A.n_blocks = (uint32_t)cache->n_blocks; A.log_block = log2_of(cache->block_size); A.max_keys = (uint32_t)(max_blocks * cache->block_size);
     if (path == Path::FUSED) {
         if (int rc = cache->bits == 16 ? launch_fused<int16_t>(A, A.max_keys, L.stream) : launch_fused<int32_t>(A, A.max_keys, L.stream)) return rc;

@@ -193,7 +193,7 @@ int atlas_kv_write(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* k, 
     if (!why) why = atlas_attn::bad_rows(k, n_tokens, shape->n_kv_heads, shape->head_dim);
     if (!why) why = atlas_attn::bad_rows(v, n_tokens, shape->n_kv_heads, shape->head_dim);
     if (!why) why = atlas_attn::bad_cache(cache);
-    if (!why && (!d_slots || (uintptr_t)d_slots % 8)) why = "kv_write: slots are null or not 8-byte aligned";
+    if (!why && ((n_tokens && !d_slots) || (uintptr_t)d_slots % 8)) why = "kv_write: slots are null or not 8-byte aligned";
     if (!why && (uintptr_t)d_status % 4) why = "kv_write: status must be 4-byte aligned";
     if (why) return fail(ATLAS_EINVAL, why);
     if (!n_tokens) return ATLAS_OK;
@@ -220,7 +220,7 @@ int atlas_kv_plan(size_t block_size, size_t n_blocks, const int32_t* d_cached_le
     if (!why && !block_ok(block_size)) why = "kv_plan: block_size must be a power of two, at most 4096";
     if (!why && (n_blocks < 1 || n_blocks > 0x7fffffff)) why = "kv_plan: n_blocks must be 1 .. 2^31 - 1";
     if (!why && (max_blocks > 0x7fffffff / block_size || table_stride < max_blocks || table_stride > 0x7fffffff)) why = "kv_plan: table_stride must be at least max_blocks, the keys of a row below 2^31";
-    if (!why && ((n_seqs && (!d_cached_lens || !d_new_lens || !d_block_table || !d_kv_lens)) || !d_free_blocks || !d_n_free || !d_n_free_out || !d_cu_new || (max_tokens && !d_slots) || !d_status)) why = "kv_plan: null argument";
+    if (!why && ((n_seqs && (!d_cached_lens || !d_new_lens || (max_blocks && !d_block_table) || !d_kv_lens)) || !d_free_blocks || !d_n_free || !d_n_free_out || !d_cu_new || (max_tokens && !d_slots) || !d_status)) why = "kv_plan: null argument";
     if (!why && n_seqs && (d_kv_lens == d_cached_lens || d_kv_lens == d_new_lens)) why = "kv_plan: kv_lens may not be cached_lens or new_lens";
     if (!why && (uintptr_t)d_slots % 8) why = "kv_plan: slots must be 8-byte aligned";
     if (!why && (uintptr_t)d_status % 4) why = "kv_plan: status must be 4-byte aligned";

@@ -272,3 +272,19 @@ def test_a_workspace_that_is_not_all_there(ws):
 def test_a_score_mul_that_32_bits_do_not_hold(mul):
     with pytest.raises(ValueError, match="score_mul"):
         _prompt(mul=mul)
+
+
+def test_steps_without_tokens_or_sequences():
+    """empty arrays have no address (torch's is 0): nothing is enqueued and nothing is wrong"""
+    import jolt_atlas_amd.attention as T
+    none = lambda *shape, dtype="int32": Fake(shape, dtype, ptr=0)  # noqa: E731
+    cache = T.KVCache(Fake((7, 2, 16, 8)), Fake((7, 2, 16, 8)))
+    cache.write(none(0, 2, 8), none(0, 2, 8), none(0, dtype="int64"))
+    at, ws = T.Attention(4, 2, 8), Fake((1 << 22,), "uint8")
+    rows = none(0, 4, 8)
+    assert at.cached(rows, Fake((1,)), none(0), cache, none(0, 5), rows, ws) is rows                  # no requests
+    assert at.cached(rows, Fake((3,)), Fake((2,)), cache, Fake((2, 5)), rows, ws) is rows             # all of them pause
+    assert at.cached(rows, Fake((3,)), Fake((2,)), cache, none(2, 0), rows, ws) is rows
+    out = Fake((5, 4, 8), ptr=1 << 41)
+    assert at.cached(Fake((5, 4, 8)), Fake((1,)), none(0), cache, none(0, 5), out, ws) is out         # only padding
+    assert at.prompt(rows, none(0, 2, 8), none(0, 2, 8), Fake((1,)), rows, ws) is rows

@@ -329,6 +329,25 @@ def test_cached_of_any_int32(atlas):
         assert np.array_equal(run_cached(q, c16, c16, table, keys, new), want_cached(q, c16, c16, table, flat, keys, new))
 
 
+@pytest.mark.parametrize("new", [1, 60, 700])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_table_without_columns(atlas, new, causal):
+    """nothing can be cached: an empty table has no address, its rows are empty, and a step that needs a block does not fit"""
+    import jolt_atlas_amd.attention as T
+    rng = np.random.default_rng(new)
+    at, cache = T.Attention(8, 2, 16, causal=causal), T.KVCache(*(Dev(np.zeros((3, 2, 16, 16), np.int32)) for _ in range(2)))
+    q, out = Dev(values(rng, (new, 8, 16))), Dev(np.full((new, 8, 16), MARK, np.int32))
+    table = Dev(np.zeros((1, 0), np.int32))
+    table.data_ptr = lambda: 0
+    at.cached(q, Dev(np.array([0, new], np.int32)), Dev(np.array([new], np.int32)), cache, table, out, workspace(at.cached_workspace_bytes(1, new, cache, 0)))
+    assert not out.numpy().any()
+    i32, pager = lambda *x: Dev(np.array(x, np.int32)), T.Pager(16, 3)  # noqa: E731
+    for have, fresh, want in ((0, new, T.NO_COLUMNS), (0, 0, 0), (0, -1, 0)):
+        status, cu, lens, n_out = i32(77), i32(77, 77), i32(77), i32(77)
+        pager.plan(i32(have), i32(fresh), table, i32(0, 1, 2), i32(3), n_out, cu, lens, Dev(np.zeros(700, np.int64)), None, status, workspace(pager.workspace_bytes(1, 700)))
+        assert (status.numpy()[0], n_out.numpy()[0], cu.numpy().tolist(), lens.numpy()[0]) == (want, 3, [0, 0], 0)
+
+
 def test_rows_behind_the_last_sequence_stay(atlas):
     import jolt_atlas_amd.attention as T
     rng = np.random.default_rng(8)
