@@ -868,7 +868,8 @@ int atlas_verify_graph(atlas_graph_t g, const atlas_hyperkzg_vk_t *vk, const int
  * caller's hipStream_t; NULL = the library stream, ATLAS_STREAM_DEFAULT = HIP's default stream.  Lengths, tables and slots are read on the
  * device when the launches run.  All pointers are device memory of the calling thread's device (atlas_init / atlas_init_thread).  A workspace
  * (16-byte aligned) belongs to one call in flight: two streams, or two captured graphs that may run at once, need one each.  Its size goes by the
- * arguments, not by the lengths on the device: a table of many columns costs atlas_attn_cached the room for max_blocks * block_size keys a sequence. */
+ * arguments, not by the lengths on the device: a table of many columns costs atlas_attn_cached the room for max_blocks * block_size keys a sequence.  The sizes never
+ * decrease: a workspace for a server's largest step serves every step of no more sequences, tokens and columns.  A size of 0: no call takes these arguments. */
 #define ATLAS_STREAM_DEFAULT ((void *)1)
 typedef struct {
     size_t n_heads, n_kv_heads;   /* head h reads the keys and values of head h / (n_heads / n_kv_heads); at most 1024 heads, n_tokens * n_heads / n_kv_heads at most 2^32 - 256 */

@@ -141,6 +141,7 @@ bool fused(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t m
 }
 enum class Path { FUSED, TILES, SPLIT };
 Path path_of(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys, bool many) {
+    if (!n_seqs || !n_tokens) return Path::FUSED;                  // nothing is launched, nothing is needed
     return fused(s, n_seqs, n_tokens, max_keys, many) ? Path::FUSED : many ? Path::TILES : Path::SPLIT;
 }
 // What a path's launches and 32-bit counters hold: a launch has fewer than 2^32 threads
@@ -156,6 +157,20 @@ const char* too_many(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens
         over = n_tokens * s->n_heads > launch / 256 || row_tiles * s->n_kv_heads > 0x40000000 || row_tiles * s->n_kv_heads * units > 0x7fffffff;
     }
     return over ? "attention: too many sequences, rows or keys for one call" : nullptr;
+}
+// What a call over a cache needs
+size_t cached_bytes(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys, Path path) {
+    if (path == Path::FUSED) return 16;
+    return path == Path::TILES ? PlanesLayout(s, n_seqs, n_tokens, std::max<size_t>(max_keys, 1)).bytes : SplitLayout(s, n_seqs, n_tokens, max_keys, nullptr).bytes;
+}
+// The most that one of at most so many sequences, tokens and keys needs: a smaller one may take another path, and the one launch needs nothing.  Each layout grows with its
+// arguments, so the largest call that can take the path stands for all: the split path has up to 96 rows to a sequence, tiles the fewest sequences.
+size_t most_bytes(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys) {
+    const size_t G = s->n_heads / s->n_kv_heads, tokens = std::min(n_tokens, 96 * n_seqs / G), seqs = n_tokens ? std::min(n_seqs, (n_tokens * G - 1) / 96) : 0;
+    size_t most = 16;
+    if (tokens && !fused(s, 1, 1, max_keys, false)) most = std::max(most, cached_bytes(s, n_seqs, tokens, max_keys, Path::SPLIT));
+    if (seqs && !fused(s, seqs, n_tokens, max_keys, true)) most = std::max(most, cached_bytes(s, seqs, n_tokens, max_keys, Path::TILES));
+    return most;
 }
 template <class CT>
 int launch_fused(const Args& A, size_t max_keys, hipStream_t stream) {
@@ -220,8 +235,7 @@ size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seq
     const size_t max_keys = max_blocks * cache->block_size;
     const Path path = path_of(shape, n_seqs, n_tokens, max_keys, many_rows(shape, n_seqs, n_tokens));
     if (too_many(shape, n_seqs, n_tokens, max_keys, true, path)) return 0;
-    if (path == Path::FUSED) return 16;
-    return path == Path::TILES ? PlanesLayout(shape, n_seqs, n_tokens, std::max<size_t>(max_keys, 1)).bytes : SplitLayout(shape, n_seqs, n_tokens, max_keys, nullptr).bytes;
+    return most_bytes(shape, n_seqs, n_tokens, max_keys);
 }
 
 int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const int32_t* d_cu_new, const int32_t* d_kv_lens, size_t n_seqs, size_t n_tokens,
@@ -240,7 +254,7 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     if (!why && (max_blocks > 0x7fffffff / cache->block_size || table_stride < max_blocks || table_stride > 0x7fffffff)) why = "attn_cached: table_stride must be at least max_blocks, the keys of a row below 2^31";
     const Path path = why ? Path::FUSED : path_of(shape, n_seqs, n_tokens, max_blocks * cache->block_size, many_rows(shape, n_seqs, n_tokens));
     if (!why) why = too_many(shape, n_seqs, n_tokens, max_blocks * cache->block_size, true, path);
-    if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_attn_cached_workspace(shape, n_seqs, n_tokens, cache, max_blocks))) why = "attn_cached: workspace is null, unaligned or too small";
+    if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < cached_bytes(shape, n_seqs, n_tokens, max_blocks * cache->block_size, path))) why = "attn_cached: workspace is null, unaligned or too small";
     if (why) return fail(ATLAS_EINVAL, why);
     if (!n_seqs || !n_tokens) return ATLAS_OK;
     Launch L;

@@ -288,3 +288,48 @@ def test_steps_without_tokens_or_sequences():
     out = Fake((5, 4, 8), ptr=1 << 41)
     assert at.cached(Fake((5, 4, 8)), Fake((1,)), none(0), cache, none(0, 5), out, ws) is out         # only padding
     assert at.prompt(rows, none(0, 2, 8), none(0, 2, 8), Fake((1,)), rows, ws) is rows
+
+
+def test_a_workspace_serves_smaller_calls():
+    """the sizes do not decrease in any argument"""
+    import jolt_atlas_amd.attention as T
+    rng = np.random.default_rng(17)
+    for _ in range(3000):
+        kv, group, d, block = int(rng.choice([1, 2, 5, 8, 16, 64])), int(rng.choice([1, 2, 3, 8, 40])), int(rng.choice([1, 16, 64, 80, 128, 200, 256])), int(rng.choice([1, 16, 128]))
+        if kv * group > 1024:
+            continue
+        at, cache = T.Attention(kv * group, kv, d), T.KVCache(*(Fake((7, kv, block, d)) for _ in range(2)))
+        small = [int(np.exp(rng.uniform(0, np.log(x)))) for x in (300, 20000, 20000)]
+        large = [x if rng.random() < 0.3 else x + int(np.exp(rng.uniform(0, np.log(x + 300)))) for x in small]
+        size = lambda a: at.cached_workspace_bytes(a[0], a[1], cache, -(-a[2] // block))  # noqa: E731
+        assert size(small) <= size(large), (kv, group, d, block, small, large)
+        assert at.prompt_workspace_bytes(*small[:2]) <= at.prompt_workspace_bytes(*large[:2]), (kv, group, d, small, large)
+
+
+@pytest.mark.parametrize("n", [0, 1, 2, 15, 16, 33, 64])
+def test_a_serving_steps_workspace_serves_fewer_requests(n):
+    """16 heads of 64, 125 blocks of 16: 16 single tokens are one launch, which needs nothing, fewer are not"""
+    import jolt_atlas_amd as A
+    import jolt_atlas_amd.attention as T
+    at, cache = T.Attention(16, 16, 64), T.KVCache(*(Fake((7, 16, 16, 64)) for _ in range(2)))
+    ws = Fake((at.cached_workspace_bytes(64, 64, cache, 125),), "uint8")
+    try:
+        at.cached(Fake((n, 16, 64)), Fake((n + 1,)), Fake((n,)), cache, Fake((n, 125)), Fake((n, 16, 64), ptr=1 << 41), ws)
+    except A.AtlasError as e:               # no device here, or addresses that are not its
+        assert "workspace" not in str(e)
+
+
+@pytest.mark.parametrize("seqs,tokens", [(0, 0), (0, 1), (0, 900), (3, 0), (1, 1)])
+def test_a_workspace_of_the_size_asked_for(seqs, tokens):
+    import jolt_atlas_amd as A
+    import jolt_atlas_amd.attention as T
+    at, cache = T.Attention(16, 16, 64), T.KVCache(*(Fake((7, 16, 16, 64)) for _ in range(2)))
+    for cols in (1, 125, 4000):
+        q, out = Fake((tokens, 16, 64)), Fake((tokens, 16, 64), ptr=1 << 41)
+        calls = [lambda: at.cached(q, Fake((seqs + 1,)), Fake((seqs,)), cache, Fake((seqs, cols)), out, Fake((at.cached_workspace_bytes(seqs, tokens, cache, cols),), "uint8")),
+                 lambda: at.prompt(q, q, q, Fake((seqs + 1,)), out, Fake((at.prompt_workspace_bytes(seqs, tokens),), "uint8"))]
+        for f in calls:
+            try:
+                f()
+            except A.AtlasError as e:       # no device here, or addresses that are not its
+                assert seqs and tokens and "workspace" not in str(e)
