@@ -5,13 +5,18 @@ values (Attention.cached) —, the cache and its write (KVCache), and the paging
 graph.Graph.trace has it, so what was generated is what atlas_prove_graph proves.
 
 Tensors are device arrays of anything that has data_ptr(), shape, stride() and dtype (torch tensors do); they are used in place, on the calling thread's
-device (init / init_thread).  stream: a hipStream_t as an integer (torch: torch.cuda.current_stream().cuda_stream, whose 0 is HIP's default
-stream), None = the library stream.  Calls enqueue and return; nothing is kept between them, so a call may be captured into a graph."""
+device (init / init_thread).  A process that uses torch imports it before this package: the one HIP runtime is then torch's.
+
+stream: a hipStream_t as an integer (torch: torch.cuda.current_stream().cuda_stream, whose 0 is HIP's default stream), or LIBRARY_STREAM, the stream that the library's
+other calls run on and that no other stream waits for or is waited for by.  None: torch's current stream where the arrays are torch tensors, so that a call comes after what
+made its inputs; the library stream for other arrays.  Calls enqueue and return; nothing is kept between them, so a call may be captured into a graph."""
 import ctypes as C
+import sys
 
 from . import AtlasError, _check, lib
 
 ONE = 1 << 14                       # scale 2^14; the score_mul that scales nothing
+LIBRARY_STREAM = "library"          # stream=
 NARROW, BAD_SLOT = 1, 2             # KVCache.write's status
 NO_BLOCKS, NO_COLUMNS, NO_TOKENS, BAD_LENGTH = 1, 2, 4, 8      # Pager.plan's status
 
@@ -38,8 +43,14 @@ lib.atlas_kv_plan_workspace.argtypes, lib.atlas_kv_plan_workspace.restype = [_sz
 lib.atlas_kv_plan.argtypes, lib.atlas_kv_plan.restype = [_sz, _sz, _vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp], C.c_int
 
 
-def _stream(stream):
-    return None if stream is None else (stream or 1)          # ATLAS_STREAM_DEFAULT
+def _stream(stream, t):
+    """the entry points' stream argument; t: one of the call's arrays"""
+    if stream is None:
+        torch = sys.modules.get("torch")
+        if torch is None or not isinstance(t, torch.Tensor) or not t.is_cuda:
+            return None
+        stream = torch.cuda.current_stream(t.device).cuda_stream
+    return None if stream is LIBRARY_STREAM else (stream or 1)          # ATLAS_STREAM_DEFAULT
 
 
 _names = {}                         # dtype -> "int32", ...: a call looks its arrays' types up six times
@@ -133,7 +144,7 @@ class KVCache:
         if v.shape[0] != n:
             raise ValueError("KVCache.write: k and v have the same number of rows")
         _check(lib.atlas_kv_write(C.byref(self._shape), C.byref(_rows(k, "k", self.n_kv_heads, self.head_dim)), C.byref(_rows(v, "v", self.n_kv_heads, self.head_dim)),
-                                  _vector(slots, "slots", "int64", n), n, C.byref(self.desc), None if status is None else _status(status), _stream(stream)))
+                                  _vector(slots, "slots", "int64", n), n, C.byref(self.desc), None if status is None else _status(status), _stream(stream, k)))
 
 
 class Attention:
@@ -165,7 +176,7 @@ class Attention:
         p, size = _workspace(workspace)
         _check(lib.atlas_attn_prompt(C.byref(self.shape), C.byref(_rows(q, "q", self.n_heads, self.head_dim)), C.byref(_rows(k, "k", self.n_kv_heads, self.head_dim)),
                                      C.byref(_rows(v, "v", self.n_kv_heads, self.head_dim)), _vector(cu_seqlens, "cu_seqlens", "int32"), n_seqs, n,
-                                     C.byref(_rows(out, "out", self.n_heads, self.head_dim)), p, size, _stream(stream)))
+                                     C.byref(_rows(out, "out", self.n_heads, self.head_dim)), p, size, _stream(stream, q)))
         return out
 
     def cached(self, q, cu_new, kv_lens, cache, block_table, out, workspace, stream=None):
@@ -179,7 +190,7 @@ class Attention:
         table, cols, stride = _table(block_table)
         _check(lib.atlas_attn_cached(C.byref(self.shape), C.byref(_rows(q, "q", self.n_heads, self.head_dim)), _vector(cu_new, "cu_new", "int32"),
                                      _vector(kv_lens, "kv_lens", "int32", n_seqs), n_seqs, n, C.byref(cache.desc), table, cols, stride,
-                                     C.byref(_rows(out, "out", self.n_heads, self.head_dim)), p, size, _stream(stream)))
+                                     C.byref(_rows(out, "out", self.n_heads, self.head_dim)), p, size, _stream(stream, q)))
         return out
 
 
@@ -202,4 +213,4 @@ class Pager:
         _check(lib.atlas_kv_plan(self.block_size, self.n_blocks, _vector(cached_lens, "cached_lens", "int32"), _vector(new_lens, "new_lens", "int32", n), n, table, cols, stride,
                                  _vector(free_blocks, "free_blocks", "int32", self.n_blocks), _vector(n_free, "n_free", "int32", 1), _vector(n_free_out, "n_free_out", "int32", 1),
                                  _vector(cu_new, "cu_new", "int32", n + 1), _vector(kv_lens, "kv_lens", "int32", n), _vector(slots, "slots", "int64"),
-                                 None if positions is None else _vector(positions, "positions", "int32", cap), cap, _status(status), p, size, _stream(stream)))
+                                 None if positions is None else _vector(positions, "positions", "int32", cap), cap, _status(status), p, size, _stream(stream, cached_lens)))

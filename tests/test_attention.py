@@ -333,3 +333,35 @@ def test_a_workspace_of_the_size_asked_for(seqs, tokens):
                 f()
             except A.AtlasError as e:       # no device here, or addresses that are not its
                 assert seqs and tokens and "workspace" not in str(e)
+
+
+def test_the_stream_of_torch_tensors(monkeypatch):
+    """without a stream of the caller's: torch's current one for torch tensors (0, its default, is the null stream), the library's for other arrays"""
+    import sys
+    import types
+    import jolt_atlas_amd.attention as T
+
+    class Tensor(Fake):
+        is_cuda, device = True, "cuda:0"
+
+    now = types.SimpleNamespace(cuda_stream=77)
+    monkeypatch.setitem(sys.modules, "torch", types.SimpleNamespace(Tensor=Tensor, cuda=types.SimpleNamespace(current_stream=lambda dev: now if dev == "cuda:0" else None)))
+    seen = {}
+    for name in ("atlas_attn_prompt", "atlas_attn_cached", "atlas_kv_write", "atlas_kv_plan"):
+        monkeypatch.setattr(T.lib, name, lambda *a, name=name: seen.__setitem__(name, a[-1]) or 0)
+
+    def streams(kind, **kw):
+        seen.clear()
+        t = lambda shape, dtype="int32", ptr=1 << 40: kind(shape, dtype, ptr=ptr)  # noqa: E731
+        at, cache, ws = T.Attention(4, 2, 8), T.KVCache(t((7, 2, 16, 8)), t((7, 2, 16, 8))), t((1 << 22,), "uint8")
+        at.prompt(t((5, 4, 8)), t((5, 2, 8)), t((5, 2, 8)), t((3,)), t((5, 4, 8), ptr=1 << 41), ws, **kw)
+        at.cached(t((3, 4, 8)), t((3,)), t((2,)), cache, t((2, 5)), t((3, 4, 8), ptr=1 << 41), ws, **kw)
+        cache.write(t((5, 2, 8)), t((5, 2, 8)), t((5,), "int64"), **kw)
+        T.Pager(16, 9).plan(t((2,)), t((2,)), t((2, 5)), t((9,)), t((1,)), t((1,)), t((3,)), t((2,)), t((6,), "int64"), None, t((1,)), ws, **kw)
+        assert len(seen) == 4 and len(set(seen.values())) == 1
+        return seen["atlas_kv_plan"]
+
+    assert streams(Fake) is None and streams(Tensor) == 77
+    now.cuda_stream = 0
+    assert streams(Tensor) == 1 and streams(Tensor, stream=5) == 5 and streams(Tensor, stream=0) == 1 and streams(Fake, stream=9) == 9
+    assert streams(Tensor, stream=T.LIBRARY_STREAM) is None and streams(Fake, stream=T.LIBRARY_STREAM) is None

@@ -820,3 +820,61 @@ def test_an_error_that_the_caller_left(atlas):
         f()
     want = prompt(q, k, v, [5])
     assert status.numpy()[0] == 0 and np.array_equal(out.numpy(), want) and np.array_equal(ck.numpy(), want)
+
+
+TORCH = """
+import sys
+import torch
+sys.path[:0] = [ROOT, ROOT + "/tests"]
+import jolt_atlas_amd as A
+import jolt_atlas_amd.attention as T
+import numpy as np
+from _attention_ref import prompt
+A.init(0)
+g = torch.Generator().manual_seed(5)
+n, H, KV, d, B = 90, 4, 2, 64, 16
+at = T.Attention(H, KV, d, 2048)
+cu = torch.tensor([0, 50, 90], dtype=torch.int32, device="cuda")
+ws = torch.empty(at.prompt_workspace_bytes(2, n), dtype=torch.uint8, device="cuda")
+big = torch.zeros(1 << 28, device="cuda")
+for side in (None, torch.cuda.Stream()):
+    with torch.cuda.stream(side or torch.cuda.default_stream()):
+        for rep in range(3):
+            h = [(torch.randn(n, x, d, generator=g) * 16384).round().to(torch.int32) for x in (H, KV, KV)]
+            q, k, v = (torch.zeros_like(x, device="cuda") for x in h)
+            out, src = torch.zeros_like(q), [x.pin_memory() for x in h]
+            torch.cuda.synchronize()
+            for _ in range(40):
+                big.add_(1.0)                          # some 20 ms of work: q, k and v come behind it
+            for x, y in zip((q, k, v), src):
+                x.copy_(y, non_blocking=True)
+            at.prompt(q, k, v, cu, out, ws)
+            kept = out.clone()                         # torch's next operation comes behind the call
+            out.zero_()
+            assert np.array_equal(kept.cpu().numpy(), prompt(*(x.numpy() for x in h), [50, 40], 2048)), (side, rep)
+            cache = T.KVCache(*(torch.zeros(9, KV, B, d, dtype=torch.int32, device="cuda") for _ in range(2)))
+            i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+            pager, table, free = T.Pager(B, 9), i32(*[-1] * 8).reshape(2, 4), i32(*range(9))
+            have, cun, lens, n_free = i32(0, 0), i32(0, 0, 0), i32(0, 0), i32(9)
+            slots, status = torch.zeros(100, dtype=torch.int64, device="cuda"), i32(7)
+            wp = torch.empty(pager.workspace_bytes(2, 100), dtype=torch.uint8, device="cuda")
+            pager.plan(have, i32(50, 40), table, free, n_free, n_free, cun, lens, slots, None, status, wp)
+            cache.write(k, v, slots, status)
+            out = torch.zeros_like(q)
+            wc = torch.empty(at.cached_workspace_bytes(2, n, cache, 4), dtype=torch.uint8, device="cuda")
+            at.cached(q, cun, lens, cache, table, out, wc)
+            assert int(status) == 0 and torch.equal(out, kept), (side, rep, int(status))
+print("torch ok", flush=True)
+"""
+
+
+def test_torch_tensors(tmp_path):
+    """torch tensors on torch's current stream, in a process of their own (torch comes first there)"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    f = tmp_path / "run.py"
+    f.write_text("ROOT = %r\n%s" % (root, TORCH))
+    r = subprocess.run([sys.executable, "-u", str(f)], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "torch ok" in r.stdout, r.stdout + r.stderr
