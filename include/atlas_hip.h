@@ -855,13 +855,14 @@ int atlas_verify_graph(atlas_graph_t g, const atlas_hyperkzg_vk_t *vk, const int
 /* ---- quantised attention for generation: the answer of a model before it is proved ------------------------------------------------
  * The attention of a model graph — Einsum (mbk,nbk->bmn), Mul by a constant, Iff with the causal mask, SoftmaxLastAxis, Einsum
  * (bmk,kbn->mbn), all at scale 2^14 — as one operator, without the graph's [heads, seq, seq] tensors, over packed prompts and token by
- * token over a paged cache of keys and values.  Integers throughout, so that a row comes out bit for bit as the traced graph (the one
- * atlas_prove_graph proves) has it, in whatever pieces the keys are visited:
+ * token over a paged cache of keys and values.  Integers throughout, so that a row in which the graph's masked keys carry no weight comes out bit for bit as the
+ * traced graph (the one atlas_prove_graph proves) has it, in whatever pieces the keys are visited:
  *     s = clamp((sum_d q k) >> 14);  s = clamp((s score_mul) >> 14);  z = min(max_j s - s, 2^18 - 1);
  *     e = (HI[z >> 9] LO[z & 511]) >> 14;  w = 2^28 / sum_j e;  p = (e w) >> 14;  out = clamp((sum_j p v) >> 14)
  * with the digit tables of SoftmaxLastAxis (atlas-onnx-tracer/src/ops/softmax.rs:74-269), floor shifts and clamps to 32 bits
- * (ops/einsum.rs:34-213).  Masked keys carry no weight (a graph whose mask fill lies 2^18 or more below every row's maximum); a row that
- * sees no key is 0.  Any int32 value is computed exactly (sums wrap modulo 2^64, as the graph's do); operands in [-8421504, 8355711]
+ * (ops/einsum.rs:34-213).  Masked keys carry no weight here.  In a graph they carry none while its mask fill lies 169985 or more (10.4) below every row's
+ * maximum; a fill of -8 or -10, as graphs have it, does so for some inputs and not for others, and only for the rows of which it holds are the two the
+ * same (atlas_attn_prompt_masked, atlas_attn_cached_masked tell).  A row that sees no key is 0.  Any int32 value is computed exactly (sums wrap modulo 2^64, as the graph's do); operands in [-8421504, 8355711]
  * with |q| |k| head_dim < 2^44 take the matrix cores (trained models stay far below: 2^18 is 16.0), rows beyond that a 64-bit path that is ~100 times slower.
  *
  * These entry points enqueue and return: no allocation, no wait, no state between calls, so they can be captured into HIP graphs.  `stream` is the
@@ -897,6 +898,19 @@ size_t atlas_attn_cached_workspace(const atlas_attn_shape_t *shape, size_t n_seq
 int atlas_attn_cached(const atlas_attn_shape_t *shape, const atlas_attn_rows_t *q, const int32_t *d_cu_new, const int32_t *d_kv_lens, size_t n_seqs, size_t n_tokens,
                       const atlas_kv_cache_t *cache, const int32_t *d_block_table, size_t max_blocks, size_t table_stride, const atlas_attn_rows_t *out,
                       void *d_workspace, size_t workspace_bytes, void *stream);
+/* The same with the question whether the graph would answer alike.  A graph has n_tokens tokens whatever is in them; its Iff gives the masked keys (those behind a
+ * row's own) the score `fill`, and the softmax some weight if that is not far enough below the row's maximum: none from 169985 below on (10.4 at scale 2^14), and
+ * above that where e is not 0.  *d_status (the caller clears it) gets ATLAS_ATTN_MASK_WEIGHS when masked keys would weigh in a row of the call, or be its
+ * maximum: that row of a trace may be another, and a proof of the trace is of another answer.  out is what the other two entry points give.  shape->causal must be 1.  A row at
+ * position n_tokens - 1 or later has no masked keys; one that sees no key is not looked at. */
+enum { ATLAS_ATTN_MASK_WEIGHS = 1 };
+typedef struct { int32_t fill; uint32_t n_tokens; uint32_t *d_status; } atlas_attn_mask_t;
+int atlas_attn_prompt_masked(const atlas_attn_shape_t *shape, const atlas_attn_rows_t *q, const atlas_attn_rows_t *k, const atlas_attn_rows_t *v,
+                             const int32_t *d_cu_seqlens, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t *out, const atlas_attn_mask_t *mask,
+                             void *d_workspace, size_t workspace_bytes, void *stream);
+int atlas_attn_cached_masked(const atlas_attn_shape_t *shape, const atlas_attn_rows_t *q, const int32_t *d_cu_new, const int32_t *d_kv_lens, size_t n_seqs,
+                             size_t n_tokens, const atlas_kv_cache_t *cache, const int32_t *d_block_table, size_t max_blocks, size_t table_stride,
+                             const atlas_attn_rows_t *out, const atlas_attn_mask_t *mask, void *d_workspace, size_t workspace_bytes, void *stream);
 /* Keys and values of n_tokens rows into the slots of a cache (slot = block * block_size + place in the block; a negative slot: the row is skipped).  Slots are
  * distinct: rows that share one leave a mixture.  *d_status (optional, the caller clears it) gets ATLAS_KV_NARROW when a value did not fit a
  * 16-bit cache (its nearest 16-bit value is stored: what follows is not the graph's answer) and ATLAS_KV_BAD_SLOT for a slot behind the cache (skipped). */

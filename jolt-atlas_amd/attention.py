@@ -1,8 +1,9 @@
 """Quantised attention for generation (atlas_attn_*, atlas_kv_*): ctypes marshalling only.
 
 The attention of a model graph in the graph executor's integers — over packed prompts (Attention.prompt) and over a paged cache of keys and
-values (Attention.cached) —, the cache and its write (KVCache), and the paging of a step from request lengths (Pager).  A row comes out bit for bit as
-graph.Graph.trace has it, so what was generated is what atlas_prove_graph proves.
+values (Attention.cached) —, the cache and its write (KVCache), and the paging of a step from request lengths (Pager).  A row in which the graph's masked keys
+carry no weight comes out bit for bit as graph.Graph.trace has it, so that what was generated is what atlas_prove_graph proves; whether they carry none goes by the
+graph's mask fill and the inputs, and a call's `status` tells.
 
 Tensors are device arrays of anything that has data_ptr(), shape, stride() and dtype (torch tensors do); they are used in place, on the calling thread's
 device (init / init_thread).  A process that uses torch imports it before this package: the one HIP runtime is then torch's.
@@ -18,6 +19,7 @@ from . import AtlasError, _check, lib
 ONE = 1 << 14                       # scale 2^14; the score_mul that scales nothing
 LIBRARY_STREAM = "library"          # stream=
 NARROW, BAD_SLOT = 1, 2             # KVCache.write's status
+MASK_WEIGHS = 1                     # Attention.prompt's and .cached's status
 NO_BLOCKS, NO_COLUMNS, NO_TOKENS, BAD_LENGTH = 1, 2, 4, 8      # Pager.plan's status
 
 
@@ -33,11 +35,17 @@ class _Cache(C.Structure):
     _fields_ = [("d_k", C.c_void_p), ("d_v", C.c_void_p), ("n_blocks", C.c_size_t), ("block_size", C.c_size_t), ("bits", C.c_int32)]
 
 
-_vp, _sz, _R, _S, _K = C.c_void_p, C.c_size_t, C.POINTER(_Rows), C.POINTER(_Shape), C.POINTER(_Cache)
+class _Mask(C.Structure):
+    _fields_ = [("fill", C.c_int32), ("n_tokens", C.c_uint32), ("d_status", C.c_void_p)]
+
+
+_vp, _sz, _R, _S, _K, _M = C.c_void_p, C.c_size_t, C.POINTER(_Rows), C.POINTER(_Shape), C.POINTER(_Cache), C.POINTER(_Mask)
 lib.atlas_attn_prompt_workspace.argtypes, lib.atlas_attn_prompt_workspace.restype = [_S, _sz, _sz], _sz
 lib.atlas_attn_prompt.argtypes, lib.atlas_attn_prompt.restype = [_S, _R, _R, _R, _vp, _sz, _sz, _R, _vp, _sz, _vp], C.c_int
 lib.atlas_attn_cached_workspace.argtypes, lib.atlas_attn_cached_workspace.restype = [_S, _sz, _sz, _K, _sz], _sz
 lib.atlas_attn_cached.argtypes, lib.atlas_attn_cached.restype = [_S, _R, _vp, _vp, _sz, _sz, _K, _vp, _sz, _sz, _R, _vp, _sz, _vp], C.c_int
+lib.atlas_attn_prompt_masked.argtypes, lib.atlas_attn_prompt_masked.restype = [_S, _R, _R, _R, _vp, _sz, _sz, _R, _M, _vp, _sz, _vp], C.c_int
+lib.atlas_attn_cached_masked.argtypes, lib.atlas_attn_cached_masked.restype = [_S, _R, _vp, _vp, _sz, _sz, _K, _vp, _sz, _sz, _R, _M, _vp, _sz, _vp], C.c_int
 lib.atlas_kv_write.argtypes, lib.atlas_kv_write.restype = [_S, _R, _R, _vp, _sz, _K, _vp, _vp], C.c_int
 lib.atlas_kv_plan_workspace.argtypes, lib.atlas_kv_plan_workspace.restype = [_sz, _sz], _sz
 lib.atlas_kv_plan.argtypes, lib.atlas_kv_plan.restype = [_sz, _sz, _vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp], C.c_int
@@ -148,13 +156,20 @@ class KVCache:
 
 
 class Attention:
-    """score_mul: the Mul node's constant at scale 2^14 (round(2^14 / sqrt(head_dim)) is the usual; ONE: the graph has no such node)"""
+    """score_mul: the Mul node's constant at scale 2^14 (round(2^14 / sqrt(head_dim)) is the usual; ONE: the graph has no such node).
+    mask_fill, mask_tokens: what the graph's Iff fills masked scores with, and the graph's tokens; a call with a `status` then tells whether masked keys
+    would weigh in the graph"""
 
-    def __init__(self, n_heads, n_kv_heads, head_dim, score_mul=ONE, causal=True):
+    def __init__(self, n_heads, n_kv_heads, head_dim, score_mul=ONE, causal=True, mask_fill=None, mask_tokens=None):
         if not -(1 << 31) <= score_mul < 1 << 31:              # ctypes would cut it to 32 bits
             raise ValueError(f"Attention: score_mul must be 1 .. 2^14, got {score_mul}")
         self.n_heads, self.n_kv_heads, self.head_dim = n_heads, n_kv_heads, head_dim
         self.shape = _Shape(n_heads, n_kv_heads, head_dim, score_mul, 1 if causal else 0)
+        if (mask_fill is None) != (mask_tokens is None):
+            raise ValueError("Attention: mask_fill and mask_tokens belong together")
+        if mask_fill is not None and not (-(1 << 31) <= mask_fill < 1 << 31 and 1 <= mask_tokens < 1 << 31):
+            raise ValueError(f"Attention: mask_fill must fit 32 bits, mask_tokens must be 1 .. 2^31 - 1, got {mask_fill}, {mask_tokens}")
+        self.mask_fill, self.mask_tokens = mask_fill, mask_tokens
 
     def prompt_workspace_bytes(self, n_seqs, n_tokens):
         return self._size(lib.atlas_attn_prompt_workspace(C.byref(self.shape), n_seqs, n_tokens))
@@ -168,19 +183,27 @@ class Attention:
             raise AtlasError("attention: the shape, the cache or the sizes are not supported")
         return n
 
-    def prompt(self, q, k, v, cu_seqlens, out, workspace, stream=None):
-        """q, out [tokens][n_heads][head_dim], k, v [tokens][n_kv_heads][head_dim], cu_seqlens int32 [n_seqs + 1]; returns out"""
+    def _mask(self, status):
+        if self.mask_fill is None:
+            raise ValueError("Attention: a status needs mask_fill and mask_tokens")
+        return C.byref(_Mask(self.mask_fill, self.mask_tokens, _status(status)))
+
+    def prompt(self, q, k, v, cu_seqlens, out, workspace, stream=None, status=None):
+        """q, out [tokens][n_heads][head_dim], k, v [tokens][n_kv_heads][head_dim], cu_seqlens int32 [n_seqs + 1]; returns out.  status: one uint32 / int32 on
+        the device that gets MASK_WEIGHS ored in when the graph's masked keys would weigh in some row, so that its trace may be another"""
         n, n_seqs = q.shape[0], cu_seqlens.shape[0] - 1
         if n_seqs < 0 or not (k.shape[0] == v.shape[0] == out.shape[0] == n):
             raise ValueError("Attention.prompt: q, k, v and out have the same number of rows, cu_seqlens one entry more than sequences")
         p, size = _workspace(workspace)
-        _check(lib.atlas_attn_prompt(C.byref(self.shape), C.byref(_rows(q, "q", self.n_heads, self.head_dim)), C.byref(_rows(k, "k", self.n_kv_heads, self.head_dim)),
-                                     C.byref(_rows(v, "v", self.n_kv_heads, self.head_dim)), _vector(cu_seqlens, "cu_seqlens", "int32"), n_seqs, n,
-                                     C.byref(_rows(out, "out", self.n_heads, self.head_dim)), p, size, _stream(stream, q)))
+        call, mask = (lib.atlas_attn_prompt, ()) if status is None else (lib.atlas_attn_prompt_masked, (self._mask(status),))
+        _check(call(C.byref(self.shape), C.byref(_rows(q, "q", self.n_heads, self.head_dim)), C.byref(_rows(k, "k", self.n_kv_heads, self.head_dim)),
+                    C.byref(_rows(v, "v", self.n_kv_heads, self.head_dim)), _vector(cu_seqlens, "cu_seqlens", "int32"), n_seqs, n,
+                    C.byref(_rows(out, "out", self.n_heads, self.head_dim)), *mask, p, size, _stream(stream, q)))
         return out
 
-    def cached(self, q, cu_new, kv_lens, cache, block_table, out, workspace, stream=None):
-        """q, out [new tokens][n_heads][head_dim], cu_new int32 [n_seqs + 1], kv_lens int32 [n_seqs], block_table int32 [n_seqs][columns]; returns out"""
+    def cached(self, q, cu_new, kv_lens, cache, block_table, out, workspace, stream=None, status=None):
+        """q, out [new tokens][n_heads][head_dim], cu_new int32 [n_seqs + 1], kv_lens int32 [n_seqs], block_table int32 [n_seqs][columns]; returns out.
+        status: as for prompt"""
         n, n_seqs = q.shape[0], cu_new.shape[0] - 1
         if (cache.n_kv_heads, cache.head_dim) != (self.n_kv_heads, self.head_dim):
             raise ValueError("Attention.cached: the cache has other heads")
@@ -188,9 +211,10 @@ class Attention:
             raise ValueError("Attention.cached: q and out have the same number of rows, cu_new one entry more than sequences, the table a row for each")
         p, size = _workspace(workspace)
         table, cols, stride = _table(block_table)
-        _check(lib.atlas_attn_cached(C.byref(self.shape), C.byref(_rows(q, "q", self.n_heads, self.head_dim)), _vector(cu_new, "cu_new", "int32"),
-                                     _vector(kv_lens, "kv_lens", "int32", n_seqs), n_seqs, n, C.byref(cache.desc), table, cols, stride,
-                                     C.byref(_rows(out, "out", self.n_heads, self.head_dim)), p, size, _stream(stream, q)))
+        call, mask = (lib.atlas_attn_cached, ()) if status is None else (lib.atlas_attn_cached_masked, (self._mask(status),))
+        _check(call(C.byref(self.shape), C.byref(_rows(q, "q", self.n_heads, self.head_dim)), _vector(cu_new, "cu_new", "int32"),
+                    _vector(kv_lens, "kv_lens", "int32", n_seqs), n_seqs, n, C.byref(cache.desc), table, cols, stride,
+                    C.byref(_rows(out, "out", self.n_heads, self.head_dim)), *mask, p, size, _stream(stream, q)))
         return out
 
 

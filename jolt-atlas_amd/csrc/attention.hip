@@ -12,12 +12,14 @@ namespace {
 using namespace atlas_attn;
 
 Rows rows_of(const atlas_attn_rows_t* r) { return Rows{r->d, (int64_t)r->token_stride, (int64_t)r->head_stride}; }
-Args args_of(const atlas_attn_shape_t* s, const atlas_attn_rows_t* q, const int32_t* cu, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t* out) {
+Args args_of(const atlas_attn_shape_t* s, const atlas_attn_rows_t* q, const int32_t* cu, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t* out,
+             const atlas_attn_mask_t* mask) {
     Args A{};
     A.q = rows_of(q); A.out = rows_of(out);
     A.cu = cu; A.n_seqs = (uint32_t)n_seqs; A.n_tokens = (uint32_t)n_tokens;
     A.H = (uint32_t)s->n_heads; A.KV = (uint32_t)s->n_kv_heads; A.G = A.H / A.KV; A.d = (uint32_t)s->head_dim;
     A.mul = s->score_mul; A.causal = s->causal;
+    if (mask) { A.fill = mask->fill; A.graph_tokens = mask->n_tokens; A.status = mask->d_status; }
     return A;
 }
 
@@ -186,20 +188,9 @@ int launch_fused(const Args& A, size_t max_keys, hipStream_t stream) {
     return rc;
 }
 
-}  // namespace
-
-extern "C" {
-
-size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens) {
-    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_count(shape, n_tokens)) return 0;
-    const Path path = path_of(shape, n_seqs, n_tokens, n_tokens, true);
-    if (too_many(shape, n_seqs, n_tokens, n_tokens, false, path)) return 0;
-    return path == Path::FUSED ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
-}
-
-int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
-                      const int32_t* d_cu_seqlens, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t* out, void* d_workspace, size_t workspace_bytes,
-                      void* stream) {
+int attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
+                const int32_t* d_cu_seqlens, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t* out,
+                const atlas_attn_mask_t* mask, void* d_workspace, size_t workspace_bytes, void* stream) {
     const char* why = bad_shape(shape);
     if (!why) why = bad_sizes(n_seqs, n_tokens);
     if (!why) why = bad_count(shape, n_tokens);
@@ -214,12 +205,13 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     const Path path = why ? Path::FUSED : path_of(shape, n_seqs, n_tokens, n_tokens, true);
     if (!why) why = too_many(shape, n_seqs, n_tokens, n_tokens, false, path);
     if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < atlas_attn_prompt_workspace(shape, n_seqs, n_tokens))) why = "attn_prompt: workspace is null, unaligned or too small";
+    if (!why && mask) why = bad_mask(shape, mask);
     if (why) return fail(ATLAS_EINVAL, why);
     if (!n_seqs || !n_tokens) return ATLAS_OK;
     Launch L;
     if (int rc = L.begin(stream)) return rc;
-    if (int rc = L.on_device({q->d, k->d, v->d, d_cu_seqlens, out->d, d_workspace})) return rc;
-    Args A = args_of(shape, q, d_cu_seqlens, n_seqs, n_tokens, out);
+    if (int rc = L.on_device({q->d, k->d, v->d, d_cu_seqlens, out->d, d_workspace, mask ? mask->d_status : nullptr})) return rc;
+    Args A = args_of(shape, q, d_cu_seqlens, n_seqs, n_tokens, out, mask);
     A.k = rows_of(k); A.v = rows_of(v);
     if (path == Path::FUSED) {
         if (int rc = launch_fused<int32_t>(A, n_tokens, L.stream)) return rc;
@@ -230,17 +222,9 @@ int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     return L.end();
 }
 
-size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
-    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_count(shape, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
-    const size_t max_keys = max_blocks * cache->block_size;
-    const Path path = path_of(shape, n_seqs, n_tokens, max_keys, many_rows(shape, n_seqs, n_tokens));
-    if (too_many(shape, n_seqs, n_tokens, max_keys, true, path)) return 0;
-    return most_bytes(shape, n_seqs, n_tokens, max_keys);
-}
-
-int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const int32_t* d_cu_new, const int32_t* d_kv_lens, size_t n_seqs, size_t n_tokens,
-                      const atlas_kv_cache_t* cache, const int32_t* d_block_table, size_t max_blocks, size_t table_stride, const atlas_attn_rows_t* out,
-                      void* d_workspace, size_t workspace_bytes, void* stream) {
+int attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const int32_t* d_cu_new, const int32_t* d_kv_lens, size_t n_seqs, size_t n_tokens,
+                const atlas_kv_cache_t* cache, const int32_t* d_block_table, size_t max_blocks, size_t table_stride, const atlas_attn_rows_t* out,
+                const atlas_attn_mask_t* mask, void* d_workspace, size_t workspace_bytes, void* stream) {
     const char* why = bad_shape(shape);
     if (!why) why = bad_sizes(n_seqs, n_tokens);
     if (!why) why = bad_count(shape, n_tokens);
@@ -255,12 +239,13 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     const Path path = why ? Path::FUSED : path_of(shape, n_seqs, n_tokens, max_blocks * cache->block_size, many_rows(shape, n_seqs, n_tokens));
     if (!why) why = too_many(shape, n_seqs, n_tokens, max_blocks * cache->block_size, true, path);
     if (!why && (!d_workspace || (uintptr_t)d_workspace % 16 || workspace_bytes < cached_bytes(shape, n_seqs, n_tokens, max_blocks * cache->block_size, path))) why = "attn_cached: workspace is null, unaligned or too small";
+    if (!why && mask) why = bad_mask(shape, mask);
     if (why) return fail(ATLAS_EINVAL, why);
     if (!n_seqs || !n_tokens) return ATLAS_OK;
     Launch L;
     if (int rc = L.begin(stream)) return rc;
-    if (int rc = L.on_device({q->d, d_cu_new, d_kv_lens, cache->d_k, cache->d_v, d_block_table, out->d, d_workspace})) return rc;
-    Args A = args_of(shape, q, d_cu_new, n_seqs, n_tokens, out);
+    if (int rc = L.on_device({q->d, d_cu_new, d_kv_lens, cache->d_k, cache->d_v, d_block_table, out->d, d_workspace, mask ? mask->d_status : nullptr})) return rc;
+    Args A = args_of(shape, q, d_cu_new, n_seqs, n_tokens, out, mask);
     // a table without columns (nothing is cached, its array may be empty) is never looked at
     A.ck = cache->d_k; A.cv = cache->d_v; A.lens = d_kv_lens; A.table = max_blocks ? d_block_table : d_kv_lens; A.table_stride = (int64_t)table_stride;
     A.n_blocks = (uint32_t)cache->n_blocks; A.log_block = log2_of(cache->block_size); A.max_keys = (uint32_t)(max_blocks * cache->block_size);
@@ -276,6 +261,49 @@ int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* 
     const SplitLayout P(shape, n_seqs, n_tokens, A.max_keys, d_workspace);
     if (int rc = cache->bits == 16 ? launch_split<int16_t>(A, P, L.stream) : launch_split<int32_t>(A, P, L.stream)) return rc;
     return L.end();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t atlas_attn_prompt_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens) {
+    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_count(shape, n_tokens)) return 0;
+    const Path path = path_of(shape, n_seqs, n_tokens, n_tokens, true);
+    if (too_many(shape, n_seqs, n_tokens, n_tokens, false, path)) return 0;
+    return path == Path::FUSED ? 16 : PlanesLayout(shape, n_seqs, n_tokens, 0).bytes;
+}
+
+int atlas_attn_prompt(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
+                      const int32_t* d_cu_seqlens, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t* out, void* d_workspace, size_t workspace_bytes,
+                      void* stream) {
+    return attn_prompt(shape, q, k, v, d_cu_seqlens, n_seqs, n_tokens, out, nullptr, d_workspace, workspace_bytes, stream);
+}
+int atlas_attn_prompt_masked(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const atlas_attn_rows_t* k, const atlas_attn_rows_t* v,
+                             const int32_t* d_cu_seqlens, size_t n_seqs, size_t n_tokens, const atlas_attn_rows_t* out, const atlas_attn_mask_t* mask, void* d_workspace, size_t workspace_bytes,
+                             void* stream) {
+    if (!mask) return fail(ATLAS_EINVAL, "attn_prompt: mask is null");
+    return attn_prompt(shape, q, k, v, d_cu_seqlens, n_seqs, n_tokens, out, mask, d_workspace, workspace_bytes, stream);
+}
+
+size_t atlas_attn_cached_workspace(const atlas_attn_shape_t* shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t* cache, size_t max_blocks) {
+    if (bad_shape(shape) || bad_sizes(n_seqs, n_tokens) || bad_count(shape, n_tokens) || bad_cache(cache) || max_blocks > 0x7fffffff / cache->block_size) return 0;
+    const size_t max_keys = max_blocks * cache->block_size;
+    const Path path = path_of(shape, n_seqs, n_tokens, max_keys, many_rows(shape, n_seqs, n_tokens));
+    if (too_many(shape, n_seqs, n_tokens, max_keys, true, path)) return 0;
+    return most_bytes(shape, n_seqs, n_tokens, max_keys);
+}
+
+int atlas_attn_cached(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const int32_t* d_cu_new, const int32_t* d_kv_lens, size_t n_seqs, size_t n_tokens,
+                      const atlas_kv_cache_t* cache, const int32_t* d_block_table, size_t max_blocks, size_t table_stride, const atlas_attn_rows_t* out,
+                      void* d_workspace, size_t workspace_bytes, void* stream) {
+    return attn_cached(shape, q, d_cu_new, d_kv_lens, n_seqs, n_tokens, cache, d_block_table, max_blocks, table_stride, out, nullptr, d_workspace, workspace_bytes, stream);
+}
+int atlas_attn_cached_masked(const atlas_attn_shape_t* shape, const atlas_attn_rows_t* q, const int32_t* d_cu_new, const int32_t* d_kv_lens, size_t n_seqs, size_t n_tokens,
+                             const atlas_kv_cache_t* cache, const int32_t* d_block_table, size_t max_blocks, size_t table_stride, const atlas_attn_rows_t* out,
+                             const atlas_attn_mask_t* mask, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (!mask) return fail(ATLAS_EINVAL, "attn_cached: mask is null");
+    return attn_cached(shape, q, d_cu_new, d_kv_lens, n_seqs, n_tokens, cache, d_block_table, max_blocks, table_stride, out, mask, d_workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

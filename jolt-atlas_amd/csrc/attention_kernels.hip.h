@@ -21,6 +21,10 @@ struct Args {
     uint32_t n_blocks, log_block, max_keys;
     uint32_t n_seqs, n_tokens, H, KV, G, d;
     int32_t mul, causal;
+    // asked whether the graph's masked keys would weigh: their score (the graph's fill), the graph's tokens, where to tell (nullptr: not asked)
+    int32_t fill;
+    uint32_t graph_tokens;
+    uint32_t* status;
 };
 
 struct Seq { uint32_t begin, n_new, keys, idx; };      // its first row of q, its new tokens, its keys
@@ -62,6 +66,13 @@ __device__ inline uint32_t exp_lds(uint32_t z, const uint32_t* s_hi, const uint3
 }
 // sums of e saturate: from 2^28 + 1 on the reciprocal floor(2^28 / sum) is 0 whatever the sum
 __device__ inline uint32_t add_sat(uint32_t a, uint32_t b) { const uint32_t s = a + b; return s < a ? 0xffffffffu : s; }
+
+// Row i of a sequence, whose maximum is m: in a graph of graph_tokens tokens the keys behind it are there, with the fill as their score.  They carry no weight, as
+// here, where their e is 0 and the fill is not the maximum itself; otherwise the graph's row may be another.
+__device__ inline bool mask_weighs(const Args& A, const Seq& s, uint32_t i, int32_t m) {
+    if ((int64_t)s.keys - s.n_new + i + 1 >= A.graph_tokens) return false;
+    return A.fill > m || exp_q((uint32_t)m - (uint32_t)A.fill, g_exp.hi, g_exp.lo) > 0;
+}
 
 // ---- any operands: a workgroup takes one (token, head), 64-bit products one by one, the scores recomputed in each of the three passes.
 // The softmax's floors are taken under the FINAL maximum and sum, so partial results cannot be rescaled as a float softmax's are: a pass for the
@@ -105,6 +116,7 @@ __device__ void row_exact(const Args& A, const Seq& s, uint32_t i, uint32_t h, i
     const uint64_t sum = s_red[0];
     __syncthreads();
     const uint32_t inv = sum ? (uint32_t)((1ull << (2 * SCALE)) / sum) : 0;
+    if (A.status && tid == 0 && sum && mask_weighs(A, s, i, (int32_t)m)) atomicOr(A.status, (uint32_t)ATLAS_ATTN_MASK_WEIGHS);
     uint64_t acc = 0;
     for (uint32_t j0 = 0; j0 < limit; j0 += NT) {
         const uint32_t j = j0 + tid;

@@ -45,6 +45,12 @@ inline bool unaligned(std::initializer_list<const void*> ps) {          // int32
     for (const void* p : ps) if ((uintptr_t)p % 4) return true;
     return false;
 }
+inline const char* bad_mask(const atlas_attn_shape_t* s, const atlas_attn_mask_t* m) {
+    if (!m || !m->d_status || unaligned({m->d_status})) return "attention: mask or its status is null or not 4-byte aligned";
+    if (m->n_tokens < 1 || m->n_tokens > 0x7fffffff) return "attention: a mask's n_tokens must be 1 .. 2^31 - 1";
+    if (!s->causal) return "attention: a graph's mask is causal";
+    return nullptr;
+}
 inline uint32_t log2_of(size_t v) { uint32_t l = 0; while (((size_t)1 << l) < v) l++; return l; }
 
 // Enqueues on the caller's stream, or on the library's: that one under its lock (another thread's pipeline may have it on a lane).  The calling thread's

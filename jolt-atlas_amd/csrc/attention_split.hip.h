@@ -340,6 +340,7 @@ __global__ __launch_bounds__(FUSED_WAVES * 64, 2) void k_attn_fused(Args A, uint
 #pragma unroll
     for (uint32_t w = 0; w < FUSED_WAVES; w++) sum += s_s[w][l];       // <= 2^25
     const uint32_t inv = m == GONE ? 0 : (1u << (2 * SCALE)) / sum;       // a row that sees no key: no weights
+    if (A.status && wave == 0 && g == 0 && mine && !exact && m != GONE && mask_weighs(A, R.s, r / A.G, m)) atomicOr(A.status, (uint32_t)ATLAS_ATTN_MASK_WEIGHS);
     // up to 128 dims the sums take the scores' place; more dims are two sweeps over the weights, their sums lie behind the scores
     constexpr int VS = value_steps(KS);
     unsigned long long* s_o = (unsigned long long*)(s_x + (KS > 2 ? TILE_ROWS * pitch : 0));
@@ -606,7 +607,9 @@ __global__ __launch_bounds__(JOIN) void k_split_join(Args A, Split S, uint32_t d
     __shared__ uint32_t s_mag[3];
     __shared__ int32_t s_q[JOIN], s_p[JOIN];
     __shared__ uint64_t s_red[JOIN];
+    __shared__ int32_t s_m;
     if (tid < 3) s_mag[tid] = 0;
+    if (tid == 3) s_m = GONE;
     __syncthreads();
     const uint32_t per = S.units[tile + 1] - S.units[tile], n = S.rows[tile + 1] - S.rows[tile];
     const uint32_t y = tid & (dp - 1), parts = JOIN / dp;
@@ -617,6 +620,8 @@ __global__ __launch_bounds__(JOIN) void k_split_join(Args A, Split S, uint32_t d
         uint32_t mq = 0, mk = 0, mv = 0;
         for (uint32_t w = w0 + tid; w <= w1; w += JOIN) { mq |= S.q_mag[w + mag]; mk |= S.k_mag[w + mag]; mv |= S.v_mag[w + mag]; }
         if (mq | mk | mv) { atomicOr(&s_mag[0], mq); atomicOr(&s_mag[1], mk); atomicOr(&s_mag[2], mv); }
+        if (A.status)
+            for (uint32_t w = w0 + tid; w <= w1; w += JOIN) atomicMax(&s_m, S.cmax[w * TILE_ROWS + S.rows[tile] * A.KV + kvh * n + r]);
         const int64_t* from = S.part + (int64_t)(S.rows[tile] * A.KV + kvh * n + r) * A.d + y;
         if (y < A.d)
 #pragma unroll 4
@@ -629,6 +634,7 @@ __global__ __launch_bounds__(JOIN) void k_split_join(Args A, Split S, uint32_t d
         row_exact<CT, JOIN>(A, s, t - s.begin, h, s_q, s_p, s_red);
         return;
     }
+    if (A.status && tid == 0 && s_m != GONE && mask_weighs(A, s, t - s.begin, s_m)) atomicOr(A.status, (uint32_t)ATLAS_ATTN_MASK_WEIGHS);
     if (tid < A.d) {
         for (uint32_t p = 1; p < parts; p++) sum += (int64_t)s_red[p * dp + tid];
         A.out.d[(int64_t)t * A.out.ts + (int64_t)h * A.out.hs + tid] = (int32_t)(sum >> SCALE);

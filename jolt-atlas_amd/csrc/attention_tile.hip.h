@@ -441,6 +441,7 @@ __global__ __launch_bounds__(256, (TileShape<DP, SPLIT>::WAVES)) void k_attn_til
             if (what == MAX) m = rescale(m, A.mul);
         }
         const uint32_t inv = sum ? (1u << (2 * SCALE)) / sum : 0;
+        if (A.status && part == 0 && half == 0 && mine && sum && mask_weighs(A, s, tok, m)) atomicOr(A.status, (uint32_t)ATLAS_ATTN_MASK_WEIGHS);
 
         // ---- the weights from the e that are held, and their product with the values.  o[.][f]: the sums with the values' digit 0, 1, 2
         v16i o0[T::OF] = {}, o1[T::OF] = {}, o2[T::OF] = {};

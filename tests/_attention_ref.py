@@ -45,6 +45,28 @@ def prompt(q, k, v, lens, score_mul=ONE, causal=True):
     return out
 
 
+def mask_weighs(q, k, limits, positions, score_mul, fill, tokens):
+    """whether a key behind some row's own, whose score is `fill` in a graph of `tokens` tokens, would have a weight or be the maximum there"""
+    hi, lo = exp_tables()
+    n, H, d = q.shape
+    G = H // k.shape[1]
+    for h in range(H):
+        kk = k[:, h // G].astype(np.int64)
+        for i in range(n):
+            see = limits[i]
+            if np.ndim(see) == 0:
+                see = np.arange(len(kk)) < see
+            if not see.any() or positions[i] + 1 >= tokens:
+                continue
+            with np.errstate(over="ignore"):
+                x = np.clip((kk[see] * q[i, h].astype(np.int64)[None, :]).sum(axis=1) >> 14, LO, HI)
+            m = int(np.clip((x * score_mul) >> 14, LO, HI).max())
+            z = min(max(m - fill, 0), (1 << 18) - 1)
+            if fill > m or (int(hi[z >> 9]) * int(lo[z & 511])) >> 14:
+                return True
+    return False
+
+
 def plan(have, new, table, free, n_free, block, n_blocks, cap):
     """the step's outputs, on copies"""
     table, free = table.copy(), free.copy()

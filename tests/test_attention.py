@@ -365,3 +365,73 @@ def test_the_stream_of_torch_tensors(monkeypatch):
     now.cuda_stream = 0
     assert streams(Tensor) == 1 and streams(Tensor, stream=5) == 5 and streams(Tensor, stream=0) == 1 and streams(Fake, stream=9) == 9
     assert streams(Tensor, stream=T.LIBRARY_STREAM) is None and streams(Fake, stream=T.LIBRARY_STREAM) is None
+
+
+def graph_attention(name):
+    """the attention layers of one of the framework's graphs at its example input, run by the oracle's executor: q, k, v, the Mul constant, the Iff's fill, the output"""
+    from tools import build_graphs
+    from oracle import graph as OG
+    nodes, _, inputs = getattr(build_graphs, name)()
+    outs, _ = OG.execute(nodes, inputs)
+    by = {nd["idx"]: nd for nd in nodes}
+    for nd in nodes:
+        if nd["op"] != "SoftmaxLastAxis":
+            continue
+        iff = by[nd["inputs"][0]]
+        att, mul = by[iff["inputs"][1]], 1 << 14
+        if att["op"] == "Mul":
+            mul, att = int(outs[att["inputs"][1]].flat[0]), by[att["inputs"][0]]
+        y = next(x for x in nodes if x["op"] == "Einsum" and x["inputs"][0] == nd["idx"])
+        shape = (nd["dims"][1], nd["dims"][0], -1)
+        yield tuple(np.ascontiguousarray(outs[i].reshape(shape)) for i in (*att["inputs"], y["inputs"][1])), mul, int(outs[iff["inputs"][2]].flat[0]), outs[y["idx"]].reshape(shape)
+
+
+@pytest.mark.parametrize("name,fill,weighs", [("microgpt_model", -10, False), ("nanogpt_model", -10, False), ("nanogpt", -10, True), ("gpt2_layer", -8, True)])
+def test_where_the_reference_is_the_frameworks_graphs(name, fill, weighs):
+    """the framework's own graphs, whose mask fill is near: the same rows where no masked key weighs, and told where one does"""
+    from _attention_ref import mask_weighs, prompt
+    told = False
+    for (q, k, v), mul, f, want in graph_attention(name):
+        n = len(q)
+        assert f == fill << 14
+        got = prompt(q, k, v, [n], mul)
+        for i in range(n):
+            tell = mask_weighs(q[i:i + 1], k, [i + 1], [i], mul, f, n)
+            assert tell or np.array_equal(got[i], want[i]), i
+            told |= tell
+    assert told == weighs
+
+
+def _masked(mask=None, status=Fake((1,)), **kw):
+    import jolt_atlas_amd.attention as T
+    at, ws = T.Attention(4, 2, 8, mask_fill=-(10 << 14), mask_tokens=64, **kw), Fake((1 << 22,), "uint8")
+    calls = [lambda: at.prompt(Fake((5, 4, 8)), Fake((5, 2, 8)), Fake((5, 2, 8)), Fake((3,)), Fake((5, 4, 8), ptr=1 << 41), ws, status=status),
+             lambda: at.cached(Fake((3, 4, 8)), Fake((3,)), Fake((2,)), T.KVCache(*(Fake((7, 2, 16, 8)) for _ in range(2))), Fake((2, 5)), Fake((3, 4, 8), ptr=1 << 41), ws, status=status)]
+    return calls
+
+
+def test_mask_refusals():
+    import jolt_atlas_amd as A
+    import jolt_atlas_amd.attention as T
+    for kw, why in ((dict(status=Fake((1,), ptr=0)), "status is null"), (dict(status=Fake((1,), ptr=(1 << 40) + 2)), "4-byte"), (dict(causal=False), "causal")):
+        for f in _masked(**kw):
+            with pytest.raises(A.AtlasError, match=why):
+                f()
+    for f in _masked(status=Fake((1,), "int64")) + _masked(status=Fake((0,))):
+        with pytest.raises(ValueError, match="status"):
+            f()
+    for kw in (dict(mask_fill=-5), dict(mask_tokens=64), dict(mask_fill=1 << 31, mask_tokens=64), dict(mask_fill=0, mask_tokens=0), dict(mask_fill=0, mask_tokens=1 << 31)):
+        with pytest.raises(ValueError, match="mask"):
+            T.Attention(4, 2, 8, **kw)
+    at = T.Attention(4, 2, 8)
+    with pytest.raises(ValueError, match="mask_fill"):
+        at.prompt(Fake((5, 4, 8)), Fake((5, 2, 8)), Fake((5, 2, 8)), Fake((3,)), Fake((5, 4, 8), ptr=1 << 41), Fake((1 << 22,), "uint8"), status=Fake((1,)))
+    null, rows, cache = C.POINTER(T._Mask)(), T._Rows(1 << 40, 32, 8), T.KVCache(*(Fake((7, 2, 16, 8)) for _ in range(2)))
+    assert A.lib.atlas_attn_prompt_masked(C.byref(at.shape), *[C.byref(rows)] * 3, 1 << 40, 1, 1, C.byref(T._Rows(1 << 41, 32, 8)), null, 1 << 40, 1 << 22, None) != 0
+    assert A.lib.atlas_attn_cached_masked(C.byref(at.shape), C.byref(rows), 1 << 40, 1 << 40, 1, 1, C.byref(cache.desc), 1 << 40, 1, 1, C.byref(T._Rows(1 << 41, 32, 8)), null,
+                                          1 << 40, 1 << 22, None) != 0
+    assert "mask" in A.lib.atlas_last_error().decode()
+    for n in (0, 1 << 31):
+        m = T._Mask(0, n, 1 << 40)
+        assert A.lib.atlas_attn_prompt_masked(C.byref(at.shape), *[C.byref(rows)] * 3, 1 << 40, 1, 1, C.byref(T._Rows(1 << 41, 32, 8)), C.byref(m), 1 << 40, 1 << 22, None) != 0
+        assert "n_tokens" in A.lib.atlas_last_error().decode()

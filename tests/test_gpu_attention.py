@@ -5,7 +5,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from _attention_ref import ONE, attend, plan, prompt
+from _attention_ref import ONE, attend, mask_weighs, plan, prompt
 from _dev import Dev, hip, ok, workspace
 
 pytestmark = pytest.mark.gpu
@@ -820,6 +820,110 @@ def test_an_error_that_the_caller_left(atlas):
         f()
     want = prompt(q, k, v, [5])
     assert status.numpy()[0] == 0 and np.array_equal(out.numpy(), want) and np.array_equal(ck.numpy(), want)
+
+
+def masked_status(q, k, v, lens, mul, fill, tokens, steps, want):
+    """the status of a prompt and of the same rows over a cache (in `steps` new tokens each), through every kernel; both outputs are `want`"""
+    import jolt_atlas_amd.attention as T
+    n, H, d = q.shape
+    KV, B = k.shape[1], 16
+    at, plain, told = T.Attention(H, KV, d, mul, mask_fill=fill, mask_tokens=tokens), T.Attention(H, KV, d, mul), set()
+    word = lambda: Dev(np.array([1 << 30], np.uint32))  # noqa: E731
+    for rows in (n, 2100, 16500):
+        more = lambda x: Dev(np.concatenate([x, np.full((rows - n,) + x.shape[1:], 1 << 20, np.int32)]))  # noqa: E731
+        a = (more(q), more(k), more(v), Dev(np.cumsum([0] + lens).astype(np.int32)), Dev(np.zeros((rows, H, d), np.int32)), workspace(at.prompt_workspace_bytes(len(lens), rows)))
+        st = word()
+        assert np.array_equal(at.prompt(*a, status=st).numpy()[:n], want) and np.array_equal(plain.prompt(*a).numpy()[:n], want)
+        told.add(int(st.numpy()[0]))
+    up = [-(-x // B) for x in lens]
+    ck, cv = (np.zeros((sum(up) + 1, KV, B, d), np.int32) for _ in range(2))
+    table, base, first = np.full((len(lens), max(up)), -1, np.int32), 1, 0
+    for i, x in enumerate(lens):
+        table[i, :up[i]] = base + np.arange(up[i])
+        for c, src in ((ck, k), (cv, v)):
+            flat = np.zeros((up[i] * B, KV, d), np.int32)
+            flat[:x] = src[first:first + x]
+            c[base:base + up[i]] = flat.reshape(up[i], B, KV, d).transpose(0, 2, 1, 3)
+        base += up[i]
+        first += x
+    cache, at_row = T.KVCache(Dev(ck), Dev(cv)), np.cumsum([0] + lens)
+    for cols in (max(up), 70, 263, 1040):
+        wide, st, got = Dev(np.concatenate([table, np.full((len(lens), cols - max(up)), -1, np.int32)], axis=1)), word(), np.zeros_like(q)
+        for p in range(0, max(lens), steps):
+            new = [max(0, min(steps, x - p)) for x in lens]
+            sel = np.concatenate([at_row[i] + p + np.arange(m) for i, m in enumerate(new)]).astype(int)
+            out = Dev(np.zeros((len(sel), H, d), np.int32))
+            a = (Dev(q[sel]), Dev(np.cumsum([0] + new).astype(np.int32)), Dev(np.array([min(x, p + m) for x, m in zip(lens, new)], np.int32)), cache, wide, out,
+                 workspace(at.cached_workspace_bytes(len(lens), len(sel), cache, cols)))
+            got[sel] = at.cached(*a, status=st).numpy()
+            assert np.array_equal(plain.cached(*a).numpy(), got[sel])
+        assert np.array_equal(got, want), cols
+        told.add(int(st.numpy()[0]))
+    assert len(told) == 1 and told <= {1 << 30, 1 << 30 | T.MASK_WEIGHS}, told
+    return told == {1 << 30 | T.MASK_WEIGHS}
+
+
+def status_of(q, k, lens, mul, fill, tokens):
+    at = np.cumsum([0] + list(lens))
+    return any(mask_weighs(q[a:b], k[a:b], list(range(1, b - a + 1)), list(range(b - a)), mul, fill, tokens) for a, b in zip(at, at[1:]))
+
+
+@pytest.mark.parametrize("H,KV,d,steps", [(2, 1, 16, 9), (4, 2, 64, 1), (2, 2, 128, 40), (3, 1, 33, 40), (8, 1, 256, 7), (2, 1, 200, 40)])
+@pytest.mark.parametrize("spoil", [None, "q", "v"])
+def test_a_mask_that_would_weigh(atlas, H, KV, d, steps, spoil):
+    """fills around every border of e: where it is 0, where it is 1 between zeros, the maximum itself, above; some of it in rows of operands of any size"""
+    rng = np.random.default_rng(d)
+    lens = [40, 1, 23]
+    n = sum(lens)
+    q, k, v = values(rng, (n, H, d), 0.5), values(rng, (n, KV, d), 0.5), values(rng, (n, KV, d))
+    if spoil == "q":
+        q[n - 5, 0, 0] = -(1 << 31)
+    if spoil == "v":
+        v[17, 0, d - 1] = (1 << 31) - 1
+    mul = int(round(ONE / np.sqrt(d)))
+    want = prompt(q, k, v, lens, mul)
+    # the least maximum of a row that has masked keys: the lowest fill that would be it
+    lo, hi = -(1 << 31), (1 << 31) - 1
+    while lo < hi:
+        mid = (lo + hi) // 2
+        if any(mask_weighs(q[a:a + m], k[a:a + m], list(range(1, m + 1)), list(range(m)), mul, mid, 64) for a, m in zip(np.cumsum([0] + lens), lens)):
+            hi = mid
+        else:
+            lo = mid + 1
+    seen = set()
+    for fill in (lo - 1, lo, lo + 511, lo + (1 << 18), -(1 << 31), (1 << 31) - 1):
+        expect = status_of(q, k, lens, mul, fill, 64)
+        seen.add(expect)
+        assert masked_status(q, k, v, lens, mul, fill, 64, steps, want) == expect, fill
+    assert seen == {False, True}
+    assert not masked_status(q, k, v, lens, mul, (1 << 31) - 1, 1, steps, want)                # a graph of one token has no masked keys
+
+
+@pytest.mark.parametrize("tokens", [23, 24, 39, 40, 41, 64])
+def test_the_last_token_of_a_graph_has_no_masked_keys(atlas, tokens):
+    rng = np.random.default_rng(tokens)
+    lens, mul = [40, 23], 2048
+    q, k, v = (values(rng, (63, h, 64)) for h in (4, 2, 2))
+    q[:39], q[40:] = k[:39].repeat(2, axis=1), k[40:].repeat(2, axis=1)                        # all rows high, but the 40th token of one sequence
+    q[39] = -k[:40].sum(axis=0, dtype=np.int64).clip(-(1 << 17), 1 << 17).repeat(2, axis=0).astype(np.int32)
+    want = prompt(q, k, v, lens, mul)
+    for fill in (-(10 << 14), 0, 1 << 20):
+        assert masked_status(q, k, v, lens, mul, fill, tokens, 8, want) == status_of(q, k, lens, mul, fill, tokens)
+
+
+@pytest.mark.parametrize("name,weighs", [("microgpt_model", False), ("nanogpt_model", False), ("nanogpt", True), ("gpt2_layer", True)])
+def test_attention_of_the_frameworks_graphs(atlas, name, weighs):
+    """the layers of the framework's own graphs, their fill -10 or -8: equal to the trace where the status stays clear, and told where it does not"""
+    from test_attention import graph_attention
+    told = False
+    for (q, k, v), mul, fill, trace in graph_attention(name):
+        n = len(q)
+        want = prompt(q, k, v, [n], mul)
+        tell = masked_status(q, k, v, [n], mul, fill, n, 5, want)
+        assert tell == status_of(q, k, [n], mul, fill, n)
+        assert tell or np.array_equal(want, trace)
+        told |= tell
+    assert told == weighs
 
 
 TORCH = """
