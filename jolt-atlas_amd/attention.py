@@ -112,7 +112,7 @@ def _table(t):
 
 def _status(t):
     """one 32-bit word that the kernels write: any array of at least one element"""
-    if _name(t.dtype) not in ("int32", "uint32") or 0 in tuple(t.shape):
+    if _name(t.dtype) not in ("int32", "uint32") or 0 in t.shape:
         raise ValueError(f"status: one int32 or uint32 expected, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -127,7 +127,9 @@ def _contiguous(t, name):
 
 
 def _workspace(w):
-    return w.data_ptr(), _contiguous(w, "workspace") * w.itemsize
+    shape = w.shape
+    n = shape[0] if len(shape) == 1 and w.stride()[0] == 1 else _contiguous(w, "workspace")
+    return w.data_ptr(), n * w.itemsize
 
 
 class KVCache:
