@@ -262,6 +262,41 @@ def test_cached_long(atlas, bits, new):
     assert np.array_equal(run_cached(q, ck, cv, table, keys, new, 2048), want_cached(q, ck, cv, table, flat, keys, new, 2048))
 
 
+# The split path lays the units of 256 keys of all row tiles and kv heads behind each other, and each workgroup has the same share of that line
+LINES = {
+    "one_unit_more_than_workgroups": (2, 1, 32, [4864] * 27, [1] * 27),                        # 513 units for 512 workgroups
+    "uneven_shares": (6, 2, 36, [3000, 517, 1, 0, 9000, 256, 257, 8200, 4095] * 5, [1, 2, 1, 1, 0, 1, 3, 1, 1] * 5),
+    "several_units": (4, 4, 16, [5000 - 37 * i for i in range(45)], [1] * 45),
+    "just_below_all_workgroups": (1, 1, 16, [16640] * 63, [1] * 63),                           # 4095 units for 512
+    "all_workgroups": (16, 8, 32, [2049 + 7 * i for i in range(64)], [1 if i % 9 else 0 for i in range(64)]),
+    "tiles_of_several_rows": (16, 2, 128, [4000, 900, 2500, 0, 3333] * 8, [5, 7, 0, 2, 9] * 8),
+    "many_sequences": (4, 2, 32, [(i * 37) % 611 for i in range(1500)], [(1, 1, 0, 2, 1)[i % 5] for i in range(1500)]),
+}
+
+
+@pytest.mark.parametrize("bits", [32, 16])
+@pytest.mark.parametrize("name", LINES)
+def test_cached_shares_of_several_units(atlas, name, bits):
+    import jolt_atlas_amd.attention as T
+    H, KV, d, keys, new = LINES[name]
+    rng = np.random.default_rng(len(keys) + bits)
+    G = H // KV
+    units = sum(-(-n * G // 16) * -(-k // 256) for k, n in zip(keys, new)) * KV
+    tiles = sum(-(-n * G // 16) for n in new)
+    assert {"one_unit_more_than_workgroups": units == 513, "uneven_shares": 512 < units < 4096 and units % 512, "several_units": 2048 < units < 4096, "just_below_all_workgroups": units == 4095,
+            "all_workgroups": units > 4096 and units % 1024, "tiles_of_several_rows": 2048 < units < 4096, "many_sequences": tiles > 1024}[name]
+    ck, cv, table, flat = paged(rng, keys, KV, d, 32, bits)
+    n = sum(new)
+    q, mul = values(rng, (n, H, d)), int(round(ONE / np.sqrt(d)))
+    got = run_cached(q, ck, cv, table, keys, new, mul, caps=(4200,))
+    at = np.cumsum([0] + new)
+    some = range(len(keys)) if len(keys) < 70 else sorted({0, 1, 2, 3, len(keys) - 1, *rng.integers(0, len(keys), 250).tolist()})
+    for i in some:
+        if new[i]:
+            limits = [max(0, keys[i] - new[i] + j + 1) for j in range(new[i])]
+            assert np.array_equal(got[at[i]:at[i + 1]], attend(q[at[i]:at[i + 1]], flat(ck, i), flat(cv, i), limits, mul)), (i, keys[i], new[i])
+
+
 def test_cached_pages_that_do_not_exist(atlas):
     """a table entry outside the cache holds no keys; keys behind the table's columns do not exist; lengths that make no sense give empty rows"""
     rng = np.random.default_rng(3)
@@ -800,6 +835,35 @@ def test_calls_of_two_threads(atlas):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not wrong
+
+
+def test_calls_of_two_threads_of_other_sizes(atlas):
+    """the scores of a short prompt stay in LDS: threads whose prompts need more and less of it do not take it from each other"""
+    import threading
+    import jolt_atlas_amd.attention as T
+    h, wrong = hip(), []
+    rng = np.random.default_rng(6)
+    start = threading.Barrier(4)
+
+    def work(rows):
+        try:
+            st = C.c_void_p()
+            ok(h.hipSetDevice(C.c_int(0)))
+            ok(h.hipStreamCreateWithFlags(C.byref(st), C.c_uint(1)))
+            at = T.Attention(1, 1, 64, 2048)
+            x, out, cu, ws = Dev(np.zeros((rows, 1, 64), np.int32)), Dev(np.zeros((rows, 1, 64), np.int32)), Dev(np.array([0, 3], np.int32)), workspace(at.prompt_workspace_bytes(1, rows))
+            start.wait()
+            for _ in range(1500):
+                at.prompt(x, x, x, cu, out, ws, stream=st.value)
+            ok(h.hipStreamSynchronize(st))
+            ok(h.hipStreamDestroy(st))
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in (2000, 1000, 1990, 1010)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong, wrong
 
 
 def test_an_error_that_the_caller_left(atlas):
