@@ -892,8 +892,9 @@ int atlas_attn_prompt(const atlas_attn_shape_t *shape, const atlas_attn_rows_t *
                       void *stream);
 /* Attention of new tokens over a paged cache that already holds their keys and values (atlas_kv_write): sequence i has the rows
  * [cu_new[i], cu_new[i + 1]) of q and out (one row: a decoding step; none: a request that pauses), they are the last of its kv_lens[i] keys; key j
- * lies in block block_table[i * table_stride + j / block_size] at j % block_size.  max_blocks columns of the table are looked at: keys beyond
- * max_blocks * block_size do not exist, nor do those of a block outside [0, n_blocks). */
+ * lies in block block_table[i * table_stride + j / block_size] at j % block_size.  max_blocks columns of the table are looked at: a longer kv_lens[i] is cut to
+ * max_blocks * block_size first, and the new tokens are then the last of the keys that are left.  The keys of a block outside [0, n_blocks) do not exist; the others keep
+ * their places.  A long chunk and many single tokens are faster as two calls: which kernels run goes by the average of rows to a sequence. */
 size_t atlas_attn_cached_workspace(const atlas_attn_shape_t *shape, size_t n_seqs, size_t n_tokens, const atlas_kv_cache_t *cache, size_t max_blocks);
 int atlas_attn_cached(const atlas_attn_shape_t *shape, const atlas_attn_rows_t *q, const int32_t *d_cu_new, const int32_t *d_kv_lens, size_t n_seqs, size_t n_tokens,
                       const atlas_kv_cache_t *cache, const int32_t *d_block_table, size_t max_blocks, size_t table_stride, const atlas_attn_rows_t *out,

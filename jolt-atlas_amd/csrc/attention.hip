@@ -84,7 +84,8 @@ int launch_tiles(const Args& A, const PlanesLayout& L, const Planes& P, hipStrea
 }
 // On average more than 96 query rows to a sequence and kv head: tiles; below, 16 rows at a time that read the cache themselves.  One MI355X, int32, 64 sequences of 2000
 // keys: 32 heads of 128 over 8, 16 new tokens (64 rows) 820 us in tiles and 833 us in 16 rows, 32 new tokens 961 and 1599 us; 16 heads of 64, 32 new
-// tokens (32 rows) 1346 and 581 us.
+// tokens (32 rows) 1346 and 581 us.  The host knows no sequence's own rows: where a few have many and many have few, all go one way (a chunk of 2000 tokens beside 63 single
+// tokens over up to 8191 keys, 32 heads of 128 over 8: 1774 us in one call, 256 + 647 in two).
 bool many_rows(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens) { return n_tokens * (s->n_heads / s->n_kv_heads) > 96 * n_seqs; }
 // Few rows: the workspace of the split path
 struct SplitLayout {
@@ -134,8 +135,9 @@ int launch_split(const Args& A, const SplitLayout& L, hipStream_t stream) {
 }
 
 // One launch while LDS holds the scores.  Few rows: up to 1024 keys, beyond that where there are workgroups enough for the chip (16 heads of 64, one token over
-// 1000 / 2000 keys: 27 / 42 us in one launch of 16 workgroups, 30 / 31 us in the split path's five; 16 such tokens over 2000 keys: 56 and 84 us).  Many rows: while
-// the 16-row workgroups fit the chip about once (16 heads of 64, a prompt of 512: 40 us and 55 us in tiles, of 1024: 92 and 85 us).
+// 1000 / 2000 keys: 28 / 42 us in one launch of 16 workgroups, 32 / 33 us in the split path's five; 16 such tokens over 2000 keys: 56 and 80 us; the rule does not
+// go by the heads: one token of 32 heads of 128 over 8 and 1000 keys takes 43 us in its 8 workgroups, 39 in five launches).  Many rows: while
+// the 16-row workgroups fit the chip about once (16 heads of 64, a prompt of 512: 39 us and 55 us in tiles, of 1024: 92 and 85 us).
 bool fused(const atlas_attn_shape_t* s, size_t n_seqs, size_t n_tokens, size_t max_keys, bool many) {
     const size_t wgs = (n_tokens * (s->n_heads / s->n_kv_heads) / TILE_ROWS + n_seqs) * s->n_kv_heads;
     if (max_keys > fused_keys(s->head_dim)) return false;

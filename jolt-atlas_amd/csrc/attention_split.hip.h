@@ -6,9 +6,9 @@
 // k_split_scores, k_split_sums and k_split_values give each of WGS workgroups the same share of that line, wherever sequences begin and end; k_split_join adds the
 // shares of a row up.  Splitting costs nothing in exactness: maxima and integer sums do not depend on the order.
 //
-// Measured: 64 sequences of up to 8191 int32 keys, one token each, 32 heads of 128 over 8 (1.19 GB): 370 us, 3.2 TB/s (a copy: 4.8) — scores 162, sums 17, values 177, join 10, plan 5; the two
-// that read the cache run at 3.7 and 3.4 TB/s, held back by the cutting into digits (a torch reduction over as much reads 3.85).  4 sequences of up to 65000 int16 keys, 32 heads over 4 (187 MB): 115 us —
-// 45, 12, 40, 14, 5; one sequence of 1000 keys, 16 heads of 64 (fused, 16 workgroups): 28 us, of which 13 are fixed (a cold instruction cache, two barriers' worth of latency) and 8 go
+// Measured: 64 sequences of up to 8191 int32 keys, one token each, 32 heads of 128 over 8 (1.19 GB): 370 us, 3.2 TB/s (a copy: 4.8) — scores 161, sums 17, values 175, join 10, plan 5; the two
+// that read the cache run at 3.7 and 3.4 TB/s, near what reading alone reaches (a torch reduction over 600 MB: 3.85; the vector unit is at work for 29 % of their cycles, the matrix
+// cores for 3-6).  4 sequences of up to 65000 int16 keys, 32 heads over 4 (187 MB): 115 us — 45, 11, 40, 14, 5; one sequence of 1000 keys, 16 heads of 64 (fused, 16 workgroups): 28 us, of which 13 are fixed (a cold instruction cache, two barriers' worth of latency) and 8 go
 // by 512 keys.
 #pragma once
 #include <algorithm>

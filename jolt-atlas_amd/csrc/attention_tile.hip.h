@@ -14,11 +14,11 @@
 // 2^21 however many keys there are.
 //
 // Three passes over the scores, since the floors are taken under the final maximum and sum: maximum; e and its sum (e is held in 16 bits while the keys are few enough, HELD, or
-// taken again); product.  Bound by the vector unit, that is by recombining five sums into each score and by the two table look-ups: per step of 64 keys and 64 rows of 128 dims two
-// workgroups on a CU take 4.1, 5.9 and 3.4 thousand cycles in the passes, the vector unit busy for 51-57 % of them and the matrix cores for 38 %.  Six prompts of up to 6000 tokens,
-// 32 heads of 128 over 8 (295 GFLOP of exact products, 24 i8 products for two of them): 1.87 ms, 158 TFLOP/s, 1.7-1.9 POP/s in int8, where a library's int8 product of
-// 8192^3 reaches 2.2.  130 new tokens for each of some of 12 sequences over up to 5001 keys (186 MB, 24 GFLOP): 562 us, 70 of them the digit planes (k_attn_planes, 4.6 TB/s read and
-// written); the rest is the longest sequence's tile, three passes one after the other.
+// taken again); product.  Bound by the vector unit (recombining five sums into each score, two table look-ups) and the matrix cores together: of the cycles in which a CU has
+// waves, the vector unit is at work for 51 % and the matrix cores for 42 %.  One prompt of 6000 tokens beside five of at most 31, 32 heads of 128 over 8 (295 GFLOP of
+// exact products, 24 i8 products for two of them): 1.79-1.93 ms, by the card; 153-165 TFLOP/s, 1.8-2.0 POP/s in int8, where a library's int8 product of
+// 8192^3 reaches 2.2-2.3.  Up to 130 new tokens for each of 12 sequences over up to 5001 keys (186 MB, 24 GFLOP): 562 us, 69 of them the digit planes (k_attn_planes, 4.6 TB/s read and
+// written); the rest is the longest sequences' tiles, three passes one after the other, while the other workgroups have run out of work.
 // Measured and dropped: 3 waves per SIMD (168 registers: spills, 2.6 ms), a raised wave priority around the products (none), the look-ups of 16 scores read together before
 // the first product (spills, 2 % slower).
 #pragma once

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void k_kv_write(WriteArgs W) {
 }
 
 // ---- the plan.  need_i = ceil((c_i + n_i) / B) - ceil(c_i / B) blocks; P_i their exclusive prefix sum over the requests, R the blocks given back: block t of request i is
-// stack[n_free + R - 1 - P_i - t].  Bound by latency: 64 single tokens 9 us (a launch in a graph takes 8), 4000 requests 27-33 us, which is the one workgroup that
+// stack[n_free + R - 1 - P_i - t].  Bound by latency: 64 single tokens 11 us (10 of them the kernel), 4000 requests 27 + 6 us, which is the one workgroup that
 // adds them up, 1024 at a time (2.5 MB are touched: 0.5 us).
 struct PlanArgs {
     const int32_t *have, *fresh;
