@@ -689,6 +689,52 @@ def test_offsets_that_make_no_sense_stay_inside(atlas, cu):
             intact(w, size)
 
 
+@pytest.mark.parametrize("H,KV,d", [(4, 2, 64), (8, 1, 128), (2, 2, 256), (6, 2, 36), (40, 1, 16)])
+@pytest.mark.parametrize("cu", [[0, 60, 60, 101], [0, 2, 3, 4], [0, 101, 30, 101], [101, 0, 101, 7]])
+def test_a_call_stays_inside_what_it_needs(atlas, H, KV, d, cu):
+    """a workspace may be smaller than the size functions' (they cover smaller calls too), down to what the call's own path needs: no byte behind that is touched"""
+    import jolt_atlas_amd.attention as T
+    rng = np.random.default_rng(d)
+    at = T.Attention(H, KV, d, 2048)
+    c = Dev(np.array(cu, np.int32))
+
+    def least(call, most):
+        lo, hi = 0, most                         # the smallest that is not refused
+        while lo < hi:
+            mid = (lo + hi) // 2
+            try:
+                call(Dev(np.empty(0, np.uint8), whole, 4096, (mid,), (1,)))
+                hi = mid
+            except atlas.AtlasError as e:
+                assert "workspace" in str(e)
+                lo = mid + 1
+        return lo
+
+    def check(call, most):
+        nonlocal whole
+        w = workspace(most + 8192)
+        whole = w.buf
+        size = least(call, most)
+        assert 0 < size <= most
+        ok(hip().hipDeviceSynchronize())
+        w = workspace(size + 8192)
+        call(w.view(4096, (size,), (1,)))
+        x = w.numpy()
+        assert (x[:4096] == 0xA5).all() and (x[4096 + size:] == 0xA5).all()
+
+    whole = None
+    for rows in (101, 2100, 16500):
+        q, k, out = (Dev(np.zeros((rows, h, d), np.int32)) for h in (H, KV, H))
+        check(lambda ws: at.prompt(q, k, k, c, out, ws), at.prompt_workspace_bytes(3, rows))
+    ck = values(rng, (6, KV, 16, d))
+    cache = T.KVCache(Dev(ck), Dev(ck))
+    for rows in (4, 101):
+        q, out = (Dev(np.zeros((rows, H, d), np.int32)) for _ in range(2))
+        for cols in (4, 80, 300, 1040):
+            table, lens = Dev(rng.integers(-2, 8, size=(3, cols)).astype(np.int32)), Dev(np.array([cols * 16, 70, 2 ** 31 - 1], np.int32))
+            check(lambda ws: at.cached(q, c, lens, cache, table, out, ws), at.cached_workspace_bytes(3, rows, cache, cols))
+
+
 @pytest.mark.parametrize("d", [32, 128])
 def test_every_kernel_captured(atlas, d):
     """tiles, tiles of long sequences and the split path inside one graph, replayed over changed inputs"""
