@@ -782,6 +782,69 @@ def test_every_kernel_captured(atlas, d):
     ok(h.hipStreamDestroy(st))
 
 
+@pytest.mark.parametrize("cols", [16, 200])
+def test_a_whole_step_captured(atlas, cols):
+    """the plan, the write and the attention with its question about the mask in one graph, replayed step by step over new lengths, keys and queries"""
+    import jolt_atlas_amd.attention as T
+    h, rng = hip(), np.random.default_rng(cols)
+    H, KV, d, B, n_blocks, cap, mul, fill = 4, 2, 64, 8, 60, 70, 2048, -(8 << 14)
+    total = [100, 61, 90]
+    data = [tuple(values(rng, (t, x, d), 0.6) for x in (H, KV, KV)) for t in total]
+    whole = [prompt(q, k, v, [len(q)], mul) for q, k, v in data]
+    at, pager = T.Attention(H, KV, d, mul, mask_fill=fill, mask_tokens=64), T.Pager(B, n_blocks)
+    i32 = lambda x: Dev(np.asarray(x, np.int32))  # noqa: E731
+    cache = T.KVCache(*(Dev(np.zeros((n_blocks, KV, B, d), np.int32)) for _ in range(2)))
+    have, new, table, free, n_free = i32([0] * 3), i32([0] * 3), i32(np.full((3, cols), -1)), i32(rng.permutation(n_blocks)), i32([n_blocks])
+    cu, lens, slots, positions, status, told, narrow = i32([0] * 4), i32([0] * 3), Dev(np.zeros(cap, np.int64)), i32([0] * cap), i32([0]), i32([0]), i32([0])
+    rows, out = [Dev(np.zeros((cap, x, d), np.int32)) for x in (H, KV, KV)], Dev(np.zeros((cap, H, d), np.int32))
+    wp, wa = workspace(pager.workspace_bytes(3, cap)), workspace(at.cached_workspace_bytes(3, cap, cache, cols))
+    up = lambda dev, x: ok(h.hipMemcpy(dev.buf.p, np.ascontiguousarray(x).ctypes.data_as(C.c_void_p), C.c_size_t(x.nbytes), C.c_int(1)))  # noqa: E731
+    st, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    ok(h.hipStreamCreateWithFlags(C.byref(st), C.c_uint(1)))
+    ok(h.hipDeviceSynchronize())
+    ok(h.hipStreamBeginCapture(st, C.c_int(0)))
+    pager.plan(have, new, table, free, n_free, n_free, cu, lens, slots, positions, status, wp, stream=st.value)
+    cache.write(rows[1], rows[2], slots, narrow, stream=st.value)
+    at.cached(rows[0], cu, lens, cache, table, out, wa, stream=st.value, status=told)
+    ok(h.hipStreamEndCapture(st, C.byref(graph)))
+    ok(h.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)))
+    now, seen = [0] * 3, set()
+    for step in ([20, 0, 1], [1, 1, 1], [30, 10, 29], [0, 50, 1], [1, -1, 1], [48, 0, 22], [0, 0, 0], [0, 61, 9]):
+        hrows, want, first, expect = [np.zeros((cap, x, d), np.int32) for x in (H, KV, KV)], np.full((cap, H, d), MARK, np.int32), 0, False
+        for i, f in enumerate(step):
+            if f < 0:
+                now[i] = 0
+                continue
+            for x, src in zip(hrows, data[i]):
+                x[first:first + f] = src[now[i]:now[i] + f]
+            want[first:first + f] = whole[i][now[i]:now[i] + f]
+            q, k, _ = data[i]
+            expect |= mask_weighs(q[now[i]:now[i] + f], k, list(range(now[i] + 1, now[i] + f + 1)), list(range(now[i], now[i] + f)), mul, fill, 64)
+            now[i] += f
+            first += f
+        had = lens.numpy()                       # a request that ends brings the tokens it has
+        up(have, np.array([had[i] if f < 0 else now[i] - f for i, f in enumerate(step)], np.int32))
+        up(new, np.array(step, np.int32))
+        for dev, x in zip(rows, hrows):
+            up(dev, x)
+        up(out, np.full((cap, H, d), MARK, np.int32))
+        up(told, np.zeros(1, np.int32))
+        ok(h.hipDeviceSynchronize())
+        ok(h.hipGraphLaunch(exe, st))
+        ok(h.hipDeviceSynchronize())
+        assert status.numpy()[0] == 0 and narrow.numpy()[0] == 0 and lens.numpy().tolist() == now
+        assert np.array_equal(out.numpy(), want), step
+        assert told.numpy()[0] == (T.MASK_WEIGHS if expect else 0), step
+        seen.add(expect)
+        assert n_free.numpy()[0] == n_blocks - sum(-(-n // B) for n in now)
+        x = values(rng, (30, H, d)), values(rng, (30, KV, d)), values(rng, (30, KV, d))          # eager work between the replays
+        assert np.array_equal(run_prompt(atlas, *x, [30], mul, pads=(0,)), prompt(*x, [30], mul))
+    assert seen == {False, True}
+    ok(h.hipGraphExecDestroy(exe))
+    ok(h.hipGraphDestroy(graph))
+    ok(h.hipStreamDestroy(st))
+
+
 def test_pointers_that_are_no_device_memory(atlas):
     import jolt_atlas_amd.attention as T
     at = T.Attention(1, 1, 4)
