@@ -861,13 +861,14 @@ int atlas_verify_graph(atlas_graph_t g, const atlas_hyperkzg_vk_t *vk, const int
  *     e = (HI[z >> 9] LO[z & 511]) >> 14;  w = 2^28 / sum_j e;  p = (e w) >> 14;  out = clamp((sum_j p v) >> 14)
  * with the digit tables of SoftmaxLastAxis (atlas-onnx-tracer/src/ops/softmax.rs:74-269), floor shifts and clamps to 32 bits
  * (ops/einsum.rs:34-213).  Masked keys carry no weight here.  In a graph they carry none while its mask fill lies 169985 or more (10.4) below every row's
- * maximum; a fill of -8 or -10, as graphs have it, does so for some inputs and not for others, and only for the rows of which it holds are the two the
- * same (atlas_attn_prompt_masked, atlas_attn_cached_masked tell).  A row that sees no key is 0.  Any int32 value is computed exactly (sums wrap modulo 2^64, as the graph's do); operands in [-8421504, 8355711]
- * with |q| |k| head_dim < 2^44 take the matrix cores (trained models stay far below: 2^18 is 16.0), rows beyond that a 64-bit path that is ~100 times slower.
+ * maximum; a fill of -8 or -10, as graphs have it, does so for some inputs and not for others, and only rows of which it holds are sure to be the trace's
+ * (atlas_attn_prompt_masked, atlas_attn_cached_masked tell).  A row that sees no key is 0.  Any int32 value is computed exactly (sums wrap modulo 2^64, as
+ * the graph's do); operands in [-8421504, 8355711] with |q| |k| head_dim at most 2^44, each rounded up to a power of two, take the matrix cores (trained models
+ * stay far below: 2^18 is 16.0), rows beyond that a 64-bit path that is ~100 times slower.
  *
  * These entry points enqueue and return: no allocation, no wait, no state between calls, so they can be captured into HIP graphs.  `stream` is the
- * caller's hipStream_t; NULL = the library stream, ATLAS_STREAM_DEFAULT = HIP's default stream.  Lengths, tables and slots are read on the
- * device when the launches run.  All pointers are device memory of the calling thread's device (atlas_init / atlas_init_thread).  A workspace
+ * caller's hipStream_t; NULL = the library stream (non-blocking: no other stream waits for it or is waited for by it), ATLAS_STREAM_DEFAULT = HIP's default
+ * stream.  Lengths, tables and slots are read on the device when the launches run.  All pointers are device memory of the calling thread's device (atlas_init / atlas_init_thread).  A workspace
  * (16-byte aligned) belongs to one call in flight: two streams, or two captured graphs that may run at once, need one each.  Its size goes by the
  * arguments, not by the lengths on the device: a table of many columns costs atlas_attn_cached the room for max_blocks * block_size keys a sequence.  The sizes never
  * decrease: a workspace for a server's largest step serves every step of no more sequences, tokens and columns.  A size of 0: no call takes these arguments. */
